@@ -560,6 +560,122 @@ int tlmg_decode_attention(int mode, int kv_dt, const float *q, const void *k_pag
 int tlmg_kv_write(int kv_dt, const float *k, const float *v, void *k_pages, void *v_pages, int n_pages,
                   int32_t page_id, int page_size, int pos, int KV, int hd, void *stream);
 
+/* ---- 8-bit KV cache: append, attention, eviction -------------------------
+ * No counterpart in the reference (its KV is f32). One layer's K and V rows
+ * are held as 8-bit codes in the page pools of the section above,
+ * [n_pages][KV][page][hd], with one f32 scale d per `block` consecutive rows
+ * of a head, [n_pages][KV][page / block]: a row's values are code * d. A block
+ * holding x is stored with d = max(max |x|, 2^-100) * (1 / Q) and codes
+ * round-to-nearest-even(x / d), all in f32: TLMG_KV8_INT8 int8 codes, Q = 127;
+ * TLMG_KV8_E4M3 8-bit floats (sign, 4 exponent, 3 mantissa bits), Q = 448. A
+ * block that holds a NaN or an infinity gets the scale NaN and codes 0.
+ *
+ * Rows and positions. Row t of a sequence is row t % page of page
+ * page_table[t / page]. A row's position (what masks and distances go by) is
+ * t, or, with `pos`, the entry of the pool pos [n_pages][KV][page]: after an
+ * eviction every head keeps rows of other positions. Positions are >= 0.
+ *
+ * All pointers are DEVICE memory; calls are asynchronous on `stream`; the
+ * structs are read before the call returns. */
+enum { TLMG_KV8_INT8 = 1, TLMG_KV8_E4M3 = 2 };
+typedef struct {
+    void    *k, *v;                 /* code pools, 16-byte aligned */
+    float   *k_scale, *v_scale;     /* scale pools */
+    int32_t *pos;                   /* position pool or NULL */
+    int32_t  fmt;                   /* TLMG_KV8_INT8 or TLMG_KV8_E4M3 */
+    int32_t  n_pages, KV, page;     /* page: a power of two, 1 .. 65536 */
+    int32_t  block;                 /* rows per scale: a power of two, at most page and 256 */
+    int32_t  hd;                    /* 64, 128 or 256 */
+} tlmg_kv8;
+
+/* A batch of sequences with new tokens. Sequence s has kv_len[s] rows, the
+ * last n = q_start[s + 1] - q_start[s] of them new; its tokens are rows
+ * q_start[s] .. of the token-major buffers (total_q tokens in all). max_q and
+ * max_kv bound n and kv_len on the host (they size the launch). A sequence
+ * whose device-side lengths break 0 <= n <= max_q, n <= kv_len <= max_kv,
+ * kv_len <= table_stride * page or the bounds of total_q is not followed:
+ * appends skip it, attention returns NaN for its tokens. A page-table entry
+ * outside [0, n_pages) is not dereferenced: rows on it are not written, and a
+ * query that sees one returns NaN. */
+typedef struct {
+    const int32_t *page_table;      /* [n_seq][table_stride] */
+    const int32_t *q_start;         /* [n_seq + 1] */
+    const int32_t *kv_len;          /* [n_seq] */
+    const int32_t *q_pos;           /* [total_q] positions of the tokens, or NULL: their row numbers */
+    int32_t n_seq, table_stride, total_q, max_q, max_kv;
+} tlmg_kv8_batch;
+
+/* Stores the new tokens' K and V rows: x_dt TLMG_DT_F32, _F16 or _BF16,
+ * k / v [total_q][KV][hd] with x_stride elements from token to token (0 =
+ * KV * hd; 16-byte aligned rows). Where the first new row continues a block
+ * begun earlier, the block's scale becomes max(old, the new rows' d) and
+ * its old rows are rounded again from code * old scale. With a position pool
+ * the tokens' positions are stored too. */
+int tlmg_kv8_append(const tlmg_kv8 *c, const tlmg_kv8_batch *b, int x_dt, const void *k, const void *v,
+                    int64_t x_stride, void *stream);
+
+/* Reads rows back as f32: rows row0[s] .. of sequence s go to rows
+ * start[s] .. start[s + 1] - 1 of k / v [total][KV][hd] (start [n_seq + 1],
+ * start[n_seq] = total). Rows on a bad page or past the table read as NaN. */
+int tlmg_kv8_read(const tlmg_kv8 *c, int n_seq, const int32_t *page_table, int table_stride, const int32_t *row0,
+                  const int32_t *start, int total, float *k, float *v, void *stream);
+
+/* How a score is formed and which keys a query sees. With z = scale * q.k:
+ * softcap > 0: z = softcap * tanh(z / softcap); slopes: z -= slopes[h] *
+ * |q_pos - k_pos|. A query sees a key iff their documents are the same (doc
+ * given: doc[s * doc_stride + position], -1 outside the table) and either
+ * k_pos < prefix[s] (prefix given) or all of: causal off or k_pos <= q_pos;
+ * window 0 or q_pos - k_pos < window. A query that sees no key returns 0
+ * with lse -inf. What a masked key's row or scale holds has no effect. */
+typedef struct {
+    float scale;                    /* 0: 1 / sqrt(hd) */
+    float softcap;                  /* 0: none */
+    const float   *slopes;          /* [H] or NULL */
+    const int32_t *prefix;          /* [n_seq] or NULL */
+    const int32_t *doc;             /* [n_seq][doc_stride] or NULL */
+    int32_t doc_stride, causal, window;
+} tlmg_kv8_score;
+
+/* Attention of the batch's tokens over their sequences' rows: q [total_q][H]
+ * [hd] of q_dt (F32, F16 or BF16; q_stride elements from token to token, 0 =
+ * H * hd, 16-byte aligned rows) -> out [total_q][H][hd] of q_dt and, where
+ * not NULL, lse f32 [total_q][H] = log sum exp of the visible scores. H is a
+ * multiple of KV, at most 16 query heads per KV head. Sums and softmax
+ * statistics are f32; f32 queries and probabilities enter the tensor cores
+ * as two f16 terms (22 bits), 16-bit ones as one.
+ *
+ * weights (may be NULL; max_q <= 64): weights[s][kv][row] += the sum of the
+ * softmax weights that the call's tokens and the KV head's query heads gave
+ * the row, w_stride >= max_kv floats per (sequence, head). One thread owns an
+ * entry: the sums are the same in every run.
+ *
+ * work: scratch of tlmg_kv8_attend_work_bytes(...), 16-byte aligned; calls
+ * that may overlap need scratch of their own. */
+size_t tlmg_kv8_attend_work_bytes(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const tlmg_kv8_score *s, int H, int q_dt,
+                                  int with_weights);
+int tlmg_kv8_attend(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const tlmg_kv8_score *s, int H, int q_dt, const void *q,
+                    int64_t q_stride, void *out, float *lse, float *weights, int64_t w_stride, void *work,
+                    size_t work_bytes, void *stream);
+
+/* Chooses the rows to keep of every (sequence, head): all of them where
+ * kv_len[s] <= n_keep, else the first `sink`, the last `recent` and, of the
+ * others, those of the largest weights (a NaN counts as the lowest, ties go to
+ * the lowest row). rows int32 [n_seq][KV][n_keep]: ascending, -1 after the
+ * last; lens[s] = min(kv_len[s], n_keep). 0 <= sink + recent <= n_keep. */
+int tlmg_kv8_select(int n_seq, int KV, const int32_t *kv_len, int max_kv, const float *weights, int64_t w_stride,
+                    int n_keep, int sink, int recent, int32_t *rows, int32_t *lens, void *stream);
+
+/* Gathers the chosen rows into other pages (of c itself or of another cache
+ * with the same KV and hd): row j of (s, kv) in dst_table's pages becomes
+ * row rows[s][kv][j] of page_table's, stored again by dst's blocks and format.
+ * No page of dst_table may be one that page_table names. dst->pos (which must
+ * exist) receives the rows' positions; weights_out [n_seq][KV][wo_stride]
+ * (may be NULL) the rows' weights, 0 elsewhere. Entries of rows outside
+ * [0, kv_len[s]) are skipped. */
+int tlmg_kv8_compact(const tlmg_kv8 *c, const tlmg_kv8 *dst, int n_seq, const int32_t *page_table, int table_stride,
+                     const int32_t *kv_len, const int32_t *dst_table, int dst_stride, const int32_t *rows, int n_keep,
+                     const float *weights, int64_t w_stride, float *weights_out, int64_t wo_stride, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,6 +70,12 @@ _SIGS = {
     "tlmg_attention_work_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
     "tlmg_decode_attention": (_I, [_I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _SZ, _P, _P]),
     "tlmg_kv_write": (_I, [_I, _P, _P, _P, _P, _I, C.c_int32, _I, _I, _I, _I, _P]),
+    "tlmg_kv8_append": (_I, [_P, _P, _I, _P, _P, _I64, _P]),
+    "tlmg_kv8_read": (_I, [_P, _I, _P, _I, _P, _P, _I, _P, _P, _P]),
+    "tlmg_kv8_attend_work_bytes": (_SZ, [_P, _P, _P, _I, _I, _I]),
+    "tlmg_kv8_attend": (_I, [_P, _P, _P, _I, _I, _P, _I64, _P, _P, _P, _I64, _P, _SZ, _P]),
+    "tlmg_kv8_select": (_I, [_I, _I, _P, _I, _P, _I64, _I, _I, _I, _P, _P, _P]),
+    "tlmg_kv8_compact": (_I, [_P, _P, _I, _P, _I, _P, _P, _I, _P, _I, _P, _I64, _P, _I64, _P]),
     "tlmg_qmv_host": (None, [_I, _P, _SZ, _P, _P, _I64, _I64]),
     "tlmg_qdot_host": (_F, [_I, _P, _P, _I64, _P]),
     "tlmg_open": (_I, [C.POINTER(Geom), _I, C.POINTER(_P)]),

@@ -1,0 +1,443 @@
+// tlmg_kv8.cu - the 8-bit KV cache's append, read-back and eviction.
+//
+// A block (`block` consecutive rows of one head) is stored with one scale
+// d = max(amax, 2^-100) * (1 / Q) and codes round(x / d); products and
+// divisions are IEEE f32 and the rounding is to nearest even, so that codes are
+// a function of the inputs alone. One warp owns one block of K or of V: it takes the maximum
+// over the block's rows, then rounds them in a second pass that finds the
+// rows in L1. All of these kernels move a few bytes per element and are bound
+// by HBM or, for one token per sequence, by the launch.
+#include <algorithm>
+
+#include "tlmg_dev.cuh"
+#include "tlmg_internal.h"
+#include "tlmg_kv8.cuh"
+
+namespace tlmg {
+
+static int log2i(int v) {
+    int l = 0;
+    while ((1 << l) < v) l++;
+    return l;
+}
+
+int kv8_check(const char *who, const tlmg_kv8 *c) {
+    if (!c) return set_error(TLMG_EINVAL, "%s: null cache", who);
+    if (c->fmt != TLMG_KV8_INT8 && c->fmt != TLMG_KV8_E4M3)
+        return set_error(TLMG_EINVAL, "%s: format %d (int8 1 or e4m3 2)", who, c->fmt);
+    if (c->hd != 64 && c->hd != 128 && c->hd != 256)
+        return set_error(TLMG_EINVAL, "%s: head_dim %d (64, 128 or 256)", who, c->hd);
+    if (c->page <= 0 || c->page > (1 << 16) || (c->page & (c->page - 1)) || c->n_pages <= 0 || c->KV <= 0)
+        return set_error(TLMG_EINVAL, "%s: page %d (a power of two up to 65536), %d pages, %d KV heads", who, c->page,
+                         c->n_pages, c->KV);
+    if (c->block <= 0 || c->block > 256 || c->block > c->page || (c->block & (c->block - 1)))
+        return set_error(TLMG_EINVAL, "%s: block %d (a power of two, at most the page of %d rows and 256)", who, c->block,
+                         c->page);
+    if ((int64_t)c->n_pages * c->KV > (int64_t)0xFFFFFFFEu / c->page)
+        return set_error(TLMG_ERANGE, "%s: %d pages x %d heads x %d rows pass 2^32 rows", who, c->n_pages, c->KV, c->page);
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return set_error(TLMG_EINVAL, "%s: null pool", who);
+    if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u)
+        return set_error(TLMG_EINVAL, "%s: code pools must be 16-byte aligned", who);
+    if (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale | (uintptr_t)c->pos) & 3u)
+        return set_error(TLMG_EINVAL, "%s: scale and position pools must be 4-byte aligned", who);
+    return TLMG_OK;
+}
+
+int kv8_check_batch(const char *who, const tlmg_kv8_batch *b) {
+    if (!b || !b->page_table || !b->q_start || !b->kv_len) return set_error(TLMG_EINVAL, "%s: null batch array", who);
+    if (b->n_seq <= 0 || b->n_seq > 65535 || b->table_stride <= 0 || b->total_q < 0 || b->max_q < 0 || b->max_kv < 0)
+        return set_error(TLMG_EINVAL, "%s: %d sequences (1 .. 65535), table stride %d, %d tokens, max_q %d, max_kv %d", who,
+                         b->n_seq, b->table_stride, b->total_q, b->max_q, b->max_kv);
+    return TLMG_OK;
+}
+
+Kv8View kv8_view(const tlmg_kv8 *c) {
+    return Kv8View{ (uint8_t *)c->k, (uint8_t *)c->v, c->k_scale, c->v_scale, c->pos, c->n_pages, c->KV, c->hd,
+                    log2i(c->page), log2i(c->block) };
+}
+
+namespace {
+
+// amax of |v| that a NaN survives (fmaxf would drop it): +inf and NaN both end as "not finite"
+__device__ __forceinline__ float amax4(float a, float4 v) {
+    const float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+    const bool nan = (v.x != v.x) | (v.y != v.y) | (v.z != v.z) | (v.w != v.w);
+    return fmaxf(a, nan ? INFINITY : m);
+}
+__device__ __forceinline__ float warp_max(float a) {
+    for (int o = 16; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+    return a;
+}
+// The scale of a block from its amax; NaN where the block is not finite.
+template <int FMT> __device__ __forceinline__ float scale_of(float amax) {
+    return amax < INFINITY ? __fmul_rn(fmaxf(amax, KV8_FLOOR), 1.0f / kv8_qmax<FMT>()) : __uint_as_float(0x7FC00000u);
+}
+template <int FMT> __device__ __forceinline__ uint32_t codes4(float4 v, float d) {
+    if (!(d == d)) return 0u;
+    return kv8_code<FMT>(__fdiv_rn(v.x, d)) | (kv8_code<FMT>(__fdiv_rn(v.y, d)) << 8) |
+           (kv8_code<FMT>(__fdiv_rn(v.z, d)) << 16) | (kv8_code<FMT>(__fdiv_rn(v.w, d)) << 24);
+}
+template <int FMT> __device__ __forceinline__ float4 values4(uint32_t w, float d) {
+    return make_float4(__fmul_rn(kv8_value<FMT>(w & 255u), d), __fmul_rn(kv8_value<FMT>((w >> 8) & 255u), d),
+                       __fmul_rn(kv8_value<FMT>((w >> 16) & 255u), d), __fmul_rn(kv8_value<FMT>(w >> 24), d));
+}
+
+constexpr int AP_WARPS = 4;
+
+// grid (ceil(blocks a sequence can touch * 2 KV / 4 warps), n_seq)
+template <int FMT, typename XT>
+__global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_append(const Kv8View c, const tlmg_kv8_batch b,
+                                                              const XT *__restrict__ xk, const XT *__restrict__ xv,
+                                                              int64_t x_stride) {
+    const int s = blockIdx.y, lane = threadIdx.x & 31;
+    Kv8Seq q;
+    if (!kv8_seq(b, c.lp, s, q) || q.n == 0) return;
+    const int unit = blockIdx.x * AP_WARPS + (threadIdx.x >> 5);
+    const int is_v = unit & 1, kv = (unit >> 1) % c.KV, t_new = q.L - q.n;
+    const int64_t blk = (int64_t)(t_new >> c.lb) + (unit >> 1) / c.KV;
+    if (blk << c.lb >= q.L) return;
+    const int t0 = (int)(blk << c.lb), t1 = min(q.L, t0 + (1 << c.lb)), ta = max(t0, t_new);
+    const int32_t e = b.page_table[(size_t)s * b.table_stride + (t0 >> c.lp)];
+    if (!c.ok(e)) return;
+    const uint32_t r0 = c.row(e, kv, t0);
+    uint8_t *codes = (is_v ? c.v : c.k) + (size_t)r0 * c.hd;
+    float *scale = (is_v ? c.vs : c.ks) + (r0 >> c.lb);
+    const XT *x = (is_v ? xv : xk) + (q.q0 + (int64_t)(ta - t_new)) * x_stride + (int64_t)kv * c.hd;
+    const int per = c.hd >> 2, lper = 31 - __clz(per), n4 = (t1 - ta) << lper;
+    float a = 0.0f;
+    for (int i = lane; i < n4; i += 32) a = amax4(a, kv8_ld4(x + (int64_t)(i >> lper) * x_stride + 4 * (i & (per - 1))));
+    float d = scale_of<FMT>(warp_max(a));
+    if (t0 < ta) {   // rows of an earlier call
+        const float old = *scale;
+        if (!(old <= d)) d = d == d ? old : d;     // max(old, d); a NaN of either side stays
+        if (!(old == d)) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(codes);
+            for (int i = lane; i < (ta - t0) << lper; i += 32) w[i] = codes4<FMT>(values4<FMT>(w[i], old), d);
+        }
+        __syncwarp();                              // every lane has read the old scale
+    }
+    if (lane == 0) *scale = d;
+    uint32_t *w = reinterpret_cast<uint32_t *>(codes + (size_t)(ta - t0) * c.hd);
+    for (int i = lane; i < n4; i += 32)
+        w[i] = codes4<FMT>(kv8_ld4(x + (int64_t)(i >> lper) * x_stride + 4 * (i & (per - 1))), d);
+    if (c.pos && !is_v)
+        for (int t = ta + lane; t < t1; t += 32)
+            c.pos[r0 + (uint32_t)(t - t0)] = b.q_pos ? b.q_pos[q.q0 + (t - t_new)] : t;
+}
+
+// One warp per (output row, KV head).
+template <int FMT>
+__global__ void __launch_bounds__(256) k_kv8_read(const Kv8View c, int n_seq, const int32_t *__restrict__ table,
+                                                  int stride, const int32_t *__restrict__ row0,
+                                                  const int32_t *__restrict__ start, int total, float *__restrict__ ko,
+                                                  float *__restrict__ vo) {
+    const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (unit >= (int64_t)total * c.KV) return;
+    const int o = (int)(unit / c.KV), kv = (int)(unit - (int64_t)o * c.KV);
+    int lo = 0, hi = n_seq;                        // the last sequence that starts at or before o
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (start[m] <= o) lo = m;
+        else hi = m;
+    }
+    const int64_t t = (int64_t)row0[lo] + (o - start[lo]);
+    int32_t e = -1;
+    if (t >= 0 && (t >> c.lp) < stride) e = table[(size_t)lo * stride + (t >> c.lp)];
+    const bool ok = c.ok(e);
+    const uint32_t r = ok ? c.row(e, kv, (int)t) : 0u;
+    const float nan = __uint_as_float(0x7FC00000u), dk = ok ? c.ks[r >> c.lb] : nan, dv = ok ? c.vs[r >> c.lb] : nan;
+    const uint32_t *wk = reinterpret_cast<const uint32_t *>(c.k + (size_t)r * c.hd),
+                   *wv = reinterpret_cast<const uint32_t *>(c.v + (size_t)r * c.hd);
+    for (int i = lane; i < c.hd >> 2; i += 32) {
+        kv8_st4(ko + unit * c.hd + 4 * i, values4<FMT>(wk[i], dk));
+        kv8_st4(vo + unit * c.hd + 4 * i, values4<FMT>(wv[i], dv));
+    }
+}
+
+// ---- eviction ----------------------------------------------------------------
+// The order of weights as unsigned keys: larger weight, larger key; -0 is 0, a NaN is the lowest (key 0).
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    if (w != w) return 0u;
+    const uint32_t u = __float_as_uint(w + 0.0f);
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+constexpr int SEL_THREADS = 1024;
+constexpr int SEL_BINS = 2048;
+
+// One CTA per (sequence, KV head). The m-th largest key of the rows between
+// the first `sink` and the last `recent` is found digit by digit (11, 11 and
+// 10 bits, a shared-memory count of each digit), then one ordered pass
+// writes the rows above it and as many rows equal to it, lowest first, as m
+// leaves.
+__global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_t *__restrict__ kv_len, int max_kv,
+                                                            const float *__restrict__ weights, int64_t w_stride,
+                                                            int n_keep, int sink, int recent, int32_t *__restrict__ rows,
+                                                            int32_t *__restrict__ lens) {
+    __shared__ uint32_t hist[SEL_BINS];
+    __shared__ uint32_t wsum[2][32];
+    __shared__ uint32_t pick_s, left_s;
+    const int kv = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int L = min(max(kv_len[s], 0), max_kv);
+    int32_t *out = rows + ((size_t)s * KV + kv) * n_keep;
+    const float *w = weights + ((size_t)s * KV + kv) * w_stride;
+    if (kv == 0 && tid == 0 && lens) lens[s] = min(L, n_keep);
+    if (L <= n_keep) {
+        for (int j = tid; j < n_keep; j += SEL_THREADS) out[j] = j < L ? j : -1;
+        return;
+    }
+    const int lo = sink, hi = L - recent, m = n_keep - sink - recent;
+    for (int j = tid; j < sink; j += SEL_THREADS) out[j] = j;
+    for (int j = tid; j < recent; j += SEL_THREADS) out[n_keep - recent + j] = hi + j;
+    if (m == 0) return;
+    uint32_t prefix = 0, left = (uint32_t)m;   // key bits found so far; rows still to take below them
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+        for (int i = tid; i < bins; i += SEL_THREADS) hist[i] = 0;
+        __syncthreads();
+        for (int t0 = lo; t0 < hi; t0 += SEL_THREADS) {
+            const int t = t0 + tid;
+            const uint32_t key = t < hi ? weight_key(w[t]) : 0u;
+            const bool in = t < hi && (pass == 0 || (key >> (shift + (pass == 2 ? 10 : 11))) == prefix);
+            const uint32_t bin = (key >> shift) & (uint32_t)(bins - 1);
+            // equal digits of a warp are counted once: accumulated weights hold many equal values
+            const uint32_t act = __ballot_sync(0xFFFFFFFFu, in);
+            if (in) {
+                const uint32_t peers = __match_any_sync(act, bin);
+                if (lane == __ffs(peers) - 1) atomicAdd(&hist[bin], (uint32_t)__popc(peers));
+            }
+        }
+        __syncthreads();
+        // suffix counts: thread i covers the bins / 1024 bins from the top
+        const int per = bins / SEL_THREADS;
+        uint32_t c0 = hist[bins - 1 - per * tid], c1 = per == 2 ? hist[bins - 2 - per * tid] : 0u, sum = c0 + c1;
+        uint32_t inc = sum;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) wsum[0][warp] = inc;
+        __syncthreads();
+        if (warp == 0) {
+            uint32_t v = wsum[0][lane];
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+                if (lane >= o) v += u;
+            }
+            wsum[1][lane] = v;
+        }
+        __syncthreads();
+        const uint32_t upto = inc + (warp ? wsum[1][warp - 1] : 0u), before = upto - sum;
+        if (before < left && upto >= left) {       // exactly one thread
+            const bool first = before + c0 >= left;
+            pick_s = (uint32_t)(bins - 1 - per * tid) - (first ? 0u : 1u);
+            left_s = left - before - (first ? 0u : c0);
+        }
+        __syncthreads();
+        prefix = (prefix << (pass == 2 ? 10 : 11)) | pick_s;
+        left = left_s;
+        __syncthreads();
+    }
+    // prefix is now the m-th largest key; `left` rows equal to it are taken
+    uint32_t n_out = 0, n_eq = 0;
+    for (int t0 = lo; t0 < hi; t0 += SEL_THREADS) {
+        const int t = t0 + tid;
+        const uint32_t key = t < hi ? weight_key(w[t]) : 0u;
+        const bool gt = t < hi && key > prefix, eq = t < hi && key == prefix;
+        const uint32_t bg = __ballot_sync(0xFFFFFFFFu, gt), be = __ballot_sync(0xFFFFFFFFu, eq);
+        if (lane == 0) {
+            wsum[0][warp] = __popc(bg);
+            wsum[1][warp] = __popc(be);
+        }
+        __syncthreads();
+        uint32_t g0 = n_out, e0 = n_eq, gt_all = 0, eq_all = 0;
+        {
+            const uint32_t a = wsum[0][lane], bq = wsum[1][lane];
+            uint32_t ga = lane < warp ? a : 0u, ea = lane < warp ? bq : 0u;
+            g0 += __reduce_add_sync(0xFFFFFFFFu, ga);
+            e0 += __reduce_add_sync(0xFFFFFFFFu, ea);
+            gt_all = __reduce_add_sync(0xFFFFFFFFu, a);
+            eq_all = __reduce_add_sync(0xFFFFFFFFu, bq);
+        }
+        const uint32_t below = (1u << lane) - 1u;
+        const uint32_t g = g0 + __popc(bg & below), q = e0 + __popc(be & below);   // larger / equal rows before t
+        if (gt || (eq && q < left)) out[sink + (int)(g + min(q, left))] = t;
+        n_out += gt_all;
+        n_eq += eq_all;
+        __syncthreads();
+    }
+}
+
+// One warp per (destination block, KV head, K or V).
+template <int FS, int FD>
+__global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_compact(const Kv8View c, const Kv8View d, const int32_t *__restrict__ table,
+                                                               int stride, const int32_t *__restrict__ kv_len,
+                                                               const int32_t *__restrict__ dtable, int dstride,
+                                                               const int32_t *__restrict__ rows, int n_keep,
+                                                               const float *__restrict__ weights, int64_t w_stride,
+                                                               float *__restrict__ wout, int64_t wo_stride) {
+    const int s = blockIdx.y, lane = threadIdx.x & 31;
+    const int unit = blockIdx.x * AP_WARPS + (threadIdx.x >> 5);
+    const int is_v = unit & 1, kv = (unit >> 1) % c.KV;
+    const int64_t j0 = (int64_t)((unit >> 1) / c.KV) << d.lb;
+    if (j0 >= n_keep) return;
+    const int nj = (int)min((int64_t)1 << d.lb, n_keep - j0);
+    const int L = kv_len[s];
+    const int32_t *src = rows + ((size_t)s * c.KV + kv) * n_keep + j0;
+    const int32_t de = (j0 >> d.lp) < dstride ? dtable[(size_t)s * dstride + (j0 >> d.lp)] : -1;
+    const bool dok = d.ok(de);
+    const uint32_t dr = dok ? d.row(de, kv, (int)j0) : 0u;
+    const int per = c.hd >> 2, lper = 31 - __clz(per);
+    const uint8_t *pool = is_v ? c.v : c.k;
+    const float *sc = is_v ? c.vs : c.ks;
+    // source row number of entry j, or -1; uniform over the lanes that share a row
+    auto source = [&](int j, uint32_t &r) {
+        const int32_t t = src[j];
+        if (t < 0 || t >= L || (t >> c.lp) >= stride) return false;
+        const int32_t e = table[(size_t)s * stride + (t >> c.lp)];
+        if (!c.ok(e)) return false;
+        r = c.row(e, kv, t);
+        return true;
+    };
+    float a = 0.0f;
+    bool any = false;
+    for (int i = lane; i < nj << lper; i += 32) {
+        uint32_t r;
+        if (!source(i >> lper, r)) continue;
+        any = true;
+        a = amax4(a, values4<FS>(reinterpret_cast<const uint32_t *>(pool + (size_t)r * c.hd)[i & (per - 1)], sc[r >> c.lb]));
+    }
+    any = __any_sync(0xFFFFFFFFu, any);
+    const float q = scale_of<FD>(warp_max(a));
+    if (dok && any) {
+        if (lane == 0) (is_v ? d.vs : d.ks)[dr >> d.lb] = q;
+        uint32_t *w = reinterpret_cast<uint32_t *>((is_v ? d.v : d.k) + (size_t)dr * d.hd);
+        for (int i = lane; i < nj << lper; i += 32) {
+            uint32_t r;
+            if (!source(i >> lper, r)) continue;
+            w[i] = codes4<FD>(values4<FS>(reinterpret_cast<const uint32_t *>(pool + (size_t)r * c.hd)[i & (per - 1)], sc[r >> c.lb]), q);
+        }
+    }
+    if (!is_v)
+        for (int j = lane; j < nj; j += 32) {
+            uint32_t r;
+            const bool ok = source(j, r);
+            if (ok && dok) d.pos[dr + (uint32_t)j] = c.pos ? c.pos[r] : src[j];
+            if (wout)
+                wout[((size_t)s * c.KV + kv) * wo_stride + j0 + j] =
+                    ok ? weights[((size_t)s * c.KV + kv) * w_stride + src[j]] : 0.0f;
+        }
+}
+
+int launched(const char *what) {
+    count_launch();
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? TLMG_OK : cuda_fail(e, what);
+}
+
+template <int FMT>
+void append_launch(const Kv8View &v, const tlmg_kv8_batch &b, int x_dt, const void *k, const void *x, int64_t stride,
+                   dim3 grid, cudaStream_t st) {
+    if (x_dt == TLMG_DT_F32)
+        k_kv8_append<FMT, float><<<grid, 32 * AP_WARPS, 0, st>>>(v, b, (const float *)k, (const float *)x, stride);
+    else if (x_dt == TLMG_DT_F16)
+        k_kv8_append<FMT, __half><<<grid, 32 * AP_WARPS, 0, st>>>(v, b, (const __half *)k, (const __half *)x, stride);
+    else
+        k_kv8_append<FMT, __nv_bfloat16><<<grid, 32 * AP_WARPS, 0, st>>>(v, b, (const __nv_bfloat16 *)k,
+                                                                        (const __nv_bfloat16 *)x, stride);
+}
+
+}  // namespace
+}  // namespace tlmg
+
+using namespace tlmg;
+
+extern "C" int tlmg_kv8_append(const tlmg_kv8 *c, const tlmg_kv8_batch *b, int x_dt, const void *k, const void *v,
+                               int64_t x_stride, void *stream) {
+    int rc = kv8_check("kv8_append", c);
+    if (!rc) rc = kv8_check_batch("kv8_append", b);
+    if (rc) return rc;
+    if (x_dt != TLMG_DT_F32 && x_dt != TLMG_DT_F16 && x_dt != TLMG_DT_BF16)
+        return set_error(TLMG_EINVAL, "kv8_append: row dtype %d (f32, f16 or bf16)", x_dt);
+    if (b->total_q == 0 || b->max_q == 0) return TLMG_OK;
+    if (!k || !v) return set_error(TLMG_EINVAL, "kv8_append: null pointer");
+    const int64_t es = x_dt == TLMG_DT_F32 ? 4 : 2, st = x_stride ? x_stride : (int64_t)c->KV * c->hd;
+    if (st < (int64_t)c->KV * c->hd || (st * es) % 16 || (((uintptr_t)k | (uintptr_t)v) & 15u))
+        return set_error(TLMG_EINVAL, "kv8_append: rows must be 16-byte aligned, %lld elements apart or more (stride %lld)",
+                         (long long)c->KV * c->hd, (long long)st);
+    const Kv8View view = kv8_view(c);
+    // n new rows touch at most this many blocks, whatever row they start at
+    const int64_t blocks = ((int64_t)b->max_q + c->block - 2) / c->block + 1;
+    const int64_t units = blocks * c->KV * 2;
+    if (units > INT32_MAX - 64) return set_error(TLMG_ERANGE, "kv8_append: %lld blocks", (long long)units);
+    const dim3 grid((unsigned)((units + AP_WARPS - 1) / AP_WARPS), b->n_seq);
+    if (c->fmt == TLMG_KV8_INT8) append_launch<TLMG_KV8_INT8>(view, *b, x_dt, k, v, st, grid, pick_stream(stream));
+    else append_launch<TLMG_KV8_E4M3>(view, *b, x_dt, k, v, st, grid, pick_stream(stream));
+    return launched("kv8_append launch");
+}
+
+extern "C" int tlmg_kv8_read(const tlmg_kv8 *c, int n_seq, const int32_t *page_table, int table_stride,
+                             const int32_t *row0, const int32_t *start, int total, float *k, float *v, void *stream) {
+    int rc = kv8_check("kv8_read", c);
+    if (rc) return rc;
+    if (n_seq <= 0 || table_stride <= 0 || total < 0)
+        return set_error(TLMG_EINVAL, "kv8_read: %d sequences, table stride %d, %d rows", n_seq, table_stride, total);
+    if (total == 0) return TLMG_OK;
+    if (!page_table || !row0 || !start || !k || !v) return set_error(TLMG_EINVAL, "kv8_read: null pointer");
+    if (((uintptr_t)k | (uintptr_t)v) & 15u) return set_error(TLMG_EINVAL, "kv8_read: k and v must be 16-byte aligned");
+    const int64_t grid = ((int64_t)total * c->KV + 7) / 8;
+    if (grid > INT32_MAX) return set_error(TLMG_ERANGE, "kv8_read: %d rows x %d heads", total, c->KV);
+    if (c->fmt == TLMG_KV8_INT8)
+        k_kv8_read<TLMG_KV8_INT8><<<(unsigned)grid, 256, 0, pick_stream(stream)>>>(kv8_view(c), n_seq, page_table, table_stride,
+                                                                                  row0, start, total, k, v);
+    else
+        k_kv8_read<TLMG_KV8_E4M3><<<(unsigned)grid, 256, 0, pick_stream(stream)>>>(kv8_view(c), n_seq, page_table, table_stride,
+                                                                                  row0, start, total, k, v);
+    return launched("kv8_read launch");
+}
+
+extern "C" int tlmg_kv8_select(int n_seq, int KV, const int32_t *kv_len, int max_kv, const float *weights, int64_t w_stride,
+                               int n_keep, int sink, int recent, int32_t *rows, int32_t *lens, void *stream) {
+    if (n_seq <= 0 || n_seq > 65535 || KV <= 0 || max_kv < 0 || w_stride < max_kv || n_keep <= 0 || sink < 0 ||
+        recent < 0 || (int64_t)sink + recent > n_keep)
+        return set_error(TLMG_EINVAL, "kv8_select: %d sequences x %d heads, max_kv %d, weight stride %lld, keep %d (%d first, %d last)",
+                         n_seq, KV, max_kv, (long long)w_stride, n_keep, sink, recent);
+    if (!kv_len || !weights || !rows) return set_error(TLMG_EINVAL, "kv8_select: null pointer");
+    k_kv8_select<<<dim3(KV, n_seq), SEL_THREADS, 0, pick_stream(stream)>>>(KV, kv_len, max_kv, weights, w_stride, n_keep, sink,
+                                                                          recent, rows, lens);
+    return launched("kv8_select launch");
+}
+
+extern "C" int tlmg_kv8_compact(const tlmg_kv8 *c, const tlmg_kv8 *dst, int n_seq, const int32_t *page_table,
+                                int table_stride, const int32_t *kv_len, const int32_t *dst_table, int dst_stride,
+                                const int32_t *rows, int n_keep, const float *weights, int64_t w_stride, float *weights_out,
+                                int64_t wo_stride, void *stream) {
+    int rc = kv8_check("kv8_compact", c);
+    if (!rc) rc = kv8_check("kv8_compact (destination)", dst);
+    if (rc) return rc;
+    if (c->KV != dst->KV || c->hd != dst->hd)
+        return set_error(TLMG_EINVAL, "kv8_compact: %d x %d heads into %d x %d", c->KV, c->hd, dst->KV, dst->hd);
+    if (!dst->pos) return set_error(TLMG_EINVAL, "kv8_compact: the destination needs a position pool");
+    if (n_seq <= 0 || n_seq > 65535 || table_stride <= 0 || dst_stride <= 0 || n_keep <= 0)
+        return set_error(TLMG_EINVAL, "kv8_compact: %d sequences, table strides %d and %d, %d rows", n_seq, table_stride,
+                         dst_stride, n_keep);
+    if (!page_table || !kv_len || !dst_table || !rows) return set_error(TLMG_EINVAL, "kv8_compact: null pointer");
+    if (weights_out && (!weights || wo_stride < n_keep))
+        return set_error(TLMG_EINVAL, "kv8_compact: weights_out needs weights and a stride of %d (%lld)", n_keep, (long long)wo_stride);
+    const int64_t units = ((int64_t)(n_keep + dst->block - 1) / dst->block) * c->KV * 2;
+    if (units > INT32_MAX - 64) return set_error(TLMG_ERANGE, "kv8_compact: %lld blocks", (long long)units);
+    const dim3 grid((unsigned)((units + AP_WARPS - 1) / AP_WARPS), n_seq);
+    const Kv8View a = kv8_view(c), d = kv8_view(dst);
+    cudaStream_t st = pick_stream(stream);
+#define TLMG_COMPACT(FS, FD)                                                                                              \
+    if (c->fmt == FS && dst->fmt == FD)                                                                                   \
+        k_kv8_compact<FS, FD><<<grid, 32 * AP_WARPS, 0, st>>>(a, d, page_table, table_stride, kv_len, dst_table, dst_stride, \
+                                                              rows, n_keep, weights, w_stride, weights_out, wo_stride);
+    TLMG_COMPACT(TLMG_KV8_INT8, TLMG_KV8_INT8)
+    TLMG_COMPACT(TLMG_KV8_INT8, TLMG_KV8_E4M3)
+    TLMG_COMPACT(TLMG_KV8_E4M3, TLMG_KV8_INT8)
+    TLMG_COMPACT(TLMG_KV8_E4M3, TLMG_KV8_E4M3)
+#undef TLMG_COMPACT
+    return launched("kv8_compact launch");
+}

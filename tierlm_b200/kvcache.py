@@ -1,0 +1,269 @@
+"""The 8-bit KV cache on CUDA tensors: append, attention, eviction (the
+tlmg_kv8_* calls of include/tlmg.h; no counterpart in the reference, whose KV
+is f32).
+
+One layer's K and V rows are 8-bit codes in page pools [n_pages][KV][page]
+[hd] (torch.int8, or torch.float8_e4m3fn) with one f32 scale per `block` rows
+of a head. A batch of sequences shares the pools: `Kv8Batch` holds the page
+tables, the lengths and where each sequence's new tokens sit. Calls run on
+torch's current stream; the cache keeps one scratch buffer per stream that
+it was used on.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+
+import torch
+
+from ._lib import BF16, F16, F32, TlmError, check, load
+from .quant import _dev, stream_handle
+
+INT8, E4M3 = 1, 2
+_FMT = {torch.int8: INT8, torch.float8_e4m3fn: E4M3}
+_X_DT = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+class _Cache(C.Structure):
+    """tlmg_kv8."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pos", C.c_void_p), ("fmt", C.c_int32), ("n_pages", C.c_int32), ("KV", C.c_int32),
+                ("page", C.c_int32), ("block", C.c_int32), ("hd", C.c_int32)]
+
+
+class _Batch(C.Structure):
+    """tlmg_kv8_batch."""
+    _fields_ = [("page_table", C.c_void_p), ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("q_pos", C.c_void_p),
+                ("n_seq", C.c_int32), ("table_stride", C.c_int32), ("total_q", C.c_int32), ("max_q", C.c_int32),
+                ("max_kv", C.c_int32)]
+
+
+class _Score(C.Structure):
+    """tlmg_kv8_score."""
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("slopes", C.c_void_p), ("prefix", C.c_void_p),
+                ("doc", C.c_void_p), ("doc_stride", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32)]
+
+
+def _i32(t: torch.Tensor | None, what: str, shape: tuple | None = None) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.int32:
+        raise TlmError(-3, f"{what} must be int32, not {t.dtype}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise TlmError(-3, f"{what} has shape {tuple(t.shape)}, not {shape}")
+    return _dev(t, what)
+
+
+def _f32(t: torch.Tensor | None, what: str, shape: tuple | None = None) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.float32:
+        raise TlmError(-3, f"{what} must be float32, not {t.dtype}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise TlmError(-3, f"{what} has shape {tuple(t.shape)}, not {shape}")
+    return _dev(t, what)
+
+
+def _rows(t: torch.Tensor, what: str, heads: int, hd: int) -> tuple[torch.Tensor, int]:
+    """[n][heads][hd] rows and their stride in elements; a copy where the
+    library cannot read them in place (heads apart, rows off 16 bytes)."""
+    if t.dtype not in _X_DT:
+        raise TlmError(-3, f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+    if t.dim() != 3 or t.shape[1:] != (heads, hd):
+        raise TlmError(-3, f"{what} has shape {tuple(t.shape)}, not [n][{heads}][{hd}]")
+    if not t.is_cuda:
+        raise TlmError(-3, f"{what} must be a CUDA tensor")
+    st = t.stride(0)
+    if t.stride(2) != 1 or t.stride(1) != hd or st < heads * hd or st * t.element_size() % 16 or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        st = heads * hd
+    return t, st
+
+
+class Kv8Batch:
+    """Sequences with new tokens: page_table int32 [n_seq][stride]; q_start
+    int32 [n_seq + 1] (sequence s's new tokens are rows q_start[s] ..
+    q_start[s + 1] - 1 of the token-major tensors); kv_len int32 [n_seq] rows
+    per sequence, the new ones last; max_q and max_kv bound the two on the
+    host; q_pos int32 [n] positions of the tokens (None: their row numbers)."""
+
+    def __init__(self, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, max_q: int, max_kv: int,
+                 q_pos: torch.Tensor | None = None):
+        if page_table.dim() != 2:
+            raise TlmError(-3, f"page_table has shape {tuple(page_table.shape)}, not [n_seq][stride]")
+        n_seq, stride = page_table.shape
+        self._keep = (page_table, q_start, kv_len, q_pos)
+        self.n_seq, self.page_table, self.kv_len, self.q_pos = n_seq, page_table, kv_len, q_pos
+        self.max_q, self.max_kv = max_q, max_kv
+        self._c = _Batch(_i32(page_table, "page_table"), _i32(q_start, "q_start", (n_seq + 1,)),
+                         _i32(kv_len, "kv_len", (n_seq,)), _i32(q_pos, "q_pos"), n_seq, stride, 0, max_q, max_kv)
+
+    def _at(self, total: int) -> _Batch:
+        if self.q_pos is not None and self.q_pos.numel() < total:
+            raise TlmError(-3, f"q_pos has {self.q_pos.numel()} entries for {total} tokens")
+        self._c.total_q = total
+        return self._c
+
+
+@dataclass(frozen=True)
+class Score:
+    """How scores are formed and masked (tlmg_kv8_score): softcap c > 0:
+    c * tanh(z / c); slopes f32 [H]: minus slopes[h] * distance; causal,
+    window, prefix int32 [n_seq] (rows below it stay visible) and doc int32
+    [n_seq][positions] (other documents are masked). scale 0: 1 / sqrt(hd)."""
+    scale: float = 0.0
+    softcap: float = 0.0
+    slopes: torch.Tensor | None = None
+    causal: bool = True
+    window: int = 0
+    prefix: torch.Tensor | None = None
+    doc: torch.Tensor | None = None
+
+    def _at(self, n_seq: int, H: int) -> _Score:
+        key = (n_seq, H)
+        if getattr(self, "_made", None) != key:
+            if self.doc is not None and (self.doc.dim() != 2 or self.doc.shape[0] != n_seq):
+                raise TlmError(-3, f"doc has shape {tuple(self.doc.shape)}, not [{n_seq}][positions]")
+            c = _Score(self.scale, self.softcap, _f32(self.slopes, "slopes", (H,)),
+                       _i32(self.prefix, "prefix", (n_seq,)), _i32(self.doc, "doc"),
+                       self.doc.shape[1] if self.doc is not None else 0, 1 if self.causal else 0, self.window)
+            object.__setattr__(self, "_c", c)   # built once: the fields never change
+            object.__setattr__(self, "_made", key)
+        return self._c
+
+
+class Kv8Cache:
+    """K and V pools of one layer (n_pages pages of page_size rows, KV heads
+    of hd) in format INT8 or E4M3, one scale per `block` rows; positions=True
+    adds the position pool that evicted sequences need."""
+
+    def __init__(self, n_pages: int, KV: int, page_size: int, hd: int, fmt: int = INT8, block: int = 16,
+                 positions: bool = False, device="cuda"):
+        if fmt not in (INT8, E4M3):
+            raise TlmError(-3, f"format {fmt} (int8 1 or e4m3 2)")
+        if block <= 0 or page_size % block:
+            raise TlmError(-3, f"block {block} does not divide the page of {page_size} rows")
+        dt = torch.int8 if fmt == INT8 else torch.float8_e4m3fn
+        shape = (n_pages, KV, page_size, hd)
+        k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dt) for _ in range(2))
+        ks, vs = (torch.zeros((n_pages, KV, page_size // block), device=device) for _ in range(2))
+        pos = torch.zeros((n_pages, KV, page_size), dtype=torch.int32, device=device) if positions else None
+        self._set(k, v, ks, vs, pos)
+
+    @classmethod
+    def from_pools(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                   pos: torch.Tensor | None = None) -> "Kv8Cache":
+        """A cache on pools that the caller holds (no copy)."""
+        self = cls.__new__(cls)
+        self._set(k, v, k_scale, v_scale, pos)
+        return self
+
+    def _set(self, k, v, k_scale, v_scale, pos) -> None:
+        if k.dtype not in _FMT or v.dtype != k.dtype:
+            raise TlmError(-3, f"code pools must both be int8 or float8_e4m3fn, not {k.dtype} and {v.dtype}")
+        if k.dim() != 4 or v.shape != k.shape:
+            raise TlmError(-3, f"code pools have shapes {tuple(k.shape)} and {tuple(v.shape)}, not [n_pages][KV][page][hd]")
+        n_pages, KV, page, hd = k.shape
+        if k_scale.dim() != 3 or k_scale.shape[2] == 0 or page % k_scale.shape[2]:
+            raise TlmError(-3, f"scale pools have shape {tuple(k_scale.shape)}, not [n_pages][KV][page / block]")
+        blocks = k_scale.shape[2]
+        self.k, self.v, self.k_scale, self.v_scale, self.pos = k, v, k_scale, v_scale, pos
+        self.KV, self.page_size, self.hd, self.block, self.fmt = KV, page, hd, page // blocks, _FMT[k.dtype]
+        self._c = _Cache(_dev(k, "k"), _dev(v, "v"), _f32(k_scale, "k_scale", (n_pages, KV, blocks)),
+                         _f32(v_scale, "v_scale", (n_pages, KV, blocks)), _i32(pos, "pos", (n_pages, KV, page)),
+                         self.fmt, n_pages, KV, page, self.block, hd)
+        self._lib = load()
+        self._work: dict[int, torch.Tensor] = {}
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, batch: Kv8Batch) -> None:
+        """Stores the batch's new rows k, v [n][KV][hd] (float32, float16 or
+        bfloat16)."""
+        k, sk = _rows(k, "k", self.KV, self.hd)
+        v, sv = _rows(v, "v", self.KV, self.hd)
+        if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
+            raise TlmError(-3, f"k and v differ: {k.dtype} x {k.shape[0]} rows, {v.dtype} x {v.shape[0]} rows")
+        if sk != sv:
+            k, v = k.contiguous(), v.contiguous()
+            sk = self.KV * self.hd
+        check(self._lib.tlmg_kv8_append(C.byref(self._c), C.byref(batch._at(k.shape[0])), _X_DT[k.dtype], k.data_ptr(),
+                                        v.data_ptr(), sk, stream_handle()))
+
+    def read(self, page_table: torch.Tensor, row0: torch.Tensor, start: torch.Tensor, total: int,
+             k: torch.Tensor | None = None, v: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Rows row0[s] .. of every sequence as float32 (rows start[s] ..
+        start[s + 1] - 1 of the results [total][KV][hd])."""
+        n_seq, stride = page_table.shape
+        shape = (total, self.KV, self.hd)
+        k = torch.empty(shape, device=self.k.device) if k is None else k
+        v = torch.empty(shape, device=self.k.device) if v is None else v
+        check(self._lib.tlmg_kv8_read(C.byref(self._c), n_seq, _i32(page_table, "page_table"), stride,
+                                      _i32(row0, "row0", (n_seq,)), _i32(start, "start", (n_seq + 1,)), total,
+                                      _f32(k, "k", shape), _f32(v, "v", shape), stream_handle()))
+        return k, v
+
+    def attend(self, q: torch.Tensor, batch: Kv8Batch, score: Score | None = None, out: torch.Tensor | None = None,
+               lse: bool | torch.Tensor = False, weights: torch.Tensor | None = None):
+        """Attention of the batch's tokens q [n][H][hd] over their sequences'
+        rows -> out (q's dtype), or (out, lse) with lse. weights float32
+        [n_seq][KV][rows >= max_kv] accumulates every row's softmax weights
+        (what evict goes by); max_q <= 64 then."""
+        if q.dim() != 3:
+            raise TlmError(-3, f"q has shape {tuple(q.shape)}, not [n][H][{self.hd}]")
+        H = q.shape[1]
+        q, sq = _rows(q, "q", H, self.hd)
+        b = batch._at(q.shape[0])
+        s = (score or Score())._at(batch.n_seq, H)
+        dt = _X_DT[q.dtype]
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            raise TlmError(-3, f"out is {out.dtype} {tuple(out.shape)}, q {q.dtype} {tuple(q.shape)}")
+        want = lse is True or isinstance(lse, torch.Tensor)
+        lse_t = lse if isinstance(lse, torch.Tensor) else torch.empty(q.shape[:2], device=q.device) if want else None
+        w_stride = 0
+        if weights is not None:
+            if weights.dim() != 3 or weights.shape[:2] != (batch.n_seq, self.KV):
+                raise TlmError(-3, f"weights have shape {tuple(weights.shape)}, not [{batch.n_seq}][{self.KV}][rows]")
+            w_stride = weights.shape[2]
+        st = stream_handle()
+        need = self._lib.tlmg_kv8_attend_work_bytes(C.byref(self._c), C.byref(b), C.byref(s), H, dt,
+                                                    0 if weights is None else 1)
+        work = self._work.get(st)
+        if work is None or work.numel() < need:
+            work = self._work[st] = torch.empty(max(need, 1 << 20), dtype=torch.uint8, device=q.device)
+        check(self._lib.tlmg_kv8_attend(C.byref(self._c), C.byref(b), C.byref(s), H, dt, q.data_ptr(), sq,
+                                        _dev(out, "out"), _f32(lse_t, "lse", tuple(q.shape[:2])),
+                                        _f32(weights, "weights"), w_stride, work.data_ptr(), work.numel(), st))
+        return (out, lse_t) if want else out
+
+    def evict(self, weights: torch.Tensor, batch: Kv8Batch, dst_table: torch.Tensor, n_keep: int, sink: int = 0,
+              recent: int = 0, dst: "Kv8Cache | None" = None, weights_out: torch.Tensor | None = None,
+              rows: torch.Tensor | None = None, lens: torch.Tensor | None = None):
+        """Cuts every (sequence, head) to n_keep rows: the first `sink`, the
+        last `recent` and those of the largest weights. The rows move into
+        dst_table's pages (of `dst`, or of this cache: other pages than
+        the sequences hold). Returns (rows int32 [n_seq][KV][n_keep], lens
+        int32 [n_seq]): the rows kept, ascending and -1 after the last, and
+        the new lengths."""
+        d = dst or self
+        n, dev = batch.n_seq, self.k.device
+        if weights.dim() != 3 or weights.shape[:2] != (n, self.KV):
+            raise TlmError(-3, f"weights have shape {tuple(weights.shape)}, not [{n}][{self.KV}][rows]")
+        if dst_table.dim() != 2 or dst_table.shape[0] != n:
+            raise TlmError(-3, f"dst_table has shape {tuple(dst_table.shape)}, not [{n}][stride]")
+        if weights_out is not None and (weights_out.dim() != 3 or weights_out.shape[:2] != (n, self.KV)):
+            raise TlmError(-3, f"weights_out has shape {tuple(weights_out.shape)}, not [{n}][{self.KV}][rows]")
+        rows = torch.empty((n, self.KV, max(n_keep, 0)), dtype=torch.int32, device=dev) if rows is None else rows
+        lens = torch.empty((n,), dtype=torch.int32, device=dev) if lens is None else lens
+        st = stream_handle()
+        w = _f32(weights, "weights")
+        r = _i32(rows, "rows", (n, self.KV, n_keep))
+        check(self._lib.tlmg_kv8_select(n, self.KV, batch._c.kv_len, batch.max_kv, w, weights.shape[2], n_keep, sink,
+                                        recent, r, _i32(lens, "lens", (n,)), st))
+        check(self._lib.tlmg_kv8_compact(C.byref(self._c), C.byref(d._c), n, batch._c.page_table, batch._c.table_stride,
+                                         batch._c.kv_len, _i32(dst_table, "dst_table"), dst_table.shape[1], r, n_keep, w,
+                                         weights.shape[2], _f32(weights_out, "weights_out"),
+                                         0 if weights_out is None else weights_out.shape[2], st))
+        return rows, lens
