@@ -491,6 +491,58 @@ def test_few_and_many_tokens(lens, news, H, KV, hd, dtype):
     check_attend(host, table, q_start, lens, q, H, causal=False)
 
 
+MANY = [   # (lens, news, H, KV, hd, page, block): more query rows per KV head than a tensor-core tile
+    ([300, 40, 7], [300, 40, 7], 8, 2, 64, 16, 16), ([500], [130], 4, 4, 128, 64, 16), ([129, 260], [128, 129], 3, 1, 64, 8, 1),
+    ([257], [257], 6, 2, 128, 32, 32), ([400, 1], [16, 0], 32, 2, 128, 256, 64), ([640], [40], 16, 1, 64, 1, 1),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt", [K.INT8, K.E4M3])
+@pytest.mark.parametrize("case", MANY)
+def test_prefill(case, fmt, dtype):
+    lens, news, H, KV, hd, page, block = case
+    host, table, q_start, q, _ = make(31, lens, news, H, KV, hd, fmt, page, block, dtype=dtype)
+    check_attend(host, table, q_start, lens, q, H)
+    check_attend(host, table, q_start, lens, q, H, causal=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("name", ["cap", "cap_small", "alibi", "alibi_both", "window", "window_one", "sinks", "prefix", "prefix_all", "doc",
+                                  "doc_jumbled", "doc_short", "all", "scale", "window_open"])
+def test_prefill_score_shapes(name, dtype):
+    lens, news, H, KV, hd = [290, 180, 20], [200, 180, 3], 4, 2, 64
+    host, table, q_start, q, rng = make(32, lens, news, H, KV, hd, K.E4M3, 16, 4, dtype=dtype)
+    check_attend(host, table, q_start, lens, q, H, **mods_of(name, rng, lens, H))
+
+
+@pytest.mark.gpu
+def test_prefill_positions_and_poison():
+    """The position pool, masked rows with NaN scales, rows without keys and bad sequences at prefill sizes."""
+    lens, news, H, KV, hd = [300, 200], [150, 140], 4, 2, 128
+    host, table, q_start, q, rng = make(33, lens, news, H, KV, hd, K.INT8, 16, 16, pos=True, dtype=torch.bfloat16)
+    for s, L in enumerate(lens):
+        for t in range(L):
+            host.pos[table[s, t // 16], :, t % 16] = rng.integers(0, 500, KV)
+    q_pos = rng.integers(0, 500, 290).astype(np.int32)
+    q_pos[:3] = [0, 499, 0]
+    host.pos[table[0, 3]] = 1000                       # never seen (causal)
+    host.ks[table[0, 3]], host.vs[table[0, 3]] = np.nan, np.nan
+    host.vs[table[1, 2]] = 1e25                        # seen by few
+    host.pos[table[1, 2]] = 498
+    check_attend(host, table, q_start, lens, q, H, q_pos=q_pos)
+    check_attend(host, table, q_start, lens, q, H, q_pos=q_pos, window=40)
+    good = host.gpu().attend(q.cuda(), batch(table, q_start, lens, q_pos))
+    out, lse = host.gpu().attend(q.cuda(), batch(table, q_start, [300, 4000], q_pos, max_kv=300), lse=True)
+    assert torch.isnan(out[150:]).all() and torch.isnan(lse[150:]).all() and (out[:150] == good[:150]).all()
+    bad = table.copy()
+    bad[1, 4] = -5                                     # positions there are unknown: every query that may see position 0
+    out = host.gpu().attend(q.cuda(), batch(bad, q_start, lens, q_pos))
+    assert torch.isnan(out[150:]).all() and (out[:150] == good[:150]).all()
+
+
 def mods_of(name, rng, lens, H):
     n = len(lens)
     doc = np.full((n, max(lens)), -1, np.int32)

@@ -45,7 +45,8 @@ int kv8_check(const char *who, const tlmg_kv8 *c) {
 
 int kv8_check_batch(const char *who, const tlmg_kv8_batch *b) {
     if (!b || !b->page_table || !b->q_start || !b->kv_len) return set_error(TLMG_EINVAL, "%s: null batch array", who);
-    if (b->n_seq <= 0 || b->n_seq > 65535 || b->table_stride <= 0 || b->total_q < 0 || b->max_q < 0 || b->max_kv < 0)
+    if (b->n_seq <= 0 || b->n_seq > 65535 || b->table_stride <= 0 || b->total_q < 0 || b->max_q < 0 ||
+        b->max_kv < 0 || b->max_kv > (1 << 30))
         return set_error(TLMG_EINVAL, "%s: %d sequences (1 .. 65535), table stride %d, %d tokens, max_q %d, max_kv %d", who,
                          b->n_seq, b->table_stride, b->total_q, b->max_q, b->max_kv);
     return TLMG_OK;

@@ -87,42 +87,18 @@ template <int HD> struct Plan {
     static constexpr int SMEM = NW * NST * STAGE;
 };
 
-// The tiles of 32 rows that some query of the tile's tokens [i0, i1) may
-// see. Rows are positions when the cache has no position pool: then they are
-// the rows below the prefix and those from the window's begin to the last
-// query's position.
-struct Range {
-    int nA, loB, n;   // tiles of the first part, first row of the second, tiles in all
-    __device__ __forceinline__ int t0(int v) const { return v < nA ? v * TILE : loB + (v - nA) * TILE; }
-};
-__device__ __forceinline__ Range key_range(const Kv8Attn &a, const Kv8Seq &q, int s, int i0, int i1) {
-    int lo = 0, hi = q.L, pre = 0;
-    if (!a.c.pos && (a.causal || a.window)) {
-        int pmin = q.L - q.n + i0, pmax = q.L - q.n + i1 - 1;
-        if (a.b.q_pos) {
-            pmin = INT32_MAX;
-            pmax = INT32_MIN;
-            for (int i = i0; i < i1; i++) {
-                const int p = a.b.q_pos[q.q0 + i];
-                pmin = min(pmin, p);
-                pmax = max(pmax, p);
-            }
+__device__ __forceinline__ Kv8Range<TILE> key_range(const Kv8Attn &a, const Kv8Seq &q, int s, int i0, int i1) {
+    int pmin = q.L - q.n + i0, pmax = q.L - q.n + i1 - 1;
+    if (a.b.q_pos && !a.c.pos && (a.causal || a.window)) {
+        pmin = INT32_MAX;
+        pmax = INT32_MIN;
+        for (int i = i0; i < i1; i++) {
+            const int p = a.b.q_pos[q.q0 + i];
+            pmin = min(pmin, p);
+            pmax = max(pmax, p);
         }
-        pre = a.prefix ? min(max(a.prefix[s], 0), q.L) : 0;
-        if (a.causal) hi = pmax >= q.L ? q.L : max(pmax, -1) + 1;
-        if (a.window) lo = min(max((int)min((int64_t)pmin - a.window + 1, (int64_t)INT32_MAX), 0), hi);
     }
-    Range r;
-    r.nA = (pre + TILE - 1) / TILE;
-    r.loB = lo / TILE * TILE;
-    const int nB = hi > r.loB ? (hi - r.loB + TILE - 1) / TILE : 0;
-    if (r.nA * TILE >= r.loB) {      // one part
-        r.n = max(r.nA, r.loB / TILE + nB);
-        r.nA = r.n;
-    } else {
-        r.n = r.nA + nB;
-    }
-    return r;
+    return kv8_range<TILE>(a, q, s, pmin, pmax);
 }
 
 template <int HD, int FMT, typename QT>
@@ -163,7 +139,7 @@ __global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ K
     const int R0 = rt * ROWS, n_rows = q.n * G;
     if (R0 >= n_rows) return;
     const int i0 = R0 / G, i1 = min(q.n, (R0 + ROWS - 1) / G + 1);
-    const Range rg = key_range(a, q, s, i0, i1);
+    const Kv8Range<TILE> rg = key_range(a, q, s, i0, i1);
     const int v0 = split * a.tiles, v1 = min(rg.n, v0 + a.tiles);
     const int n_my = v1 - v0 > warp ? (v1 - v0 - warp + NW - 1) / NW : 0;   // tiles v0 + warp + NW i
 
@@ -583,7 +559,7 @@ __global__ void __launch_bounds__(WG_THREADS) k_kv8_weights(const __grid_constan
     const int n_rows = q.n * a.G, n_rt = (n_rows + ROWS - 1) / ROWS;
     for (int R = tid; R < n_rows; R += WG_THREADS) l2[R] = a.lse2[(q.q0 + (int64_t)(R / a.G)) * a.H + kvh * a.G + R % a.G];
     for (int r = tid; r < n_rt; r += WG_THREADS) {
-        const Range rg = key_range(a, q, s, r * ROWS / a.G, min(q.n, (r * ROWS + ROWS - 1) / a.G + 1));
+        const Kv8Range<TILE> rg = key_range(a, q, s, r * ROWS / a.G, min(q.n, (r * ROWS + ROWS - 1) / a.G + 1));
         end_a[r] = rg.nA * TILE;
         lo_b[r] = rg.loB;
         end_b[r] = rg.loB + (rg.n - rg.nA) * TILE;
@@ -632,6 +608,7 @@ bool smem_opt_in(const void *fn, size_t bytes) {
 }
 
 struct Split {
+    bool wide;             // the tcgen05 kernel serves the call
     int n, tiles;          // spans, 32-row tiles per span
     int64_t rtiles;        // query tiles
     size_t part, scores, total;   // floats of the partial results / scores, bytes in all
@@ -641,6 +618,8 @@ struct Split {
 Split split_plan(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_score &s, int H, int q_dt, bool weights) {
     Split p{};
     const int G = H / c.KV, rows = q_dt == TLMG_DT_F32 ? 8 : 16;
+    p.wide = !weights && kv8_prefill_serves(c, b, H, q_dt);
+    if (p.wide) return p;
     p.rtiles = ((int64_t)b.max_q * G + rows - 1) / rows;
     // rows that a query tile can see at most (the prefix is only known to the device)
     int64_t vis = b.max_kv;
@@ -786,5 +765,6 @@ extern "C" int tlmg_kv8_attend(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const
         a.lse2 = a.scores + rows * p.s_stride;
     }
     cudaStream_t cs = pick_stream(stream);
+    if (p.wide) return kv8_prefill(a, c->fmt, q_dt, cs);
     return c->fmt == TLMG_KV8_INT8 ? launch_split_hd<TLMG_KV8_INT8>(a, p, q_dt, cs) : launch_split_hd<TLMG_KV8_E4M3>(a, p, q_dt, cs);
 }

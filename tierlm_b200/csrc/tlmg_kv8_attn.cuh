@@ -1,5 +1,7 @@
 // tlmg_kv8_attn.cuh - arguments of the 8-bit cache's attention kernels.
 #pragma once
+#include <algorithm>
+
 #include "tlmg_kv8.cuh"
 
 namespace tlmg {
@@ -23,5 +25,38 @@ struct Kv8Attn {
     float *po, *pm, *pl, *scores, *lse2;
     int64_t s_stride;
 };
+
+// The key tiles of TILE rows that a tile of queries at positions pmin ..
+// pmax may see. Rows are positions when the cache has no position pool: then
+// they are the rows below the prefix and those from the window's begin to
+// the last query's position.
+template <int TILE> struct Kv8Range {
+    int nA, loB, n;   // tiles of the first part, first row of the second, tiles in all
+    __device__ __forceinline__ int t0(int v) const { return v < nA ? v * TILE : loB + (v - nA) * TILE; }
+};
+template <int TILE>
+__device__ __forceinline__ Kv8Range<TILE> kv8_range(const Kv8Attn &a, const Kv8Seq &q, int s, int pmin, int pmax) {
+    int lo = 0, hi = q.L, pre = 0;
+    if (!a.c.pos && (a.causal || a.window)) {
+        pre = a.prefix ? min(max(a.prefix[s], 0), q.L) : 0;
+        if (a.causal) hi = pmax >= q.L ? q.L : max(pmax, -1) + 1;
+        if (a.window) lo = min(max((int)min((int64_t)pmin - a.window + 1, (int64_t)INT32_MAX), 0), hi);
+    }
+    Kv8Range<TILE> r;
+    r.nA = (pre + TILE - 1) / TILE;
+    r.loB = lo / TILE * TILE;
+    const int nB = hi > r.loB ? (hi - r.loB + TILE - 1) / TILE : 0;
+    if (r.nA * TILE >= r.loB) {      // one part
+        r.n = max(r.nA, r.loB / TILE + nB);
+        r.nA = r.n;
+    } else {
+        r.n = r.nA + nB;
+    }
+    return r;
+}
+
+// The form for many query rows (tlmg_kv8_prefill.cu): whether it serves a call, and the call.
+bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt);
+int kv8_prefill(const Kv8Attn &a, int fmt, int q_dt, cudaStream_t st);
 
 }  // namespace tlmg

@@ -1,0 +1,612 @@
+// tlmg_kv8_prefill.cu - attention over the 8-bit KV cache for many query rows,
+// on tcgen05 (16-bit queries, head_dim 64 and 128).
+//
+// One CTA per SM takes 256 query rows (token, head of the group) of one KV
+// head in two tiles A and B of 128, and walks the visible keys in tiles of
+// 128. Roles, 13 warps:
+//   warps 0-3, 4-7  softmax of tile A, B: thread = query row = TMEM lane
+//   warps 8-11      K and V codes -> f16 in shared memory, once for both tiles
+//   warp 12         one thread issues the MMAs
+// Per key tile and query tile: S = Q K^T (8 x tcgen05.mma M128 N128 K16 at
+// hd 128, operands in shared memory, S f32 in TMEM); the softmax warps read S
+// and write P as f16 over it; O += P V (A operand P from TMEM, V from shared
+// memory, O f32 in TMEM). While one tile's softmax runs, the tensor core
+// works for the other: TMEM is full at 2 x (S 128 + O 128) columns.
+//
+// Scales. A key's score is S * k_scale (per column) * the row's factor; the
+// weight that multiplies V's code is p * v_scale. Each row keeps a reference
+// w = max over its visible keys of score + log2(v_scale) and stores
+// p'' = 2^(score - w + 14), so p'' * v_scale < 2^15 fits f16 whatever the scales
+// of other rows, and the row sum of p'' divides the result. The reference
+// follows the maximum when it grew by more than a factor of two; then the
+// warp multiplies its O rows in TMEM (its MMAs are done: the commit that
+// announced S covers the PV before it).
+//
+// Layouts. Shared-memory operands are 8 x 16-byte core matrices without
+// swizzle: chunk c (8 dims) of row r at (r / 8) * hd * 16 + c * 128 + (r % 8) *
+// 16, so 8 lanes write 8 rows of one chunk, 128 contiguous bytes. The same
+// bytes are K as a K-major B operand (contraction over dims) and V as an
+// MN-major one (contraction over keys).
+//
+// Every wait is bounded: a role whose wait runs out sets a flag, all roles
+// leave, and the CTA's outputs are NaN.
+#include <cstdint>
+#include <utility>
+#include <vector>
+
+#include "tlmg_dev.cuh"
+#include "tlmg_internal.h"
+#include "tlmg_kv8.cuh"
+#include "tlmg_kv8_attn.cuh"
+
+namespace tlmg {
+namespace {
+
+constexpr int TK = 128;           // keys of a tile
+constexpr int TQ = 128;           // query rows of a tile
+constexpr int THREADS = 13 * 32;
+constexpr int META = 4;           // buffers of per-key scales
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ uint32_t saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+template <int HD> struct Smem {
+    alignas(128) uint8_t q[2][TQ * HD * 2];
+    alignas(128) uint8_t k[2][TK * HD * 2];
+    alignas(128) uint8_t v[2][TK * HD * 2];
+    alignas(16) float ks[META][TK], vs[META][TK], lv[META][TK];
+    int pos[META][TK], doc[META][TK];
+    uint32_t row[2][TK];
+    uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], meta_full[META], drain;
+    uint32_t tmem;
+    int abort, pmin, pmax;
+};
+
+__device__ __forceinline__ void mbar_init(uint64_t *b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(saddr(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t *b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(b)) : "memory");
+}
+// Waits for phase `parity`; false when it did not come in about a second or another role gave up.
+__device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, int *abort) {
+    for (uint32_t i = 0; i < (1u << 20); i++) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+                     : "=r"(done)
+                     : "r"(saddr(b)), "r"(parity)
+                     : "memory");
+        if (done) return true;
+        if ((i & 63u) == 63u && abort && *(volatile int *)abort) return false;
+    }
+    if (abort) *(volatile int *)abort = 1;
+    return false;
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void umma_commit(uint64_t *b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(b)) : "memory");
+}
+
+// Shared-memory operand descriptor, no swizzle, version 1: start, leading and stride byte offsets.
+__device__ __forceinline__ uint64_t umma_desc(uint32_t start, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((start >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
+           ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);
+}
+// Instruction descriptor: D f32, A and B f16, A K-major, B K-major or MN-major, M 128.
+constexpr uint32_t idesc(int n, bool b_mn) {
+    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TQ >> 4) << 24);
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    const uint32_t z = 0;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(id), "r"(acc), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    const uint32_t z = 0;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(id), "r"(acc), "r"(z)
+                 : "memory");
+}
+
+#define TLMG_R32(V)                                                                                                       \
+    V(0), V(1), V(2), V(3), V(4), V(5), V(6), V(7), V(8), V(9), V(10), V(11), V(12), V(13), V(14), V(15), V(16), V(17),   \
+        V(18), V(19), V(20), V(21), V(22), V(23), V(24), V(25), V(26), V(27), V(28), V(29), V(30), V(31)
+#define TLMG_OUT(I) "=r"(v[I])
+#define TLMG_IN(I) "r"(v[I])
+// 32 columns of the warp's lanes; the load and its wait are one statement
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+                 "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;\n"
+                 : TLMG_R32(TLMG_OUT)
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};\n" ::TLMG_R32(TLMG_IN),
+                 "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15};\n" ::"r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+                 "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// packed pairs of f32 (one issue slot for two)
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pk(float x, float y) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ f2 pku(uint32_t x, uint32_t y) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+    return r;
+}
+__device__ __forceinline__ void upk(f2 a, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+constexpr float TOP = 14.0f;   // log2 of the largest p * v_scale right after a row's reference moved
+
+template <int HD, int FMT, typename QT>
+__global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constant__ Kv8Attn a) {
+    extern __shared__ __align__(128) uint8_t raw[];
+    Smem<HD> &sm = *reinterpret_cast<Smem<HD> *>(raw);
+    constexpr int SBO = HD * 16;              // bytes between 8-row groups of an operand
+    constexpr int PC = HD / 16;               // 16-byte pieces of a code row
+    constexpr int NP = TK * PC / 128;         // pieces of a tile per converting thread
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int s = blockIdx.z, kvh = blockIdx.y;
+    const int rt = gridDim.x - 1 - blockIdx.x;   // the last tokens see the most keys: they go first
+    QT *out = static_cast<QT *>(a.out);
+    Kv8Seq q;
+    if (!kv8_seq(a.b, a.c.lp, s, q)) {
+        const float nan = __uint_as_float(0x7FC00000u);
+        const int64_t i0 = max(q.q0, 0), i1 = min((int64_t)a.b.q_start[s + 1], (int64_t)a.b.total_q);
+        for (int64_t R = (int64_t)blockIdx.x * (THREADS / 32) + warp; R < (i1 - i0) * a.G; R += (int64_t)gridDim.x * (THREADS / 32)) {
+            const int64_t row = (i0 + R / a.G) * a.H + kvh * a.G + R % a.G;
+            for (int d = 4 * lane; d < HD; d += 128) kv8_st4(out + row * HD + d, make_float4(nan, nan, nan, nan));
+            if (lane == 0 && a.lse) a.lse[row] = nan;
+        }
+        return;
+    }
+    const int n_rows = q.n * a.G, R0 = rt * 2 * TQ;
+    if (R0 >= n_rows) return;
+    const bool two = R0 + TQ < n_rows;
+    const int i0 = R0 / a.G, i1 = min(q.n, (R0 + 2 * TQ - 1) / a.G + 1);
+    if (tid == 0) {
+        sm.abort = 0;
+        sm.pmin = INT32_MAX;
+        sm.pmax = INT32_MIN;
+        mbar_init(&sm.q_full, two ? 2 * TQ : TQ);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sm.k_full[i], 128);
+            mbar_init(&sm.v_full[i], 128);
+            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_empty[i], 1);
+            mbar_init(&sm.s_full[i], 1);
+            mbar_init(&sm.p_full[i], TQ);
+            mbar_init(&sm.o_full[i], 1);
+        }
+        for (int i = 0; i < META; i++) mbar_init(&sm.meta_full[i], 128);
+        mbar_init(&sm.drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sm.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    for (int i = i0 + tid; i < i1; i += THREADS) {
+        const int p = a.b.q_pos ? a.b.q_pos[q.q0 + i] : q.L - q.n + i;
+        atomicMin(&sm.pmin, p);
+        atomicMax(&sm.pmax, p);
+    }
+    __syncthreads();
+    const int pmin = sm.pmin, pmax = sm.pmax;
+    const Kv8Range<TK> rg = kv8_range<TK>(a, q, s, pmin, pmax);
+    const uint32_t tmem = sm.tmem;
+    const int32_t *docs = a.doc ? a.doc + (size_t)s * a.doc_stride : nullptr;
+    const int n = rg.n;
+
+    if (warp < 8) {
+        // ---- softmax of one query tile ----
+        const int w = warp >> 2, r = tid & (TQ - 1);
+        if (w == 0 || two) {
+            const int R = R0 + w * TQ + r;
+            const bool live = R < n_rows;
+            const int tok = live ? R / a.G : i0, h = kvh * a.G + (live ? R % a.G : 0);
+            const int qp = a.b.q_pos ? a.b.q_pos[q.q0 + tok] : q.L - q.n + tok;
+            const int qd = docs ? (qp >= 0 && qp < a.doc_stride ? docs[qp] : -1) : -1;
+            const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+            const int pre = a.prefix ? a.prefix[s] : 0;
+            const int64_t orow = (q.q0 + (int64_t)tok) * a.H + h;
+            float qsc;
+            {   // the query row as f16, its largest element brought to 2^9 .. 2^10
+                const QT *x = static_cast<const QT *>(a.q) + (q.q0 + (int64_t)tok) * a.q_stride + (int64_t)h * HD;
+                float m = 0.0f;
+                for (int d = 0; d < HD; d += 4) {
+                    const float4 v = kv8_ld4(x + d);
+                    m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                }
+                const int e = min(max((int)((__float_as_uint(m) >> 23) & 255u) - 136, -100), 100);
+                const float up = live ? __int_as_float((127 - e) << 23) : 0.0f;
+                qsc = __int_as_float((127 + e) << 23) * a.scale * kv8_f16_unit<FMT>();
+                uint8_t *dst = sm.q[w] + (r >> 3) * SBO + (r & 7) * 16;
+                for (int c = 0; c < HD / 8; c++) {
+                    const float4 v0 = kv8_ld4(x + 8 * c), v1 = kv8_ld4(x + 8 * c + 4);
+                    *reinterpret_cast<uint4 *>(dst + c * 128) =
+                        make_uint4(pack_f16(v0.x * up, v0.y * up), pack_f16(v0.z * up, v0.w * up),
+                                   pack_f16(v1.x * up, v1.y * up), pack_f16(v1.z * up, v1.w * up));
+                }
+                fence_async_smem();
+                mbar_arrive(&sm.q_full);
+            }
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // this warp's 32 TMEM lanes
+            const uint32_t ts = tmem + lanes + w * TK, to = tmem + lanes + 2 * TK + w * HD;
+            const bool shaped = a.softcap > 0.0f || a.slopes || docs || a.c.pos;
+            const float qs2 = qsc * LOG2E, capl = a.softcap * LOG2E, capx = qsc * a.inv_cap * 2.0f * LOG2E;
+            const f2 q2 = pk(qs2, qs2);
+            float wref = -INFINITY;
+            f2 sum0 = pk(0.0f, 0.0f), sum1 = pk(0.0f, 0.0f);
+            bool ok = true;
+            for (int j = 0; j < n; j++) {
+                const int t0 = rg.t0(j), mb = j & (META - 1);
+                ok = mbar_wait(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait(&sm.s_full[w], j & 1, &sm.abort);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                tc_after();
+                const float4 *ks4 = reinterpret_cast<const float4 *>(sm.ks[mb]), *vs4 = reinterpret_cast<const float4 *>(sm.vs[mb]),
+                             *lv4 = reinterpret_cast<const float4 *>(sm.lv[mb]);
+                // every key of the tile is seen by every row of the CTA, its score is a plain product
+                const bool plain = !shaped && t0 + TK <= q.L && (!a.causal || t0 + TK - 1 <= pmin) && (!a.window || pmax - t0 < a.window);
+                float m0 = -INFINITY, m1 = -INFINITY;
+                if (plain) {
+#pragma unroll
+                    for (int c = 0; c < TK / 32; c++) {
+                        uint32_t x[32];
+                        tmem_ld32(ts + 32 * c, x);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float4 k = ks4[8 * c + i], l = lv4[8 * c + i];
+                            float y0, y1, y2, y3;
+                            upk(fma2(mul2(pku(x[4 * i], x[4 * i + 1]), pk(k.x, k.y)), q2, pk(l.x, l.y)), y0, y1);
+                            upk(fma2(mul2(pku(x[4 * i + 2], x[4 * i + 3]), pk(k.z, k.w)), q2, pk(l.z, l.w)), y2, y3);
+                            m0 = fmaxf(m0, fmaxf(y0, y1));
+                            m1 = fmaxf(m1, fmaxf(y2, y3));
+                        }
+                    }
+                } else {
+                    // scores in log2 units, masked ones -inf, written back over S
+#pragma unroll 1
+                    for (int c = 0; c < TK / 32; c++) {
+                        uint32_t x[32];
+                        tmem_ld32(ts + 32 * c, x);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const int col = 32 * c + i, t = t0 + col;
+                            const int kp = a.c.pos ? sm.pos[mb][col] : t;
+                            float z = __uint_as_float(x[i]) * sm.ks[mb][col];
+                            if (a.softcap > 0.0f) {   // tanh(y) = 1 - 2 / (e^2y + 1)
+                                const float e = ex2(z * capx);
+                                z = __fmaf_rn(-2.0f * capl, __fdividef(1.0f, e + 1.0f), capl);
+                            } else {
+                                z *= qs2;
+                            }
+                            if (a.slopes) z = __fmaf_rn(-slope, fabsf((float)(qp - kp)), z);
+                            bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
+                            see = see && t < q.L && (!docs || sm.doc[mb][col] == qd);
+                            z = see ? z : -INFINITY;
+                            m0 = fmaxf(m0, z + sm.lv[mb][col]);
+                            x[i] = __float_as_uint(z);
+                        }
+                        tmem_st32(ts + 32 * c, x);
+                    }
+                    tmem_wait_st();
+                }
+                m0 = fmaxf(m0, m1);
+                const bool grow = m0 > wref + 1.0f;
+                if (__any_sync(0xFFFFFFFFu, grow)) {
+                    const float f = grow && wref != -INFINITY ? ex2(wref - m0) : 1.0f;
+                    if (grow) wref = m0;
+                    const f2 f2v = pk(f, f);
+                    sum0 = mul2(sum0, f2v);
+                    sum1 = mul2(sum1, f2v);
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < HD / 32; c++) {
+                            uint32_t x[32];
+                            tmem_ld32(to + 32 * c, x);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+                            tmem_st32(to + 32 * c, x);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                const float sub = wref == -INFINITY ? 0.0f : TOP - wref;
+                const f2 sub2 = pk(sub, sub);
+#pragma unroll
+                for (int c = 0; c < TK / 32; c++) {
+                    uint32_t x[32], p[16];
+                    tmem_ld32(ts + 32 * c, x);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float4 v = vs4[8 * c + i];
+                        f2 e0, e1;
+                        if (plain) {
+                            const float4 k = ks4[8 * c + i];
+                            e0 = fma2(mul2(pku(x[4 * i], x[4 * i + 1]), pk(k.x, k.y)), q2, sub2);
+                            e1 = fma2(mul2(pku(x[4 * i + 2], x[4 * i + 3]), pk(k.z, k.w)), q2, sub2);
+                        } else {
+                            e0 = add2(pku(x[4 * i], x[4 * i + 1]), sub2);
+                            e1 = add2(pku(x[4 * i + 2], x[4 * i + 3]), sub2);
+                        }
+                        float y0, y1, y2, y3;
+                        upk(e0, y0, y1);
+                        upk(e1, y2, y3);
+                        const f2 p0 = pk(ex2(y0), ex2(y1)), p1 = pk(ex2(y2), ex2(y3));
+                        sum0 = add2(sum0, p0);
+                        sum1 = add2(sum1, p1);
+                        float u0, u1, u2, u3;
+                        upk(mul2(p0, pk(v.x, v.y)), u0, u1);
+                        upk(mul2(p1, pk(v.z, v.w)), u2, u3);
+                        if (!plain) {   // a masked key's scale has no part in this, whatever it is
+                            u0 = y0 == -INFINITY ? 0.0f : u0;
+                            u1 = y1 == -INFINITY ? 0.0f : u1;
+                            u2 = y2 == -INFINITY ? 0.0f : u2;
+                            u3 = y3 == -INFINITY ? 0.0f : u3;
+                        }
+                        p[2 * i] = pack_f16(u0, u1);
+                        p[2 * i + 1] = pack_f16(u2, u3);
+                    }
+                    tmem_st16(ts + 16 * c, p);   // columns whose scores are read already
+                }
+                tmem_wait_st();
+                tc_before();
+                mbar_arrive(&sm.p_full[w]);
+            }
+            if (ok && n > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.o_full[w], 0, &sm.abort));
+            tc_after();
+            float l0, l1, l2, l3;
+            upk(sum0, l0, l1);
+            upk(sum1, l2, l3);
+            const float l = (l0 + l1) + (l2 + l3);
+            const float inv = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? 0.0f : __fdividef(kv8_f16_unit<FMT>(), l);
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; c++) {
+                uint32_t x[32];
+                if (ok && n > 0) {
+                    tmem_ld32(to + 32 * c, x);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = 0;
+                }
+                if (live)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        kv8_st4(out + orow * HD + 32 * c + i,
+                                make_float4(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv,
+                                            __uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv));
+            }
+            if (live && a.lse) a.lse[orow] = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? -INFINITY : (log2f(l) - (wref == -INFINITY ? 0.0f : TOP - wref)) * LN2;
+        }
+    } else if (warp < 12) {
+        // ---- codes to f16 ----
+        const int c = tid - 256;
+        const int prow = (c & 7) + 8 * (c / (8 * PC)), piece = (c >> 3) % PC;   // first row and piece of this thread
+        constexpr int RSTEP = 8 * (128 / (8 * PC));                            // its next row
+        const int32_t *table = a.b.page_table + (size_t)s * a.b.table_stride;
+        const float nan = __uint_as_float(0x7FC00000u);
+        uint4 kr[NP], vr[NP];
+        int32_t te = -1, te_next = -1;
+        auto entry = [&](int j) {
+            if (j >= n) return -1;
+            const int t = rg.t0(j) + c;
+            return t < q.L ? __ldg(table + (t >> a.c.lp)) : -1;
+        };
+        float mk = 0.0f, mv = 0.0f;
+        int mp = 0, md = -1;
+        auto rows_of = [&](int j, int32_t e) {   // row numbers of tile j; its scales into registers
+            const int t = rg.t0(j) + c;
+            const bool have = t < q.L && a.c.ok(e);
+            const uint32_t rid = have ? a.c.row(e, kvh, t) : 0xFFFFFFFFu;
+            sm.row[j & 1][c] = rid;
+            mk = have ? __ldg(a.c.ks + (rid >> a.c.lb)) : nan;
+            mv = have ? __ldg(a.c.vs + (rid >> a.c.lb)) : nan;
+            if (a.c.pos) mp = have ? __ldg(a.c.pos + rid) : 0;
+            if (docs) {
+                const int p = a.c.pos ? mp : t;
+                md = p >= 0 && p < a.doc_stride ? __ldg(docs + p) : -1;
+            }
+        };
+        auto put_meta = [&](int j) {
+            const int mb = j & (META - 1);
+            sm.ks[mb][c] = mk;
+            sm.vs[mb][c] = mv;
+            sm.lv[mb][c] = fmaxf(log2f(mv), -60.0f);
+            sm.pos[mb][c] = mp;
+            sm.doc[mb][c] = md;
+            mbar_arrive(&sm.meta_full[mb]);
+        };
+        auto load = [&](const uint8_t *pool, int j, uint4 (&x)[NP]) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const uint32_t rid = sm.row[j & 1][prow + RSTEP * i];
+                x[i] = rid != 0xFFFFFFFFu ? __ldg(reinterpret_cast<const uint4 *>(pool + (size_t)rid * HD + 16 * piece)) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto convert = [&](uint8_t *dst, const uint4 (&x)[NP]) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const int r = prow + RSTEP * i;
+                uint8_t *d = dst + (r >> 3) * SBO + piece * 256 + (r & 7) * 16;
+                const uint32_t b0 = kv8_bias<FMT>(x[i].x), b1 = kv8_bias<FMT>(x[i].y), b2 = kv8_bias<FMT>(x[i].z), b3 = kv8_bias<FMT>(x[i].w);
+                *reinterpret_cast<uint4 *>(d) = make_uint4(kv8_half2<FMT, 0>(b0), kv8_half2<FMT, 1>(b0), kv8_half2<FMT, 0>(b1), kv8_half2<FMT, 1>(b1));
+                *reinterpret_cast<uint4 *>(d + 128) = make_uint4(kv8_half2<FMT, 0>(b2), kv8_half2<FMT, 1>(b2), kv8_half2<FMT, 0>(b3), kv8_half2<FMT, 1>(b3));
+            }
+            fence_async_smem();
+        };
+        auto bar = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+        bool ok = true;
+        if (n > 0) {
+            rows_of(0, entry(0));
+            te = entry(1);
+            bar();
+            load(a.c.k, 0, kr);
+            load(a.c.v, 0, vr);
+            put_meta(0);
+        }
+        for (int j = 0; j < n; j++) {
+            te_next = entry(j + 2);
+            // after a wait that ran out the thread goes on to the barriers, without work
+            if (j >= 2) ok = mbar_wait(&sm.k_empty[j & 1], ((j >> 1) - 1) & 1, &sm.abort) && ok;
+            if (ok) {
+                convert(sm.k[j & 1], kr);
+                mbar_arrive(&sm.k_full[j & 1]);
+                if (j + 1 < n) rows_of(j + 1, te);
+            }
+            te = te_next;
+            bar();
+            if (ok && j + 1 < n) load(a.c.k, j + 1, kr);
+            if (j >= 2) ok = mbar_wait(&sm.v_empty[j & 1], ((j >> 1) - 1) & 1, &sm.abort) && ok;
+            if (ok) {
+                convert(sm.v[j & 1], vr);
+                mbar_arrive(&sm.v_full[j & 1]);
+                if (j + 1 < n) {
+                    load(a.c.v, j + 1, vr);
+                    put_meta(j + 1);
+                }
+            }
+        }
+    } else if (lane == 0) {
+        // ---- MMAs ----
+        constexpr uint32_t id_qk = idesc(TK, false), id_pv = idesc(HD, true);
+        auto qk = [&](int w, int j) {
+            const uint32_t qa = saddr(sm.q[w]), ka = saddr(sm.k[j & 1]);
+#pragma unroll
+            for (int k = 0; k < HD / 16; k++)
+                umma_ss(tmem + w * TK, umma_desc(qa + 256 * k, 128, SBO), umma_desc(ka + 256 * k, 128, SBO), id_qk, k > 0);
+            umma_commit(&sm.s_full[w]);
+        };
+        auto pv = [&](int w, int j) {
+            const uint32_t va = saddr(sm.v[j & 1]);
+#pragma unroll
+            for (int k = 0; k < TK / 16; k++)
+                umma_ts(tmem + 2 * TK + w * HD, tmem + w * TK + 8 * k, umma_desc(va + 2 * SBO * k, SBO, 128), id_pv, j > 0 || k > 0);
+        };
+        const int nw = two ? 2 : 1;
+        bool ok = n == 0 || (mbar_wait(&sm.q_full, 0, &sm.abort) && mbar_wait(&sm.k_full[0], 0, &sm.abort));
+        if (ok && n > 0) {
+            tc_after();
+            for (int w = 0; w < nw; w++) qk(w, 0);
+            umma_commit(&sm.k_empty[0]);
+        }
+        for (int j = 0; ok && j < n; j++) {
+            for (int w = 0; ok && w < nw; w++) {
+                ok = mbar_wait(&sm.p_full[w], j & 1, &sm.abort) && mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, &sm.abort);
+                if (!ok) break;
+                tc_after();
+                pv(w, j);
+                if (w == nw - 1) umma_commit(&sm.v_empty[j & 1]);
+                if (j + 1 < n) {
+                    ok = mbar_wait(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, &sm.abort);
+                    if (!ok) break;
+                    tc_after();
+                    qk(w, j + 1);
+                    if (w == nw - 1) umma_commit(&sm.k_empty[(j + 1) & 1]);
+                } else {
+                    umma_commit(&sm.o_full[w]);
+                }
+            }
+        }
+        // nothing may be in flight when the TMEM goes
+        umma_commit(&sm.drain);
+        mbar_wait(&sm.drain, 0, nullptr);
+    }
+    __syncwarp();
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+bool smem_opt_in(const void *fn, size_t bytes) {
+    static thread_local std::vector<std::pair<const void *, int>> done;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    for (auto &d : done)
+        if (d.first == fn && d.second == dev) return true;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    done.push_back({ fn, dev });
+    return true;
+}
+
+template <int HD, int FMT, typename QT> int launch(const Kv8Attn &a, cudaStream_t st) {
+    auto fn = k_kv8_prefill<HD, FMT, QT>;
+    constexpr size_t bytes = sizeof(Smem<HD>);
+    static_assert(bytes <= 227 * 1024, "shared memory");
+    if (!smem_opt_in((const void *)fn, bytes)) return set_error(TLMG_EIO, "kv8_attend: shared memory opt-in failed");
+    const int64_t tiles = ((int64_t)a.b.max_q * a.G + 2 * TQ - 1) / (2 * TQ);
+    fn<<<dim3((unsigned)tiles, a.c.KV, a.b.n_seq), THREADS, bytes, st>>>(a);
+    count_launch();
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? TLMG_OK : cuda_fail(e, "kv8_attend launch");
+}
+template <int HD, int FMT> int launch_q(const Kv8Attn &a, int q_dt, cudaStream_t st) {
+    return q_dt == TLMG_DT_F16 ? launch<HD, FMT, __half>(a, st) : launch<HD, FMT, __nv_bfloat16>(a, st);
+}
+template <int HD> int launch_fmt(const Kv8Attn &a, int fmt, int q_dt, cudaStream_t st) {
+    return fmt == TLMG_KV8_INT8 ? launch_q<HD, TLMG_KV8_INT8>(a, q_dt, st) : launch_q<HD, TLMG_KV8_E4M3>(a, q_dt, st);
+}
+
+}  // namespace
+
+bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt) {
+    return q_dt != TLMG_DT_F32 && c.hd <= 128 && (int64_t)b.max_q * (H / c.KV) >= TQ;
+}
+
+int kv8_prefill(const Kv8Attn &a, int fmt, int q_dt, cudaStream_t st) {
+    return a.c.hd == 64 ? launch_fmt<64>(a, fmt, q_dt, st) : launch_fmt<128>(a, fmt, q_dt, st);
+}
+
+}  // namespace tlmg
