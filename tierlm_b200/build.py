@@ -32,6 +32,10 @@ NVCC_FLAGS = [
 # per-step device functions are compiled separately under the same cap.
 FILE_FLAGS = {"tlmg_fused.cu": ["-maxrregcount=96"]}
 
+# Compiled as whole programs: ptxas moves registers between a kernel's
+# warpgroups (setmaxnreg) only outside relocatable device code.
+WHOLE = {"tlmg_kv8_prefill.cu"}
+
 
 def nvcc() -> str:
     for cand in (os.environ.get("NVCC"), shutil.which("nvcc"), "/usr/local/cuda/bin/nvcc"):
@@ -64,7 +68,8 @@ def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> 
     objs = []
     for src in sources():
         obj = objdir / (src.stem + ".o")
-        cmd = [cc, *NVCC_FLAGS, *FILE_FLAGS.get(src.name, []), "-I", str(INCLUDE), "-dc", str(src), "-o", str(obj)]
+        cmd = [cc, *NVCC_FLAGS, *FILE_FLAGS.get(src.name, []), "-I", str(INCLUDE),
+               "-c" if src.name in WHOLE else "-dc", str(src), "-o", str(obj)]
         if ptxas_v:
             cmd[1:1] = ["-Xptxas", "-v"]
         if verbose:

@@ -3,10 +3,10 @@
 //
 // One CTA per SM takes 256 query rows (token, head of the group) of one KV
 // head in two tiles A and B of 128, and walks the visible keys in tiles of
-// 128. Roles, 13 warps:
+// 128. Roles, 16 warps:
 //   warps 0-3, 4-7  softmax of tile A, B: thread = query row = TMEM lane
 //   warps 8-11      K and V codes -> f16 in shared memory, once for both tiles
-//   warp 12         one thread issues the MMAs
+//   warps 12-15     the first issues the MMAs (a warpgroup, for its share of the registers)
 // Per key tile and query tile: S = Q K^T (8 x tcgen05.mma M128 N128 K16 at
 // hd 128, operands in shared memory, S f32 in TMEM); the softmax warps read S
 // and write P as f16 over it; O += P V (A operand P from TMEM, V from shared
@@ -44,7 +44,11 @@ namespace {
 
 constexpr int TK = 128;           // keys of a tile
 constexpr int TQ = 128;           // query rows of a tile
-constexpr int THREADS = 13 * 32;
+constexpr int THREADS = 16 * 32;
+// Registers a thread: 128 at launch (512 x 128 = the SM's 65,536), then 2 x 128 x 160 + 128 x 112 + 128 x 80 = 65,536.
+constexpr int REGS_SOFTMAX = 160, REGS_CONVERT = 112, REGS_MMA = 80;
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int META = 4;           // buffers of per-key scales
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -54,8 +58,9 @@ template <int HD> struct Smem {
     alignas(128) uint8_t q[2][TQ * HD * 2];
     alignas(128) uint8_t k[2][TK * HD * 2];
     alignas(128) uint8_t v[2][TK * HD * 2];
-    alignas(16) float ks[META][TK], vs[META][TK], lv[META][TK];
-    int pos[META][TK], doc[META][TK];
+    alignas(16) float ks[META][TK], vs[META][TK], lv[META][TK], rv[META][TK];   // scales; of V also log2 and 1 / scale
+    alignas(16) int pos[META][TK], doc[META][TK];
+    alignas(4) uint8_t tame[META][4];
     uint32_t row[2][TK];
     uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], meta_full[META], drain;
     uint32_t tmem;
@@ -70,6 +75,7 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *b) {
 }
 // Waits for phase `parity`; false when it did not come in about a second or another role gave up.
 __device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, int *abort) {
+#pragma unroll 1
     for (uint32_t i = 0; i < (1u << 20); i++) {
         uint32_t done;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
@@ -82,13 +88,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, int *abo
     if (abort) *(volatile int *)abort = 1;
     return false;
 }
+// The same with one outcome for a warp. (One lane polling and a shuffle of its result took 1.6 times as long over all:
+// a shuffle waits in the queue that the MMAs are issued through; 18k case 1,087 us, with the vote 1,004.)
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t *b, uint32_t parity, int *abort) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort));
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void umma_commit(uint64_t *b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(b)) : "memory");
-}
-
 // Shared-memory operand descriptor, no swizzle, version 1: start, leading and stride byte offsets.
 __device__ __forceinline__ uint64_t umma_desc(uint32_t start, uint32_t lbo, uint32_t sbo) {
     return (uint64_t)((start >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
@@ -98,18 +105,26 @@ __device__ __forceinline__ uint64_t umma_desc(uint32_t start, uint32_t lbo, uint
 constexpr uint32_t idesc(int n, bool b_mn) {
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TQ >> 4) << 24);
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+// The whole warp runs the issuing code, converged and on warp-uniform values (descriptors then live in uniform
+// registers); `lead` is set in one lane, which alone issues. Code that one lane runs by itself takes about 200 clocks
+// per MMA to move its operands, three times what the MMA takes.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t lead) {
     const uint32_t z = 0;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
-                 "l"(a), "l"(b), "r"(id), "r"(acc), "r"(z)
+    asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(id), "r"(acc), "r"(z), "r"(lead)
                  : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t lead) {
     const uint32_t z = 0;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
-                 "r"(a), "l"(b), "r"(id), "r"(acc), "r"(z)
+    asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(id), "r"(acc), "r"(z), "r"(lead)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t *b, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(saddr(b)), "r"(lead)
                  : "memory");
 }
 
@@ -126,6 +141,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
                  : TLMG_R32(TLMG_OUT)
                  : "r"(addr)
                  : "memory");
+}
+__device__ __forceinline__ void tmem_ld4(uint32_t addr, uint32_t (&v)[4]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];\n\ttcgen05.wait::ld.sync.aligned;\n"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&v)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0, %1, %2, %3};\n" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st2(uint32_t addr, const uint32_t (&v)[2]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%2], {%0, %1};\n" ::"r"(v[0]), "r"(v[1]), "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
@@ -180,9 +208,22 @@ __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// tanh(x) = x (c0 + c1 x^2 + .. + c5 x^10) for |x| < TANH_X within 2e-7: fitted (reweighted least squares towards the
+// smallest maximum) to tanh(x) / x over x^2 in [0, TANH_X^2]. Two issue slots and a half an element; the exponential
+// form takes two of the slower special-function results.
+constexpr float TANH_X = 0.8f;
+__device__ constexpr float TANH_C[6] = { 0.9999999403953552f, -0.33332714438438416f, 0.13321532309055328f, -0.05313541740179062f, 0.019130872562527657f, -0.004378729499876499f };
+
+// softcap * log2(e) * tanh(y) by the exponential
+__device__ __forceinline__ float cap_exp(float y, float capl) {
+    return __fmaf_rn(-2.0f * capl, __fdividef(1.0f, ex2(y * (2.0f * LOG2E)) + 1.0f), capl);
+}
+
 constexpr float TOP = 14.0f;   // log2 of the largest p * v_scale right after a row's reference moved
 
-template <int HD, int FMT, typename QT>
+// SHAPED: softcap, slopes, documents or a position pool; without them the code is half the size, and the instruction
+// cache is what these roles share most tightly.
+template <int HD, int FMT, typename QT, bool SHAPED>
 __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constant__ Kv8Attn a) {
     extern __shared__ __align__(128) uint8_t raw[];
     Smem<HD> &sm = *reinterpret_cast<Smem<HD> *>(raw);
@@ -190,14 +231,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     constexpr int PC = HD / 16;               // 16-byte pieces of a code row
     constexpr int NP = TK * PC / 128;         // pieces of a tile per converting thread
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int s = blockIdx.z, kvh = blockIdx.y;
-    const int rt = gridDim.x - 1 - blockIdx.x;   // the last tokens see the most keys: they go first
+    const int s = blockIdx.y, kvh = blockIdx.x % a.c.KV;
+    const int tiles = gridDim.x / a.c.KV, rt = tiles - 1 - blockIdx.x / a.c.KV;   // the last tokens see the most keys: first
     QT *out = static_cast<QT *>(a.out);
     Kv8Seq q;
     if (!kv8_seq(a.b, a.c.lp, s, q)) {
         const float nan = __uint_as_float(0x7FC00000u);
         const int64_t i0 = max(q.q0, 0), i1 = min((int64_t)a.b.q_start[s + 1], (int64_t)a.b.total_q);
-        for (int64_t R = (int64_t)blockIdx.x * (THREADS / 32) + warp; R < (i1 - i0) * a.G; R += (int64_t)gridDim.x * (THREADS / 32)) {
+        for (int64_t R = (int64_t)rt * (THREADS / 32) + warp; R < (i1 - i0) * a.G; R += (int64_t)tiles * (THREADS / 32)) {
             const int64_t row = (i0 + R / a.G) * a.H + kvh * a.G + R % a.G;
             for (int d = 4 * lane; d < HD; d += 128) kv8_st4(out + row * HD + d, make_float4(nan, nan, nan, nan));
             if (lane == 0 && a.lse) a.lse[row] = nan;
@@ -214,8 +255,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
         sm.pmax = INT32_MIN;
         mbar_init(&sm.q_full, two ? 2 * TQ : TQ);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sm.k_full[i], 128);
-            mbar_init(&sm.v_full[i], 128);
+            mbar_init(&sm.k_full[i], 64);
+            mbar_init(&sm.v_full[i], 64);
             mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_empty[i], 1);
             mbar_init(&sm.s_full[i], 1);
@@ -247,6 +288,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
 
     if (warp < 8) {
         // ---- softmax of one query tile ----
+        regs_up<REGS_SOFTMAX>();
         const int w = warp >> 2, r = tid & (TQ - 1);
         if (w == 0 || two) {
             const int R = R0 + w * TQ + r;
@@ -280,134 +322,210 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             }
             const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // this warp's 32 TMEM lanes
             const uint32_t ts = tmem + lanes + w * TK, to = tmem + lanes + 2 * TK + w * HD;
-            const bool shaped = a.softcap > 0.0f || a.slopes || docs || a.c.pos;
-            const float qs2 = qsc * LOG2E, capl = a.softcap * LOG2E, capx = qsc * a.inv_cap * 2.0f * LOG2E;
-            const f2 q2 = pk(qs2, qs2);
-            float wref = -INFINITY;
-            f2 sum0 = pk(0.0f, 0.0f), sum1 = pk(0.0f, 0.0f);
+            const bool lists = SHAPED && (docs || a.c.pos);        // masks that go by a table
+            const float qs2 = qsc * LOG2E, capl = a.softcap * LOG2E, capx = qsc * a.inv_cap;
+            const float mul = SHAPED && a.softcap > 0.0f ? capx : qs2;
+            float wref = -INFINITY, lsum = 0.0f;
             bool ok = true;
+#pragma unroll 1
             for (int j = 0; j < n; j++) {
                 const int t0 = rg.t0(j), mb = j & (META - 1);
-                ok = mbar_wait(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait(&sm.s_full[w], j & 1, &sm.abort);
-                ok = __all_sync(0xFFFFFFFFu, ok);
+                ok = mbar_wait_warp(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait_warp(&sm.s_full[w], j & 1, &sm.abort);
                 if (!ok) break;
                 tc_after();
-                const float4 *ks4 = reinterpret_cast<const float4 *>(sm.ks[mb]), *vs4 = reinterpret_cast<const float4 *>(sm.vs[mb]),
-                             *lv4 = reinterpret_cast<const float4 *>(sm.lv[mb]);
-                // every key of the tile is seen by every row of the CTA, its score is a plain product
-                const bool plain = !shaped && t0 + TK <= q.L && (!a.causal || t0 + TK - 1 <= pmin) && (!a.window || pmax - t0 < a.window);
-                float m0 = -INFINITY, m1 = -INFINITY;
-                if (plain) {
+                const float *ks = sm.ks[mb], *vs = sm.vs[mb], *lv = sm.lv[mb];
+                // every key of the tile is seen by every row of the CTA
+                const bool open = !lists && t0 + TK <= q.L && (!a.causal || t0 + TK - 1 <= pmin) && (!a.window || pmax - t0 < a.window);
+                // one scale for 8 keys, none of them extreme: the scales come in per group
+                const bool grp = a.c.lb >= 3 && *reinterpret_cast<const uint32_t *>(sm.tame[mb]) == 0x01010101u;
+                const bool rawS = open && grp && !(SHAPED && (a.softcap > 0.0f || a.slopes));
+                // Without tables a row sees the columns below c_pre and those in [c_lo, c_hi).
+                const int c_hi = min(a.causal ? (qp >= t0 + TK ? TK : qp + 1 - t0) : TK, q.L - t0);
+                const int c_lo = a.window ? (int)max((int64_t)qp - a.window + 1 - t0, (int64_t)0) : 0;
+                const int c_pre = min(pre - t0, q.L - t0);
+                float m0 = -INFINITY;
+                uint32_t xa[32];
+                if (rawS) {
+#pragma unroll 1
+                    for (int c = 0; c < TK; c += 32) {
+                        tmem_ld32(ts + c, xa);
 #pragma unroll
-                    for (int c = 0; c < TK / 32; c++) {
-                        uint32_t x[32];
-                        tmem_ld32(ts + 32 * c, x);
+                        for (int g = 0; g < 32; g += 8) {
+                            float y = __uint_as_float(xa[g]), y1 = __uint_as_float(xa[g + 1]);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float4 k = ks4[8 * c + i], l = lv4[8 * c + i];
-                            float y0, y1, y2, y3;
-                            upk(fma2(mul2(pku(x[4 * i], x[4 * i + 1]), pk(k.x, k.y)), q2, pk(l.x, l.y)), y0, y1);
-                            upk(fma2(mul2(pku(x[4 * i + 2], x[4 * i + 3]), pk(k.z, k.w)), q2, pk(l.z, l.w)), y2, y3);
-                            m0 = fmaxf(m0, fmaxf(y0, y1));
-                            m1 = fmaxf(m1, fmaxf(y2, y3));
+                            for (int i = 2; i < 8; i += 2) {
+                                y = fmaxf(y, __uint_as_float(xa[g + i]));
+                                y1 = fmaxf(y1, __uint_as_float(xa[g + i + 1]));
+                            }
+                            m0 = fmaxf(m0, __fmaf_rn(fmaxf(y, y1), ks[c + g] * qs2, lv[c + g]));
                         }
                     }
-                } else {
+                } else if (grp) {
                     // scores in log2 units, masked ones -inf, written back over S
 #pragma unroll 1
-                    for (int c = 0; c < TK / 32; c++) {
-                        uint32_t x[32];
-                        tmem_ld32(ts + 32 * c, x);
+                    for (int c = 0; c < TK; c += 32) {
+                        // (the flags are made to look new in every round: the compiler would copy the loop for each of them)
+                        int cap = SHAPED && a.softcap > 0.0f, ali = SHAPED && a.slopes, by_pos = SHAPED && a.c.pos, by_doc = SHAPED && docs, shut = !open;
+                        if constexpr (SHAPED) asm volatile("" : "+r"(cap), "+r"(ali), "+r"(by_pos), "+r"(by_doc), "+r"(shut));
+                        tmem_ld32(ts + c, xa);
+                        float z[32];
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const int col = 32 * c + i, t = t0 + col;
-                            const int kp = a.c.pos ? sm.pos[mb][col] : t;
-                            float z = __uint_as_float(x[i]) * sm.ks[mb][col];
-                            if (a.softcap > 0.0f) {   // tanh(y) = 1 - 2 / (e^2y + 1)
-                                const float e = ex2(z * capx);
-                                z = __fmaf_rn(-2.0f * capl, __fdividef(1.0f, e + 1.0f), capl);
-                            } else {
-                                z *= qs2;
+                        for (int g = 0; g < 32; g += 8) {
+                            const float k = ks[c + g] * mul;
+#pragma unroll
+                            for (int i = 0; i < 8; i++) z[g + i] = __uint_as_float(xa[g + i]) * k;
+                        }
+                        if (cap) {
+                            float big = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 32; i++) big = fmaxf(big, fabsf(z[i]));
+                            if (__all_sync(0xFFFFFFFFu, big < TANH_X)) {   // (a NaN may pass: the polynomial keeps it)
+                                const f2 cl = pk(capl, capl);
+#pragma unroll
+                                for (int i = 0; i < 32; i += 2) {
+                                    const f2 y = pk(z[i], z[i + 1]), y2 = mul2(y, y);
+                                    f2 r = pk(TANH_C[5], TANH_C[5]);
+#pragma unroll
+                                    for (int k = 4; k >= 0; k--) r = fma2(r, y2, pk(TANH_C[k], TANH_C[k]));
+                                    upk(mul2(mul2(r, y), cl), z[i], z[i + 1]);
+                                }
+                            } else {   // tanh(y) = 1 - 2 / (e^2y + 1)
+#pragma unroll
+                                for (int i = 0; i < 32; i++) z[i] = cap_exp(z[i], capl);
                             }
-                            if (a.slopes) z = __fmaf_rn(-slope, fabsf((float)(qp - kp)), z);
+                        }
+                        if (ali) {
+                            if (by_pos) {
+#pragma unroll
+                                for (int i = 0; i < 32; i++) z[i] = __fmaf_rn(-slope, fabsf((float)(qp - sm.pos[mb][c + i])), z[i]);
+                            } else {
+                                const float far = (float)(qp - t0 - c);
+#pragma unroll
+                                for (int i = 0; i < 32; i++) z[i] = __fmaf_rn(-slope, fabsf(far - (float)i), z[i]);
+                            }
+                        }
+                        if (shut) {
+                            const int lo = c_lo - c, hi = c_hi - c, pr = c_pre - c;
+                            if (by_pos) {
+#pragma unroll
+                                for (int i = 0; i < 32; i++) {
+                                    const int kp = sm.pos[mb][c + i];
+                                    const bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
+                                    z[i] = see && t0 + c + i < q.L ? z[i] : -INFINITY;
+                                }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 32; i++) z[i] = (i >= lo && i < hi) || i < pr ? z[i] : -INFINITY;
+                            }
+                            if (by_doc) {
+#pragma unroll
+                                for (int i = 0; i < 32; i += 4) {
+                                    const int4 d = *reinterpret_cast<const int4 *>(&sm.doc[mb][c + i]);
+                                    z[i] = d.x == qd ? z[i] : -INFINITY;
+                                    z[i + 1] = d.y == qd ? z[i + 1] : -INFINITY;
+                                    z[i + 2] = d.z == qd ? z[i + 2] : -INFINITY;
+                                    z[i + 3] = d.w == qd ? z[i + 3] : -INFINITY;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int g = 0; g < 32; g += 8) {
+                            float y = z[g], y1 = z[g + 1];
+#pragma unroll
+                            for (int i = 2; i < 8; i += 2) y = fmaxf(y, z[g + i]), y1 = fmaxf(y1, z[g + i + 1]);
+                            m0 = fmaxf(m0, fmaxf(y, y1) + lv[c + g]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; i++) xa[i] = __float_as_uint(z[i]);
+                        tmem_st32(ts + c, xa);
+                    }
+                    tmem_wait_st();
+                } else {
+                    // scales of single keys: the same, four columns a round
+#pragma unroll 1
+                    for (int c = 0; c < TK; c += 4) {
+                        uint32_t x[4];
+                        tmem_ld4(ts + c, x);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int col = c + i, t = t0 + col, kp = SHAPED && a.c.pos ? sm.pos[mb][col] : t;
+                            float z = __uint_as_float(x[i]) * (ks[col] * mul);
+                            if (SHAPED && a.softcap > 0.0f) z = cap_exp(z, capl);
+                            if (SHAPED && a.slopes) z = __fmaf_rn(-slope, fabsf((float)(qp - kp)), z);
                             bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
-                            see = see && t < q.L && (!docs || sm.doc[mb][col] == qd);
+                            see = see && t < q.L && (!(SHAPED && docs) || sm.doc[mb][col] == qd);
                             z = see ? z : -INFINITY;
-                            m0 = fmaxf(m0, z + sm.lv[mb][col]);
+                            m0 = fmaxf(m0, z + lv[col]);
                             x[i] = __float_as_uint(z);
                         }
-                        tmem_st32(ts + 32 * c, x);
+                        tmem_st4(ts + c, x);
                     }
                     tmem_wait_st();
                 }
-                m0 = fmaxf(m0, m1);
                 const bool grow = m0 > wref + 1.0f;
                 if (__any_sync(0xFFFFFFFFu, grow)) {
                     const float f = grow && wref != -INFINITY ? ex2(wref - m0) : 1.0f;
                     if (grow) wref = m0;
-                    const f2 f2v = pk(f, f);
-                    sum0 = mul2(sum0, f2v);
-                    sum1 = mul2(sum1, f2v);
+                    lsum *= f;
                     if (j > 0) {
 #pragma unroll 1
-                        for (int c = 0; c < HD / 32; c++) {
-                            uint32_t x[32];
-                            tmem_ld32(to + 32 * c, x);
+                        for (int c = 0; c < HD; c += 32) {
+                            tmem_ld32(to + c, xa);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
-                            tmem_st32(to + 32 * c, x);
+                            for (int i = 0; i < 32; i++) xa[i] = __float_as_uint(__uint_as_float(xa[i]) * f);
+                            tmem_st32(to + c, xa);
                         }
                         tmem_wait_st();
                     }
                 }
                 const float sub = wref == -INFINITY ? 0.0f : TOP - wref;
-                const f2 sub2 = pk(sub, sub);
+                if (grp) {
+                    // p * v_scale = 2^(score + sub + log2 v_scale); the group's sum over v_scale is the sum of its p
+#pragma unroll 1
+                    for (int c = 0; c < TK; c += 32) {
+                        uint32_t p[16];
+                        tmem_ld32(ts + c, xa);
 #pragma unroll
-                for (int c = 0; c < TK / 32; c++) {
-                    uint32_t x[32], p[16];
-                    tmem_ld32(ts + 32 * c, x);
+                        for (int g = 0; g < 32; g += 8) {
+                            const float k = rawS ? ks[c + g] * qs2 : 1.0f, off = sub + lv[c + g];
+                            const f2 k2 = pk(k, k), o2 = pk(off, off);
+                            float y[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float4 v = vs4[8 * c + i];
-                        f2 e0, e1;
-                        if (plain) {
-                            const float4 k = ks4[8 * c + i];
-                            e0 = fma2(mul2(pku(x[4 * i], x[4 * i + 1]), pk(k.x, k.y)), q2, sub2);
-                            e1 = fma2(mul2(pku(x[4 * i + 2], x[4 * i + 3]), pk(k.z, k.w)), q2, sub2);
-                        } else {
-                            e0 = add2(pku(x[4 * i], x[4 * i + 1]), sub2);
-                            e1 = add2(pku(x[4 * i + 2], x[4 * i + 3]), sub2);
+                            for (int i = 0; i < 8; i += 2) {
+                                upk(fma2(pku(xa[g + i], xa[g + i + 1]), k2, o2), y[i], y[i + 1]);
+                                y[i] = ex2(y[i]), y[i + 1] = ex2(y[i + 1]);
+                                p[(g + i) / 2] = pack_f16(y[i], y[i + 1]);
+                            }
+                            float u0, u1;
+                            upk(add2(add2(pk(y[0], y[1]), pk(y[2], y[3])), add2(pk(y[4], y[5]), pk(y[6], y[7]))), u0, u1);
+                            lsum = __fmaf_rn(u0 + u1, sm.rv[mb][c + g], lsum);
                         }
-                        float y0, y1, y2, y3;
-                        upk(e0, y0, y1);
-                        upk(e1, y2, y3);
-                        const f2 p0 = pk(ex2(y0), ex2(y1)), p1 = pk(ex2(y2), ex2(y3));
-                        sum0 = add2(sum0, p0);
-                        sum1 = add2(sum1, p1);
-                        float u0, u1, u2, u3;
-                        upk(mul2(p0, pk(v.x, v.y)), u0, u1);
-                        upk(mul2(p1, pk(v.z, v.w)), u2, u3);
-                        if (!plain) {   // a masked key's scale has no part in this, whatever it is
-                            u0 = y0 == -INFINITY ? 0.0f : u0;
-                            u1 = y1 == -INFINITY ? 0.0f : u1;
-                            u2 = y2 == -INFINITY ? 0.0f : u2;
-                            u3 = y3 == -INFINITY ? 0.0f : u3;
-                        }
-                        p[2 * i] = pack_f16(u0, u1);
-                        p[2 * i + 1] = pack_f16(u2, u3);
+                        tmem_st16(ts + c / 2, p);   // columns whose scores are read already
                     }
-                    tmem_st16(ts + 16 * c, p);   // columns whose scores are read already
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < TK; c += 4) {
+                        uint32_t x[4], p[2];
+                        tmem_ld4(ts + c, x);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float y = __uint_as_float(x[i]), e = ex2(y + sub);
+                            lsum += e;
+                            // a masked key's scale has no part in this, whatever it is
+                            x[i] = __float_as_uint(y == -INFINITY ? 0.0f : e * vs[c + i]);
+                        }
+                        p[0] = pack_f16(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                        p[1] = pack_f16(__uint_as_float(x[2]), __uint_as_float(x[3]));
+                        tmem_st2(ts + c / 2, p);
+                    }
                 }
                 tmem_wait_st();
                 tc_before();
                 mbar_arrive(&sm.p_full[w]);
             }
-            if (ok && n > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.o_full[w], 0, &sm.abort));
+            if (ok && n > 0) ok = mbar_wait_warp(&sm.o_full[w], 0, &sm.abort);
             tc_after();
-            float l0, l1, l2, l3;
-            upk(sum0, l0, l1);
-            upk(sum1, l2, l3);
-            const float l = (l0 + l1) + (l2 + l3);
+            const float l = lsum;
             const float inv = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? 0.0f : __fdividef(kv8_f16_unit<FMT>(), l);
 #pragma unroll 1
             for (int c = 0; c < HD / 32; c++) {
@@ -429,12 +547,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
         }
     } else if (warp < 12) {
         // ---- codes to f16 ----
+        regs_down<REGS_CONVERT>();
         const int c = tid - 256;
-        const int prow = (c & 7) + 8 * (c / (8 * PC)), piece = (c >> 3) % PC;   // first row and piece of this thread
-        constexpr int RSTEP = 8 * (128 / (8 * PC));                            // its next row
+        const bool is_v = c >= 64;                // two warps convert K, two V: the same code
+        const int h = c & 63;
+        const int prow = (h & 7) + 8 * (h / (8 * PC)), piece = (h >> 3) % PC;   // first row and piece of this thread
+        constexpr int RSTEP = 8 * (64 / (8 * PC));                             // its next row
+        const uint8_t *pool = is_v ? a.c.v : a.c.k;
+        uint8_t *dst0 = (is_v ? sm.v[0] : sm.k[0]) + (prow >> 3) * SBO + piece * 256 + (prow & 7) * 16;
+        uint64_t *full = is_v ? sm.v_full : sm.k_full, *empty = is_v ? sm.v_empty : sm.k_empty;
         const int32_t *table = a.b.page_table + (size_t)s * a.b.table_stride;
         const float nan = __uint_as_float(0x7FC00000u);
-        uint4 kr[NP], vr[NP];
+        uint4 xa[NP], xb[NP];
         int32_t te = -1, te_next = -1;
         auto entry = [&](int j) {
             if (j >= n) return -1;
@@ -448,8 +572,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             const bool have = t < q.L && a.c.ok(e);
             const uint32_t rid = have ? a.c.row(e, kvh, t) : 0xFFFFFFFFu;
             sm.row[j & 1][c] = rid;
-            mk = have ? __ldg(a.c.ks + (rid >> a.c.lb)) : nan;
-            mv = have ? __ldg(a.c.vs + (rid >> a.c.lb)) : nan;
+            const float none = t < q.L ? nan : 1.0f;   // a bad page: NaN for whoever sees it
+            mk = have ? __ldg(a.c.ks + (rid >> a.c.lb)) : none;
+            mv = have ? __ldg(a.c.vs + (rid >> a.c.lb)) : none;
             if (a.c.pos) mp = have ? __ldg(a.c.pos + rid) : 0;
             if (docs) {
                 const int p = a.c.pos ? mp : t;
@@ -460,28 +585,29 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             const int mb = j & (META - 1);
             sm.ks[mb][c] = mk;
             sm.vs[mb][c] = mv;
-            sm.lv[mb][c] = fmaxf(log2f(mv), -60.0f);
+            sm.lv[mb][c] = fmaxf(__log2f(mv), -60.0f);
+            sm.rv[mb][c] = __fdividef(1.0f, mv);
+            const bool tame = __all_sync(0xFFFFFFFFu, mv > 0x1p-60f && mv < 0x1p60f);
+            if (lane == 0) sm.tame[mb][warp - 8] = tame;
             sm.pos[mb][c] = mp;
             sm.doc[mb][c] = md;
             mbar_arrive(&sm.meta_full[mb]);
         };
-        auto load = [&](const uint8_t *pool, int j, uint4 (&x)[NP]) {
+        auto load = [&](int j, int i0, uint4 (&x)[NP]) {   // pieces i0 .. i0 + NP - 1 of the thread
 #pragma unroll
             for (int i = 0; i < NP; i++) {
-                const uint32_t rid = sm.row[j & 1][prow + RSTEP * i];
+                const uint32_t rid = sm.row[j & 1][prow + RSTEP * (i0 + i)];
                 x[i] = rid != 0xFFFFFFFFu ? __ldg(reinterpret_cast<const uint4 *>(pool + (size_t)rid * HD + 16 * piece)) : make_uint4(0, 0, 0, 0);
             }
         };
-        auto convert = [&](uint8_t *dst, const uint4 (&x)[NP]) {
+        auto convert = [&](int j, int i0, const uint4 (&x)[NP]) {
+            uint8_t *d = dst0 + (j & 1) * (TK * HD * 2) + i0 * (RSTEP / 8) * SBO;
 #pragma unroll
-            for (int i = 0; i < NP; i++) {
-                const int r = prow + RSTEP * i;
-                uint8_t *d = dst + (r >> 3) * SBO + piece * 256 + (r & 7) * 16;
+            for (int i = 0; i < NP; i++, d += RSTEP / 8 * SBO) {
                 const uint32_t b0 = kv8_bias<FMT>(x[i].x), b1 = kv8_bias<FMT>(x[i].y), b2 = kv8_bias<FMT>(x[i].z), b3 = kv8_bias<FMT>(x[i].w);
                 *reinterpret_cast<uint4 *>(d) = make_uint4(kv8_half2<FMT, 0>(b0), kv8_half2<FMT, 1>(b0), kv8_half2<FMT, 0>(b1), kv8_half2<FMT, 1>(b1));
                 *reinterpret_cast<uint4 *>(d + 128) = make_uint4(kv8_half2<FMT, 0>(b2), kv8_half2<FMT, 1>(b2), kv8_half2<FMT, 0>(b3), kv8_half2<FMT, 1>(b3));
             }
-            fence_async_smem();
         };
         auto bar = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
         bool ok = true;
@@ -489,76 +615,84 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             rows_of(0, entry(0));
             te = entry(1);
             bar();
-            load(a.c.k, 0, kr);
-            load(a.c.v, 0, vr);
+            load(0, 0, xa);
+            load(0, NP, xb);
             put_meta(0);
         }
+#pragma unroll 1
         for (int j = 0; j < n; j++) {
             te_next = entry(j + 2);
-            // after a wait that ran out the thread goes on to the barriers, without work
-            if (j >= 2) ok = mbar_wait(&sm.k_empty[j & 1], ((j >> 1) - 1) & 1, &sm.abort) && ok;
-            if (ok) {
-                convert(sm.k[j & 1], kr);
-                mbar_arrive(&sm.k_full[j & 1]);
-                if (j + 1 < n) rows_of(j + 1, te);
-            }
+            // row numbers of the next tile while this one waits for its buffer
+            if (j + 1 < n) rows_of(j + 1, te);
             te = te_next;
             bar();
-            if (ok && j + 1 < n) load(a.c.k, j + 1, kr);
-            if (j >= 2) ok = mbar_wait(&sm.v_empty[j & 1], ((j >> 1) - 1) & 1, &sm.abort) && ok;
+            // after a wait that ran out the thread goes on to the barriers, without work
+            if (j >= 2) ok = mbar_wait_warp(&empty[j & 1], ((j >> 1) - 1) & 1, &sm.abort) && ok;
             if (ok) {
-                convert(sm.v[j & 1], vr);
-                mbar_arrive(&sm.v_full[j & 1]);
+                convert(j, 0, xa);
+                if (j + 1 < n) load(j + 1, 0, xa);
+                convert(j, NP, xb);
+                fence_async_smem();
+                mbar_arrive(&full[j & 1]);
                 if (j + 1 < n) {
-                    load(a.c.v, j + 1, vr);
+                    load(j + 1, NP, xb);
                     put_meta(j + 1);
                 }
             }
         }
-    } else if (lane == 0) {
+    } else {
         // ---- MMAs ----
-        constexpr uint32_t id_qk = idesc(TK, false), id_pv = idesc(HD, true);
-        auto qk = [&](int w, int j) {
-            const uint32_t qa = saddr(sm.q[w]), ka = saddr(sm.k[j & 1]);
+        regs_down<REGS_MMA>();
+        if (warp == 12) {
+            constexpr uint32_t id_qk = idesc(TK, false), id_pv = idesc(HD, true);
+            const uint32_t lead = lane == 0, tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+            const int nt = __shfl_sync(0xFFFFFFFFu, n, 0), nw = __shfl_sync(0xFFFFFFFFu, two ? 2 : 1, 0);
+            // operand descriptors of the first step; a step further is a constant added to the start address (16-byte units)
+            const uint64_t dq = umma_desc(saddr(sm.q[0]), 128, SBO), dk = umma_desc(saddr(sm.k[0]), 128, SBO),
+                           dv = umma_desc(saddr(sm.v[0]), SBO, 128);
+            constexpr int BUF = TK * HD * 2 / 16;   // from a first buffer to its second
+            auto qk = [&](int w, int j) {
+                const uint64_t qa = dq + w * BUF, ka = dk + (j & 1) * BUF;
 #pragma unroll
-            for (int k = 0; k < HD / 16; k++)
-                umma_ss(tmem + w * TK, umma_desc(qa + 256 * k, 128, SBO), umma_desc(ka + 256 * k, 128, SBO), id_qk, k > 0);
-            umma_commit(&sm.s_full[w]);
-        };
-        auto pv = [&](int w, int j) {
-            const uint32_t va = saddr(sm.v[j & 1]);
+                for (int k = 0; k < HD / 16; k++) umma_ss(tm + w * TK, qa + 16 * k, ka + 16 * k, id_qk, k > 0, lead);
+                umma_commit(&sm.s_full[w], lead);
+            };
+            auto pv = [&](int w, int j) {
+                const uint64_t va = dv + (j & 1) * BUF;
 #pragma unroll
-            for (int k = 0; k < TK / 16; k++)
-                umma_ts(tmem + 2 * TK + w * HD, tmem + w * TK + 8 * k, umma_desc(va + 2 * SBO * k, SBO, 128), id_pv, j > 0 || k > 0);
-        };
-        const int nw = two ? 2 : 1;
-        bool ok = n == 0 || (mbar_wait(&sm.q_full, 0, &sm.abort) && mbar_wait(&sm.k_full[0], 0, &sm.abort));
-        if (ok && n > 0) {
-            tc_after();
-            for (int w = 0; w < nw; w++) qk(w, 0);
-            umma_commit(&sm.k_empty[0]);
-        }
-        for (int j = 0; ok && j < n; j++) {
-            for (int w = 0; ok && w < nw; w++) {
-                ok = mbar_wait(&sm.p_full[w], j & 1, &sm.abort) && mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, &sm.abort);
-                if (!ok) break;
+                for (int k = 0; k < TK / 16; k++)
+                    umma_ts(tm + 2 * TK + w * HD, tm + w * TK + 8 * k, va + 2 * SBO / 16 * k, id_pv, j > 0 || k > 0, lead);
+            };
+            bool ok = nt == 0 || (mbar_wait(&sm.q_full, 0, &sm.abort) && mbar_wait(&sm.k_full[0], 0, &sm.abort));
+            if (ok && nt > 0) {
                 tc_after();
-                pv(w, j);
-                if (w == nw - 1) umma_commit(&sm.v_empty[j & 1]);
-                if (j + 1 < n) {
-                    ok = mbar_wait(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, &sm.abort);
+                for (int w = 0; w < nw; w++) qk(w, 0);
+                umma_commit(&sm.k_empty[0], lead);
+            }
+#pragma unroll 1
+            for (int j = 0; ok && j < nt; j++) {
+#pragma unroll 1
+                for (int w = 0; ok && w < nw; w++) {
+                    ok = mbar_wait(&sm.p_full[w], j & 1, &sm.abort) && mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, &sm.abort);
                     if (!ok) break;
                     tc_after();
-                    qk(w, j + 1);
-                    if (w == nw - 1) umma_commit(&sm.k_empty[(j + 1) & 1]);
-                } else {
-                    umma_commit(&sm.o_full[w]);
+                    pv(w, j);
+                    if (w == nw - 1) umma_commit(&sm.v_empty[j & 1], lead);
+                    if (j + 1 < nt) {
+                        ok = mbar_wait(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, &sm.abort);
+                        if (!ok) break;
+                        tc_after();
+                        qk(w, j + 1);
+                        if (w == nw - 1) umma_commit(&sm.k_empty[(j + 1) & 1], lead);
+                    } else {
+                        umma_commit(&sm.o_full[w], lead);
+                    }
                 }
             }
+            // nothing may be in flight when the TMEM goes
+            umma_commit(&sm.drain, lead);
+            mbar_wait(&sm.drain, 0, nullptr);
         }
-        // nothing may be in flight when the TMEM goes
-        umma_commit(&sm.drain);
-        mbar_wait(&sm.drain, 0, nullptr);
     }
     __syncwarp();
     tc_before();
@@ -581,16 +715,19 @@ bool smem_opt_in(const void *fn, size_t bytes) {
     return true;
 }
 
-template <int HD, int FMT, typename QT> int launch(const Kv8Attn &a, cudaStream_t st) {
-    auto fn = k_kv8_prefill<HD, FMT, QT>;
+template <int HD, int FMT, typename QT, bool SHAPED> int launch_shape(const Kv8Attn &a, cudaStream_t st) {
+    auto fn = k_kv8_prefill<HD, FMT, QT, SHAPED>;
     constexpr size_t bytes = sizeof(Smem<HD>);
     static_assert(bytes <= 227 * 1024, "shared memory");
     if (!smem_opt_in((const void *)fn, bytes)) return set_error(TLMG_EIO, "kv8_attend: shared memory opt-in failed");
     const int64_t tiles = ((int64_t)a.b.max_q * a.G + 2 * TQ - 1) / (2 * TQ);
-    fn<<<dim3((unsigned)tiles, a.c.KV, a.b.n_seq), THREADS, bytes, st>>>(a);
+    fn<<<dim3((unsigned)(tiles * a.c.KV), a.b.n_seq), THREADS, bytes, st>>>(a);
     count_launch();
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? TLMG_OK : cuda_fail(e, "kv8_attend launch");
+}
+template <int HD, int FMT, typename QT> int launch(const Kv8Attn &a, cudaStream_t st) {
+    return a.softcap > 0.0f || a.slopes || a.doc || a.c.pos ? launch_shape<HD, FMT, QT, true>(a, st) : launch_shape<HD, FMT, QT, false>(a, st);
 }
 template <int HD, int FMT> int launch_q(const Kv8Attn &a, int q_dt, cudaStream_t st) {
     return q_dt == TLMG_DT_F16 ? launch<HD, FMT, __half>(a, st) : launch<HD, FMT, __nv_bfloat16>(a, st);
