@@ -3,10 +3,10 @@
 //
 // One CTA per SM takes 256 query rows (token, head of the group) of one KV
 // head in two tiles A and B of 128, and walks the visible keys in tiles of
-// 128. Roles, 16 warps:
+// 128. Roles, 20 warps:
 //   warps 0-3, 4-7  softmax of tile A, B: thread = query row = TMEM lane
-//   warps 8-11      K and V codes -> f16 in shared memory, once for both tiles
-//   warps 12-15     the first issues the MMAs (a warpgroup, for its share of the registers)
+//   warps 8-15      K and V codes -> f16 in shared memory, once for both tiles
+//   warps 16-19     the first issues the MMAs (a warpgroup, for its share of the registers)
 // Per key tile and query tile: S = Q K^T (8 x tcgen05.mma M128 N128 K16 at
 // hd 128, operands in shared memory, S f32 in TMEM); the softmax warps read S
 // and write P as f16 over it; O += P V (A operand P from TMEM, V from shared
@@ -44,9 +44,10 @@ namespace {
 
 constexpr int TK = 128;           // keys of a tile
 constexpr int TQ = 128;           // query rows of a tile
-constexpr int THREADS = 16 * 32;
-// Registers a thread: 128 at launch (512 x 128 = the SM's 65,536), then 2 x 128 x 160 + 128 x 112 + 128 x 80 = 65,536.
-constexpr int REGS_SOFTMAX = 160, REGS_CONVERT = 112, REGS_MMA = 80;
+constexpr int THREADS = 20 * 32;
+constexpr int CV = 256;           // converting threads
+// Registers a thread: 96 at launch (640 x 96 = 61,440), then 256 x 128 + 256 x 72 + 128 x 72 = 60,416.
+constexpr int REGS_SOFTMAX = 128, REGS_CONVERT = 72, REGS_MMA = 72;
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int META = 4;           // buffers of per-key scales
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     Smem<HD> &sm = *reinterpret_cast<Smem<HD> *>(raw);
     constexpr int SBO = HD * 16;              // bytes between 8-row groups of an operand
     constexpr int PC = HD / 16;               // 16-byte pieces of a code row
-    constexpr int NP = TK * PC / 128;         // pieces of a tile per converting thread
+    constexpr int NP = TK * PC / CV;          // pieces of half a tile per converting thread
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int s = blockIdx.y, kvh = blockIdx.x % a.c.KV;
     const int tiles = gridDim.x / a.c.KV, rt = tiles - 1 - blockIdx.x / a.c.KV;   // the last tokens see the most keys: first
@@ -255,8 +256,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
         sm.pmax = INT32_MIN;
         mbar_init(&sm.q_full, two ? 2 * TQ : TQ);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sm.k_full[i], 64);
-            mbar_init(&sm.v_full[i], 64);
+            mbar_init(&sm.k_full[i], CV / 2);
+            mbar_init(&sm.v_full[i], CV / 2);
             mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_empty[i], 1);
             mbar_init(&sm.s_full[i], 1);
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
         mbar_init(&sm.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -545,14 +546,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             }
             if (live && a.lse) a.lse[orow] = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? -INFINITY : (log2f(l) - (wref == -INFINITY ? 0.0f : TOP - wref)) * LN2;
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         // ---- codes to f16 ----
         regs_down<REGS_CONVERT>();
         const int c = tid - 256;
-        const bool is_v = c >= 64;                // two warps convert K, two V: the same code
-        const int h = c & 63;
+        const bool is_v = c >= CV / 2;            // half of the warps convert K, half V: the same code
+        const int h = c & (CV / 2 - 1);
         const int prow = (h & 7) + 8 * (h / (8 * PC)), piece = (h >> 3) % PC;   // first row and piece of this thread
-        constexpr int RSTEP = 8 * (64 / (8 * PC));                             // its next row
+        constexpr int RSTEP = 8 * (CV / 2 / (8 * PC));                             // its next row
         const uint8_t *pool = is_v ? a.c.v : a.c.k;
         uint8_t *dst0 = (is_v ? sm.v[0] : sm.k[0]) + (prow >> 3) * SBO + piece * 256 + (prow & 7) * 16;
         uint64_t *full = is_v ? sm.v_full : sm.k_full, *empty = is_v ? sm.v_empty : sm.k_empty;
@@ -561,13 +562,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
         uint4 xa[NP], xb[NP];
         int32_t te = -1, te_next = -1;
         auto entry = [&](int j) {
-            if (j >= n) return -1;
+            if (j >= n || c >= TK) return -1;
             const int t = rg.t0(j) + c;
             return t < q.L ? __ldg(table + (t >> a.c.lp)) : -1;
         };
         float mk = 0.0f, mv = 0.0f;
         int mp = 0, md = -1;
         auto rows_of = [&](int j, int32_t e) {   // row numbers of tile j; its scales into registers
+            if (c >= TK) return;
             const int t = rg.t0(j) + c;
             const bool have = t < q.L && a.c.ok(e);
             const uint32_t rid = have ? a.c.row(e, kvh, t) : 0xFFFFFFFFu;
@@ -582,6 +584,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             }
         };
         auto put_meta = [&](int j) {
+            if (c >= TK) return;
             const int mb = j & (META - 1);
             sm.ks[mb][c] = mk;
             sm.vs[mb][c] = mv;
@@ -609,7 +612,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                 *reinterpret_cast<uint4 *>(d + 128) = make_uint4(kv8_half2<FMT, 0>(b2), kv8_half2<FMT, 1>(b2), kv8_half2<FMT, 0>(b3), kv8_half2<FMT, 1>(b3));
             }
         };
-        auto bar = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+        auto bar = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
         bool ok = true;
         if (n > 0) {
             rows_of(0, entry(0));
@@ -643,7 +646,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     } else {
         // ---- MMAs ----
         regs_down<REGS_MMA>();
-        if (warp == 12) {
+        if (warp == 16) {
             constexpr uint32_t id_qk = idesc(TK, false), id_pv = idesc(HD, true);
             const uint32_t lead = lane == 0, tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
             const int nt = __shfl_sync(0xFFFFFFFFu, n, 0), nw = __shfl_sync(0xFFFFFFFFu, two ? 2 : 1, 0);
@@ -698,7 +701,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 bool smem_opt_in(const void *fn, size_t bytes) {
