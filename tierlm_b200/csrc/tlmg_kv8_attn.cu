@@ -735,6 +735,7 @@ extern "C" int tlmg_kv8_attend(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const
     a.b = *b;
     a.H = H;
     a.G = H / c->KV;
+    a.inv_g = a.G > 1 ? (uint32_t)((0x100000000ull + a.G - 1) / a.G) : 0u;
     a.q = q;
     a.q_stride = st;
     a.out = out;

@@ -10,6 +10,7 @@ struct Kv8Attn {
     Kv8View c;
     tlmg_kv8_batch b;
     int H, G;
+    uint32_t inv_g;   // ceil(2^32 / G); 0 for G = 1
     const void *q;
     int64_t q_stride;
     void *out;

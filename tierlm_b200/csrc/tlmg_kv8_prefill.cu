@@ -3,13 +3,13 @@
 //
 // One CTA per SM takes 256 query rows (token, head of the group) of one KV
 // head in two tiles A and B of 128, and walks the visible keys in tiles of
-// 128. Roles, 20 warps:
-//   warps 0-3, 4-7  softmax of tile A, B: thread = query row = TMEM lane
-//   warps 8-15      K and V codes -> f16 in shared memory, once for both tiles
-//   warps 16-19     the first issues the MMAs (a warpgroup, for its share of the registers)
+// 128. Roles, 28 warps:
+//   warps 0-7, 8-15  softmax of tile A, B: two threads per query row (= TMEM lane), each with half of the keys
+//   warps 16-23      K and V codes -> f16 in shared memory, once for both tiles
+//   warps 24-27      the first issues the MMAs (a warpgroup, for its share of the registers)
 // Per key tile and query tile: S = Q K^T (8 x tcgen05.mma M128 N128 K16 at
 // hd 128, operands in shared memory, S f32 in TMEM); the softmax warps read S
-// and write P as f16 over it; O += P V (A operand P from TMEM, V from shared
+// and write P as f16 over it (each half over its own columns); O += P V (A operand P from TMEM, V from shared
 // memory, O f32 in TMEM). While one tile's softmax runs, the tensor core
 // works for the other: TMEM is full at 2 x (S 128 + O 128) columns.
 //
@@ -44,10 +44,12 @@ namespace {
 
 constexpr int TK = 128;           // keys of a tile
 constexpr int TQ = 128;           // query rows of a tile
-constexpr int THREADS = 20 * 32;
+constexpr int THREADS = 28 * 32;
+constexpr int CK = 16;            // columns of a round of the softmax loops: few registers, four warps a scheduler
+constexpr int HC = TK / 2;        // keys of a softmax thread: two threads share a query row
 constexpr int CV = 256;           // converting threads
-// Registers a thread: 96 at launch (640 x 96 = 61,440), then 256 x 128 + 256 x 72 + 128 x 72 = 60,416.
-constexpr int REGS_SOFTMAX = 128, REGS_CONVERT = 72, REGS_MMA = 72;
+// Registers a thread: 72 at launch (896 x 72 = 64,512), then 512 x 80 + 256 x 56 + 128 x 72 = 64,512.
+constexpr int REGS_SOFTMAX = 80, REGS_CONVERT = 56, REGS_MMA = 72;
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int META = 4;           // buffers of per-key scales
@@ -63,7 +65,8 @@ template <int HD> struct Smem {
     alignas(16) int pos[META][TK], doc[META][TK];
     alignas(4) uint8_t tame[META][4];
     uint32_t row[2][TK];
-    uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], meta_full[META], drain;
+    float qs[2][TQ], part[2][2][TQ], sums[2][2][TQ];     // [tile][half][row]: the halves' maxima; in the end their sums
+    uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], x_full[2], o_full[2], meta_full[META], drain;
     uint32_t tmem;
     int abort, pmin, pmax;
 };
@@ -141,6 +144,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
                  "tcgen05.wait::ld.sync.aligned;\n"
                  : TLMG_R32(TLMG_OUT)
                  : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ldc(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+                 "[%16];\n\ttcgen05.wait::ld.sync.aligned;\n"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};\n" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr)
                  : "memory");
 }
 __device__ __forceinline__ void tmem_ld4(uint32_t addr, uint32_t (&v)[4]) {
@@ -246,29 +262,32 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
         }
         return;
     }
+    // R / G for the rows of a call (fewer than 2^20): the division's own code would be a good part of the start
+    auto token_of = [&](int R) { return (int)__umulhi((uint32_t)R, a.inv_g) + (a.G == 1 ? R : 0); };
     const int n_rows = q.n * a.G, R0 = rt * 2 * TQ;
     if (R0 >= n_rows) return;
     const bool two = R0 + TQ < n_rows;
-    const int i0 = R0 / a.G, i1 = min(q.n, (R0 + 2 * TQ - 1) / a.G + 1);
+    const int i0 = token_of(R0), i1 = min(q.n, token_of(R0 + 2 * TQ - 1) + 1);
     if (tid == 0) {
         sm.abort = 0;
         sm.pmin = INT32_MAX;
         sm.pmax = INT32_MIN;
-        mbar_init(&sm.q_full, two ? 2 * TQ : TQ);
+        mbar_init(&sm.q_full, two ? 4 * TQ : 2 * TQ);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sm.k_full[i], CV / 2);
             mbar_init(&sm.v_full[i], CV / 2);
             mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_empty[i], 1);
             mbar_init(&sm.s_full[i], 1);
-            mbar_init(&sm.p_full[i], TQ);
+            mbar_init(&sm.p_full[i], 2 * TQ);
+            mbar_init(&sm.x_full[i], 2 * TQ);
             mbar_init(&sm.o_full[i], 1);
         }
         for (int i = 0; i < META; i++) mbar_init(&sm.meta_full[i], 128);
         mbar_init(&sm.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 16) {
+    if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -287,49 +306,64 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     const int32_t *docs = a.doc ? a.doc + (size_t)s * a.doc_stride : nullptr;
     const int n = rg.n;
 
-    if (warp < 8) {
+    if (warp < 16) {
         // ---- softmax of one query tile ----
         regs_up<REGS_SOFTMAX>();
-        const int w = warp >> 2, r = tid & (TQ - 1);
+        const int w = warp >> 3, half = (warp >> 2) & 1, r = tid & (TQ - 1), k0 = half * HC;
         if (w == 0 || two) {
             const int R = R0 + w * TQ + r;
             const bool live = R < n_rows;
-            const int tok = live ? R / a.G : i0, h = kvh * a.G + (live ? R % a.G : 0);
+            const int tok = live ? token_of(R) : i0, h = kvh * a.G + (live ? R - tok * a.G : 0);
             const int qp = a.b.q_pos ? a.b.q_pos[q.q0 + tok] : q.L - q.n + tok;
             const int qd = docs ? (qp >= 0 && qp < a.doc_stride ? docs[qp] : -1) : -1;
             const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
             const int pre = a.prefix ? a.prefix[s] : 0;
             const int64_t orow = (q.q0 + (int64_t)tok) * a.H + h;
-            float qsc;
-            {   // the query row as f16, its largest element brought to 2^9 .. 2^10
-                const QT *x = static_cast<const QT *>(a.q) + (q.q0 + (int64_t)tok) * a.q_stride + (int64_t)h * HD;
-                float m = 0.0f;
-                for (int d = 0; d < HD; d += 4) {
-                    const float4 v = kv8_ld4(x + d);
-                    m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-                }
-                const int e = min(max((int)((__float_as_uint(m) >> 23) & 255u) - 136, -100), 100);
-                const float up = live ? __int_as_float((127 - e) << 23) : 0.0f;
-                qsc = __int_as_float((127 + e) << 23) * a.scale * kv8_f16_unit<FMT>();
-                uint8_t *dst = sm.q[w] + (r >> 3) * SBO + (r & 7) * 16;
-                for (int c = 0; c < HD / 8; c++) {
-                    const float4 v0 = kv8_ld4(x + 8 * c), v1 = kv8_ld4(x + 8 * c + 4);
-                    *reinterpret_cast<uint4 *>(dst + c * 128) =
-                        make_uint4(pack_f16(v0.x * up, v0.y * up), pack_f16(v0.z * up, v0.w * up),
-                                   pack_f16(v1.x * up, v1.y * up), pack_f16(v1.z * up, v1.w * up));
+            {   // query rows as f16, each row's largest element brought to 2^9 .. 2^10: a warp takes 8 rows at a time, four
+                // lanes a row, and writes 128 contiguous bytes per chunk
+                const int r8 = lane & 7, cq = lane >> 3;
+#pragma unroll 1
+                for (int g = 0; g < 2; g++) {
+                    uint4 x[HD / 32];
+                    const int rr = R0 + w * TQ + (warp & 7) * 16 + 8 * g + r8;
+                    const int tk = rr < n_rows ? token_of(rr) : i0, hh = kvh * a.G + (rr < n_rows ? rr - tk * a.G : 0);
+                    const QT *src = static_cast<const QT *>(a.q) + (q.q0 + (int64_t)tk) * a.q_stride + hh * HD + 8 * cq;
+#pragma unroll
+                    for (int i = 0; i < HD / 32; i++) x[i] = *reinterpret_cast<const uint4 *>(src + 32 * i);
+                    const int row = (warp & 7) * 16 + 8 * g + r8;
+                    float m = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < HD / 32; i++) {
+                        const float4 u = kv8_ld4(reinterpret_cast<const QT *>(&x[i])), v = kv8_ld4(reinterpret_cast<const QT *>(&x[i]) + 4);
+                        m = fmaxf(m, fmaxf(fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))),
+                                           fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)))));
+                    }
+                    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
+                    const int e = min(max((int)((__float_as_uint(m) >> 23) & 255u) - 136, -100), 100);
+                    const float up = R0 + w * TQ + row < n_rows ? __int_as_float((127 - e) << 23) : 0.0f;
+                    if (cq == 0) sm.qs[w][row] = __int_as_float((127 + e) << 23) * a.scale * kv8_f16_unit<FMT>();
+                    uint8_t *dst = sm.q[w] + (row >> 3) * SBO + (row & 7) * 16 + cq * 128;
+#pragma unroll
+                    for (int i = 0; i < HD / 32; i++) {
+                        const float4 u = kv8_ld4(reinterpret_cast<const QT *>(&x[i])), v = kv8_ld4(reinterpret_cast<const QT *>(&x[i]) + 4);
+                        *reinterpret_cast<uint4 *>(dst + 512 * i) = make_uint4(pack_f16(u.x * up, u.y * up), pack_f16(u.z * up, u.w * up),
+                                                                             pack_f16(v.x * up, v.y * up), pack_f16(v.z * up, v.w * up));
+                    }
                 }
                 fence_async_smem();
                 mbar_arrive(&sm.q_full);
             }
+            bool ok = mbar_wait_warp(&sm.q_full, 0, &sm.abort);
+            const float qsc = sm.qs[w][r];
             const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // this warp's 32 TMEM lanes
             const uint32_t ts = tmem + lanes + w * TK, to = tmem + lanes + 2 * TK + w * HD;
             const bool lists = SHAPED && (docs || a.c.pos);        // masks that go by a table
             const float qs2 = qsc * LOG2E, capl = a.softcap * LOG2E, capx = qsc * a.inv_cap;
             const float mul = SHAPED && a.softcap > 0.0f ? capx : qs2;
             float wref = -INFINITY, lsum = 0.0f;
-            bool ok = true;
 #pragma unroll 1
-            for (int j = 0; j < n; j++) {
+            for (int j = 0; ok && j < n; j++) {
                 const int t0 = rg.t0(j), mb = j & (META - 1);
                 ok = mbar_wait_warp(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait_warp(&sm.s_full[w], j & 1, &sm.abort);
                 if (!ok) break;
@@ -345,13 +379,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                 const int c_lo = a.window ? (int)max((int64_t)qp - a.window + 1 - t0, (int64_t)0) : 0;
                 const int c_pre = min(pre - t0, q.L - t0);
                 float m0 = -INFINITY;
-                uint32_t xa[32];
+                uint32_t xa[CK];
                 if (rawS) {
 #pragma unroll 1
-                    for (int c = 0; c < TK; c += 32) {
-                        tmem_ld32(ts + c, xa);
+                    for (int c = k0; c < k0 + HC; c += CK) {
+                        tmem_ldc(ts + c, xa);
 #pragma unroll
-                        for (int g = 0; g < 32; g += 8) {
+                        for (int g = 0; g < CK; g += 8) {
                             float y = __uint_as_float(xa[g]), y1 = __uint_as_float(xa[g + 1]);
 #pragma unroll
                             for (int i = 2; i < 8; i += 2) {
@@ -364,14 +398,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                 } else if (grp) {
                     // scores in log2 units, masked ones -inf, written back over S
 #pragma unroll 1
-                    for (int c = 0; c < TK; c += 32) {
+                    for (int c = k0; c < k0 + HC; c += CK) {
                         // (the flags are made to look new in every round: the compiler would copy the loop for each of them)
                         int cap = SHAPED && a.softcap > 0.0f, ali = SHAPED && a.slopes, by_pos = SHAPED && a.c.pos, by_doc = SHAPED && docs, shut = !open;
                         if constexpr (SHAPED) asm volatile("" : "+r"(cap), "+r"(ali), "+r"(by_pos), "+r"(by_doc), "+r"(shut));
-                        tmem_ld32(ts + c, xa);
-                        float z[32];
+                        tmem_ldc(ts + c, xa);
+                        float z[CK];
 #pragma unroll
-                        for (int g = 0; g < 32; g += 8) {
+                        for (int g = 0; g < CK; g += 8) {
                             const float k = ks[c + g] * mul;
 #pragma unroll
                             for (int i = 0; i < 8; i++) z[g + i] = __uint_as_float(xa[g + i]) * k;
@@ -379,11 +413,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                         if (cap) {
                             float big = 0.0f;
 #pragma unroll
-                            for (int i = 0; i < 32; i++) big = fmaxf(big, fabsf(z[i]));
+                            for (int i = 0; i < CK; i++) big = fmaxf(big, fabsf(z[i]));
                             if (__all_sync(0xFFFFFFFFu, big < TANH_X)) {   // (a NaN may pass: the polynomial keeps it)
                                 const f2 cl = pk(capl, capl);
 #pragma unroll
-                                for (int i = 0; i < 32; i += 2) {
+                                for (int i = 0; i < CK; i += 2) {
                                     const f2 y = pk(z[i], z[i + 1]), y2 = mul2(y, y);
                                     f2 r = pk(TANH_C[5], TANH_C[5]);
 #pragma unroll
@@ -392,35 +426,35 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                                 }
                             } else {   // tanh(y) = 1 - 2 / (e^2y + 1)
 #pragma unroll
-                                for (int i = 0; i < 32; i++) z[i] = cap_exp(z[i], capl);
+                                for (int i = 0; i < CK; i++) z[i] = cap_exp(z[i], capl);
                             }
                         }
                         if (ali) {
                             if (by_pos) {
 #pragma unroll
-                                for (int i = 0; i < 32; i++) z[i] = __fmaf_rn(-slope, fabsf((float)(qp - sm.pos[mb][c + i])), z[i]);
+                                for (int i = 0; i < CK; i++) z[i] = __fmaf_rn(-slope, fabsf((float)(qp - sm.pos[mb][c + i])), z[i]);
                             } else {
                                 const float far = (float)(qp - t0 - c);
 #pragma unroll
-                                for (int i = 0; i < 32; i++) z[i] = __fmaf_rn(-slope, fabsf(far - (float)i), z[i]);
+                                for (int i = 0; i < CK; i++) z[i] = __fmaf_rn(-slope, fabsf(far - (float)i), z[i]);
                             }
                         }
                         if (shut) {
                             const int lo = c_lo - c, hi = c_hi - c, pr = c_pre - c;
                             if (by_pos) {
 #pragma unroll
-                                for (int i = 0; i < 32; i++) {
+                                for (int i = 0; i < CK; i++) {
                                     const int kp = sm.pos[mb][c + i];
                                     const bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
                                     z[i] = see && t0 + c + i < q.L ? z[i] : -INFINITY;
                                 }
                             } else {
 #pragma unroll
-                                for (int i = 0; i < 32; i++) z[i] = (i >= lo && i < hi) || i < pr ? z[i] : -INFINITY;
+                                for (int i = 0; i < CK; i++) z[i] = (i >= lo && i < hi) || i < pr ? z[i] : -INFINITY;
                             }
                             if (by_doc) {
 #pragma unroll
-                                for (int i = 0; i < 32; i += 4) {
+                                for (int i = 0; i < CK; i += 4) {
                                     const int4 d = *reinterpret_cast<const int4 *>(&sm.doc[mb][c + i]);
                                     z[i] = d.x == qd ? z[i] : -INFINITY;
                                     z[i + 1] = d.y == qd ? z[i + 1] : -INFINITY;
@@ -430,21 +464,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                             }
                         }
 #pragma unroll
-                        for (int g = 0; g < 32; g += 8) {
+                        for (int g = 0; g < CK; g += 8) {
                             float y = z[g], y1 = z[g + 1];
 #pragma unroll
                             for (int i = 2; i < 8; i += 2) y = fmaxf(y, z[g + i]), y1 = fmaxf(y1, z[g + i + 1]);
                             m0 = fmaxf(m0, fmaxf(y, y1) + lv[c + g]);
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; i++) xa[i] = __float_as_uint(z[i]);
-                        tmem_st32(ts + c, xa);
+                        for (int i = 0; i < CK; i++) xa[i] = __float_as_uint(z[i]);
+                        tmem_st16(ts + c, xa);
                     }
                     tmem_wait_st();
                 } else {
                     // scales of single keys: the same, four columns a round
 #pragma unroll 1
-                    for (int c = 0; c < TK; c += 4) {
+                    for (int c = k0; c < k0 + HC; c += 4) {
                         uint32_t x[4];
                         tmem_ld4(ts + c, x);
 #pragma unroll
@@ -463,6 +497,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                     }
                     tmem_wait_st();
                 }
+                // the other half's maximum: both threads of a row go by the same reference
+                sm.part[w][half][r] = m0;
+                mbar_arrive(&sm.x_full[w]);
+                ok = mbar_wait_warp(&sm.x_full[w], j & 1, &sm.abort);
+                if (!ok) break;
+                m0 = fmaxf(m0, sm.part[w][half ^ 1][r]);
                 const bool grow = m0 > wref + 1.0f;
                 if (__any_sync(0xFFFFFFFFu, grow)) {
                     const float f = grow && wref != -INFINITY ? ex2(wref - m0) : 1.0f;
@@ -470,11 +510,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                     lsum *= f;
                     if (j > 0) {
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += 32) {
-                            tmem_ld32(to + c, xa);
+                        for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += CK) {
+                            tmem_ldc(to + c, xa);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) xa[i] = __float_as_uint(__uint_as_float(xa[i]) * f);
-                            tmem_st32(to + c, xa);
+                            for (int i = 0; i < CK; i++) xa[i] = __float_as_uint(__uint_as_float(xa[i]) * f);
+                            tmem_st16(to + c, xa);
                         }
                         tmem_wait_st();
                     }
@@ -483,11 +523,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                 if (grp) {
                     // p * v_scale = 2^(score + sub + log2 v_scale); the group's sum over v_scale is the sum of its p
 #pragma unroll 1
-                    for (int c = 0; c < TK; c += 32) {
-                        uint32_t p[16];
-                        tmem_ld32(ts + c, xa);
+                    for (int c = k0; c < k0 + HC; c += CK) {
+                        uint32_t p[CK / 2];
+                        tmem_ldc(ts + c, xa);
 #pragma unroll
-                        for (int g = 0; g < 32; g += 8) {
+                        for (int g = 0; g < CK; g += 8) {
                             const float k = rawS ? ks[c + g] * qs2 : 1.0f, off = sub + lv[c + g];
                             const f2 k2 = pk(k, k), o2 = pk(off, off);
                             float y[8];
@@ -501,11 +541,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                             upk(add2(add2(pk(y[0], y[1]), pk(y[2], y[3])), add2(pk(y[4], y[5]), pk(y[6], y[7]))), u0, u1);
                             lsum = __fmaf_rn(u0 + u1, sm.rv[mb][c + g], lsum);
                         }
-                        tmem_st16(ts + c / 2, p);   // columns whose scores are read already
+                        tmem_st8(ts + (c + k0) / 2, p);   // columns whose scores are read already
                     }
                 } else {
 #pragma unroll 1
-                    for (int c = 0; c < TK; c += 4) {
+                    for (int c = k0; c < k0 + HC; c += 4) {
                         uint32_t x[4], p[2];
                         tmem_ld4(ts + c, x);
 #pragma unroll
@@ -517,39 +557,49 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                         }
                         p[0] = pack_f16(__uint_as_float(x[0]), __uint_as_float(x[1]));
                         p[1] = pack_f16(__uint_as_float(x[2]), __uint_as_float(x[3]));
-                        tmem_st2(ts + c / 2, p);
+                        tmem_st2(ts + (c + k0) / 2, p);
                     }
                 }
                 tmem_wait_st();
                 tc_before();
                 mbar_arrive(&sm.p_full[w]);
             }
-            if (ok && n > 0) ok = mbar_wait_warp(&sm.o_full[w], 0, &sm.abort);
+            float l = 0.0f;
+            if (ok && n > 0) {
+                sm.sums[w][half][r] = lsum;
+                mbar_arrive(&sm.x_full[w]);
+                ok = mbar_wait_warp(&sm.x_full[w], n & 1, &sm.abort) && mbar_wait_warp(&sm.o_full[w], 0, &sm.abort);
+                l = lsum + sm.sums[w][half ^ 1][r];
+            }
             tc_after();
-            const float l = lsum;
             const float inv = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? 0.0f : __fdividef(kv8_f16_unit<FMT>(), l);
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; c++) {
+            for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                 uint32_t x[32];
                 if (ok && n > 0) {
-                    tmem_ld32(to + 32 * c, x);
+                    tmem_ld32(to + c, x);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; i++) x[i] = 0;
                 }
                 if (live)
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        kv8_st4(out + orow * HD + 32 * c + i,
-                                make_float4(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv,
-                                            __uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv));
+                    for (int i = 0; i < 32; i += 8) {
+                        uint4 o;
+                        kv8_st4(reinterpret_cast<QT *>(&o), make_float4(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv,
+                                                                        __uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv));
+                        kv8_st4(reinterpret_cast<QT *>(&o) + 4, make_float4(__uint_as_float(x[i + 4]) * inv, __uint_as_float(x[i + 5]) * inv,
+                                                                            __uint_as_float(x[i + 6]) * inv, __uint_as_float(x[i + 7]) * inv));
+                        *reinterpret_cast<uint4 *>(out + orow * HD + c + i) = o;
+                    }
             }
-            if (live && a.lse) a.lse[orow] = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? -INFINITY : (log2f(l) - (wref == -INFINITY ? 0.0f : TOP - wref)) * LN2;
+            if (live && half == 0 && a.lse)
+                a.lse[orow] = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? -INFINITY : (log2f(l) - (wref == -INFINITY ? 0.0f : TOP - wref)) * LN2;
         }
-    } else if (warp < 16) {
+    } else if (warp < 24) {
         // ---- codes to f16 ----
         regs_down<REGS_CONVERT>();
-        const int c = tid - 256;
+        const int c = tid - 512;
         const bool is_v = c >= CV / 2;            // half of the warps convert K, half V: the same code
         const int h = c & (CV / 2 - 1);
         const int prow = (h & 7) + 8 * (h / (8 * PC)), piece = (h >> 3) % PC;   // first row and piece of this thread
@@ -591,7 +641,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             sm.lv[mb][c] = fmaxf(__log2f(mv), -60.0f);
             sm.rv[mb][c] = __fdividef(1.0f, mv);
             const bool tame = __all_sync(0xFFFFFFFFu, mv > 0x1p-60f && mv < 0x1p60f);
-            if (lane == 0) sm.tame[mb][warp - 8] = tame;
+            if (lane == 0) sm.tame[mb][warp - 16] = tame;
             sm.pos[mb][c] = mp;
             sm.doc[mb][c] = md;
             mbar_arrive(&sm.meta_full[mb]);
@@ -633,11 +683,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             if (j >= 2) ok = mbar_wait_warp(&empty[j & 1], ((j >> 1) - 1) & 1, &sm.abort) && ok;
             if (ok) {
                 convert(j, 0, xa);
-                if (j + 1 < n) load(j + 1, 0, xa);
                 convert(j, NP, xb);
                 fence_async_smem();
                 mbar_arrive(&full[j & 1]);
                 if (j + 1 < n) {
+                    load(j + 1, 0, xa);
                     load(j + 1, NP, xb);
                     put_meta(j + 1);
                 }
@@ -646,7 +696,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     } else {
         // ---- MMAs ----
         regs_down<REGS_MMA>();
-        if (warp == 16) {
+        if (warp == 24) {
             constexpr uint32_t id_qk = idesc(TK, false), id_pv = idesc(HD, true);
             const uint32_t lead = lane == 0, tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
             const int nt = __shfl_sync(0xFFFFFFFFu, n, 0), nw = __shfl_sync(0xFFFFFFFFu, two ? 2 : 1, 0);
@@ -664,7 +714,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                 const uint64_t va = dv + (j & 1) * BUF;
 #pragma unroll
                 for (int k = 0; k < TK / 16; k++)
-                    umma_ts(tm + 2 * TK + w * HD, tm + w * TK + 8 * k, va + 2 * SBO / 16 * k, id_pv, j > 0 || k > 0, lead);
+                    umma_ts(tm + 2 * TK + w * HD, tm + w * TK + 8 * k + (k >= HC / 16 ? HC / 2 : 0), va + 2 * SBO / 16 * k, id_pv, j > 0 || k > 0, lead);
             };
             bool ok = nt == 0 || (mbar_wait(&sm.q_full, 0, &sm.abort) && mbar_wait(&sm.k_full[0], 0, &sm.abort));
             if (ok && nt > 0) {
@@ -701,7 +751,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == 24) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 bool smem_opt_in(const void *fn, size_t bytes) {
