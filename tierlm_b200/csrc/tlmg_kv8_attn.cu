@@ -1,11 +1,11 @@
 // tlmg_kv8_attn.cu - attention over the 8-bit KV cache, split over the rows.
 //
 // One CTA takes a span of a sequence's rows, one KV head and a tile of query
-// rows (a query row is one token's one head of the group; 8 rows for f32
-// queries, 16 for 16-bit ones), and keeps a running maximum, sum and output
-// per row; a second kernel joins the spans. This is the form for few query
-// rows per KV head: it is bound by HBM, since a code byte of K or V feeds
-// only 2 x 16 multiply-adds.
+// rows (a query row is one token's one head of the group; 8 rows, or 16 where
+// a 16-bit call has more than 8 per KV head), and keeps a running maximum, sum
+// and output per row; a second kernel joins the spans. This is the form for
+// few query rows per KV head: it is bound by HBM as far as the instructions per
+// byte allow, since a code byte of K or V feeds only 2 x 8 multiply-adds.
 //
 // Products run on mma.sync.m16n8k16 (f16 in, f32 out): the query rows of a
 // group (1 .. 16) are below the 64-row minimum of tcgen05.mma, and at the HBM
@@ -17,7 +17,7 @@
 // probabilities as one f16 (11 bits, below the rounding of a 16-bit output).
 //
 // A warp owns tiles of 32 rows. Its lanes copy exactly the bytes that they
-// themselves multiply (cp.async into a ring of NST stages, no barrier between
+// themselves multiply (cp.async into a ring of two stages, no barrier between
 // warps): contraction order is free, so lane (g, t4) holds the 16-byte pieces
 // t4, t4 + 4, .. of key row g (mod 8) as its B fragments, and for V the hd / 8
 // columns from g hd / 8 on of the four rows that its probabilities belong to.
@@ -54,6 +54,12 @@ template <int N> __device__ __forceinline__ void cpN(uint32_t dst, const void *s
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[2], uint32_t b0, uint32_t b1) {   // rows 8 .. 15 zero
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%6,%5,%6}, {%7,%8}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(0u), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                  "{%0,%1,%2,%3};"
@@ -83,7 +89,7 @@ template <int HD> struct Plan {
     static constexpr int VP = VB / CH;                       // copies per row
     static constexpr int META = 2 * TILE * HD;               // offset of scales, positions, documents
     static constexpr int STAGE = 2 * TILE * HD + 4 * TILE * 4;
-    static constexpr int NST = HD <= 128 ? 3 : 2;
+    static constexpr int NST = 2;
     static constexpr int SMEM = NW * NST * STAGE;
 };
 
@@ -101,10 +107,11 @@ __device__ __forceinline__ Kv8Range<TILE> key_range(const Kv8Attn &a, const Kv8S
     return kv8_range<TILE>(a, q, s, pmin, pmax);
 }
 
-template <int HD, int FMT, typename QT>
-__global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ Kv8Attn a) {
+template <int HD, int FMT, typename QT, int RM>
+__global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const __grid_constant__ Kv8Attn a) {
     constexpr bool F32 = sizeof(QT) == 4;
-    constexpr int ROWS = F32 ? 8 : 16, RM = F32 ? 1 : 2;     // query rows of the CTA; rows of a thread
+    constexpr int ROWS = 8 * RM;                             // query rows of the CTA (RM of a thread)
+    constexpr int QR = F32 || RM == 2 ? 4 : 2;               // registers of a query fragment: rows 8 .. 15 may be zeros
     constexpr int NT = HD / 8, KC = HD / 64, NST = Plan<HD>::NST;
     using P = Plan<HD>;
     extern __shared__ __align__(16) uint8_t sm[];
@@ -147,19 +154,21 @@ __global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ K
     const int32_t *docs = a.doc ? a.doc + (size_t)s * a.doc_stride : nullptr;
     uint8_t *ring = sm + (size_t)warp * NST * P::STAGE;
     int32_t te = -1;
+    // pages of 32 rows and more hold a tile whole: one entry, row offsets that the compiler knows
+    const bool whole = a.c.lp >= 5;
     auto load_te = [&](int i) {
         if (i < n_my) {
-            const int t = rg.t0(v0 + warp + NW * i) + lane;
+            const int t = rg.t0(v0 + warp + NW * i) + (whole ? 0 : lane);
             te = t < q.L ? __ldg(table + (t >> a.c.lp)) : -1;
         }
     };
     auto issue = [&](int i) {
         if (i < n_my) {
-            const int t = rg.t0(v0 + warp + NW * i) + lane;
-            const bool ok = t < q.L && a.c.ok(te);
-            const uint32_t rid = ok ? a.c.row(te, kvh, t) : 0u;
+            const int t0 = rg.t0(v0 + warp + NW * i), t = t0 + lane;
             uint8_t *st = ring + (i % NST) * P::STAGE;
             const uint32_t sb = saddr(st), mb = sb + P::META + 4 * lane;
+            const bool ok = t < q.L && a.c.ok(te);
+            const uint32_t rid = ok ? a.c.row(te, kvh, t) : 0u;
             if (ok) {
                 cpN<4>(mb, a.c.ks + (rid >> a.c.lb), 4);
                 cpN<4>(mb + 4 * TILE, a.c.vs + (rid >> a.c.lb), 4);
@@ -174,23 +183,44 @@ __global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ K
                 if (t < a.doc_stride) cpN<4>(mb + 12 * TILE, docs + t, 4);
                 else reinterpret_cast<int *>(st + P::META)[3 * TILE + lane] = -1;
             }
+            const uint32_t kd = sb + lane * 16, vd = sb + TILE * HD + lane * P::CH;
+            if (whole) {
+                const int lim = a.c.ok(te) ? q.L - t0 : 0;   // rows of the tile that there are
+                const size_t r0 = lim > 0 ? (size_t)a.c.row(te, kvh, t0) * HD : 0;
+                const uint8_t *ks = a.c.k + r0 + (lim > g ? g * HD : 0) + 16 * t4, *vs = a.c.v + r0 + g * P::VB;
 #pragma unroll
-            for (int nt = 0; nt < 4; nt++) {
-                const uint32_t r = __shfl_sync(0xFFFFFFFFu, rid, 8 * nt + g);
-                const int nb = __shfl_sync(0xFFFFFFFFu, ok ? 16 : 0, 8 * nt + g);
-                const uint8_t *src = a.c.k + (size_t)r * HD + 16 * t4;
+                for (int nt = 0; nt < 4; nt++) {
+                    const bool in = 8 * nt + g < lim;
 #pragma unroll
-                for (int c = 0; c < KC; c++) cpN<16>(sb + ((nt * KC + c) * 32 + lane) * 16, src + 64 * c, nb);
-            }
+                    for (int c = 0; c < KC; c++)
+                        cpN<16>(kd + (nt * KC + c) * 512, in ? ks + 8 * nt * HD + 64 * c : a.c.k, in ? 16 : 0);
+                }
 #pragma unroll
-            for (int kr = 0; kr < 8; kr++) {   // rows 16 (kr / 4) + 2 t4 + {0, 1, 8, 9}
-                const int row = 16 * (kr >> 2) + 2 * t4 + (kr & 1) + 8 * ((kr >> 1) & 1);
-                const uint32_t r = __shfl_sync(0xFFFFFFFFu, rid, row);
-                const int nb = __shfl_sync(0xFFFFFFFFu, ok ? P::CH : 0, row);
-                const uint8_t *src = a.c.v + (size_t)r * HD + g * P::VB;
+                for (int kr = 0; kr < 8; kr++) {   // rows 16 (kr / 4) + 2 t4 + {0, 1, 8, 9}
+                    const int row = 16 * (kr >> 2) + (kr & 1) + 8 * ((kr >> 1) & 1) + 2 * t4;
+                    const bool in = row < lim;
 #pragma unroll
-                for (int c = 0; c < P::VP; c++)
-                    cpN<P::CH>(sb + TILE * HD + ((kr * P::VP + c) * 32 + lane) * P::CH, src + 16 * c, nb);
+                    for (int c = 0; c < P::VP; c++)
+                        cpN<P::CH>(vd + (kr * P::VP + c) * 32 * P::CH, in ? vs + row * HD + 16 * c : a.c.v, in ? P::CH : 0);
+                }
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < 4; nt++) {
+                    const uint32_t r = __shfl_sync(0xFFFFFFFFu, rid, 8 * nt + g);
+                    const int nb = __shfl_sync(0xFFFFFFFFu, ok ? 16 : 0, 8 * nt + g);
+                    const uint8_t *src = a.c.k + (size_t)r * HD + 16 * t4;
+#pragma unroll
+                    for (int c = 0; c < KC; c++) cpN<16>(kd + (nt * KC + c) * 512, src + 64 * c, nb);
+                }
+#pragma unroll
+                for (int kr = 0; kr < 8; kr++) {
+                    const int row = 16 * (kr >> 2) + 2 * t4 + (kr & 1) + 8 * ((kr >> 1) & 1);
+                    const uint32_t r = __shfl_sync(0xFFFFFFFFu, rid, row);
+                    const int nb = __shfl_sync(0xFFFFFFFFu, ok ? P::CH : 0, row);
+                    const uint8_t *src = a.c.v + (size_t)r * HD + g * P::VB;
+#pragma unroll
+                    for (int c = 0; c < P::VP; c++) cpN<P::CH>(vd + (kr * P::VP + c) * 32 * P::CH, src + 16 * c, nb);
+                }
             }
         }
         cp_commit();   // an empty group past the end keeps the count uniform
@@ -203,7 +233,7 @@ __global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ K
     load_te(NST - 1);
 
     // this thread's query rows: f16 fragments, the power of two taken out, masks
-    uint32_t qa[4 * KC][4];
+    uint32_t qa[4 * KC][QR];
     float qs[RM], slope[RM];
     int qp[RM], qd[RM];
     {
@@ -248,11 +278,14 @@ __global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ K
             if constexpr (F32) {
                 split_f16(x[0].x, x[0].y, qa[c][0], qa[c][1]);
                 split_f16(x[0].z, x[0].w, qa[c][2], qa[c][3]);
-            } else {
+            } else if constexpr (RM == 2) {
                 qa[c][0] = pack_f16(x[0].x, x[0].y);
                 qa[c][1] = pack_f16(x[1].x, x[1].y);
                 qa[c][2] = pack_f16(x[0].z, x[0].w);
                 qa[c][3] = pack_f16(x[1].z, x[1].w);
+            } else {
+                qa[c][0] = pack_f16(x[0].x, x[0].y);
+                qa[c][1] = pack_f16(x[0].z, x[0].w);
             }
         }
     }
@@ -294,9 +327,6 @@ __global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ K
         const bool full = !docs && !a.c.pos && t0 + TILE <= q.L &&
                           __all_sync(0xFFFFFFFFu, (!a.causal || t0 + TILE - 1 <= pmin) && (!a.window || pmax - t0 < a.window));
         float z[RM][8], vs[8];
-        float mx[RM];
-#pragma unroll
-        for (int r = 0; r < RM; r++) mx[r] = -INFINITY;
 #pragma unroll
         for (int nt = 0; nt < 4; nt++) {
             const float2 ks2 = *reinterpret_cast<const float2 *>(ms + 8 * nt + 2 * t4);
@@ -304,25 +334,57 @@ __global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ K
             vs[2 * nt] = vs2.x;
             vs[2 * nt + 1] = vs2.y;
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int col = 8 * nt + 2 * t4 + u, t = t0 + col;
-                const int kp = a.c.pos ? mi[2 * TILE + col] : t;
+            for (int r = 0; r < RM; r++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float dot = F32 ? __fmaf_rn(sc[nt][2 + u], LO, sc[nt][u]) : sc[nt][2 * r + u];
+                    z[r][2 * nt + u] = dot * ((u ? ks2.y : ks2.x) * qs[r]);
+                }
+        }
+        if (a.softcap > 0.0f) {
+            float big = 0.0f;
+#pragma unroll
+            for (int r = 0; r < RM; r++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    z[r][j] *= a.inv_cap;
+                    big = fmaxf(big, fabsf(z[r][j]));
+                }
+            if (__all_sync(0xFFFFFFFFu, big < TANH_X)) {   // (a NaN may pass: the polynomial keeps it)
+#pragma unroll
+                for (int r = 0; r < RM; r++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) z[r][j] = a.softcap * kv8_tanh_small(z[r][j]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < RM; r++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) z[r][j] = a.softcap * tanhf(z[r][j]);
+            }
+        }
+        if (a.slopes) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int col = 8 * (j >> 1) + 2 * t4 + (j & 1), kp = a.c.pos ? mi[2 * TILE + col] : t0 + col;
+#pragma unroll
+                for (int r = 0; r < RM; r++) z[r][j] = z[r][j] - slope[r] * fabsf((float)(qp[r] - kp));
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RM; r++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) z[r][j] *= LOG2E;
+        if (!full) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int col = 8 * (j >> 1) + 2 * t4 + (j & 1), t = t0 + col, kp = a.c.pos ? mi[2 * TILE + col] : t;
                 int kd = -1;
                 if (docs) kd = a.c.pos ? (kp >= 0 && kp < a.doc_stride ? __ldg(docs + kp) : -1) : mi[3 * TILE + col];
 #pragma unroll
                 for (int r = 0; r < RM; r++) {
-                    const float dot = F32 ? __fmaf_rn(sc[nt][2 + u], LO, sc[nt][u]) : sc[nt][2 * r + u];
-                    float v = dot * ((u ? ks2.y : ks2.x) * qs[r]);
-                    if (a.softcap > 0.0f) v = a.softcap * tanhf(v * a.inv_cap);
-                    if (a.slopes) v = v - slope[r] * fabsf((float)(qp[r] - kp));
-                    v *= LOG2E;
-                    if (!full) {
-                        bool see = kp < pre || ((!a.causal || kp <= qp[r]) && (!a.window || qp[r] - kp < a.window));
-                        see = see && t < q.L && (!docs || kd == qd[r]);
-                        v = see ? v : -INFINITY;
-                    }
-                    z[r][2 * nt + u] = v;
-                    mx[r] = fmaxf(mx[r], v);
+                    bool see = kp < pre || ((!a.causal || kp <= qp[r]) && (!a.window || qp[r] - kp < a.window));
+                    see = see && t < q.L && (!docs || kd == qd[r]);
+                    z[r][j] = see ? z[r][j] : -INFINITY;
                 }
             }
         }
@@ -338,20 +400,20 @@ __global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ K
             }
         }
         float alpha[RM], back[RM];
-        uint32_t pa[2][4];
+        uint32_t pa[2][QR];
 #pragma unroll
         for (int r = 0; r < RM; r++) {
-            float m = mx[r];
+            float m = fmaxf(fmaxf(fmaxf(z[r][0], z[r][1]), fmaxf(z[r][2], z[r][3])), fmaxf(fmaxf(z[r][4], z[r][5]), fmaxf(z[r][6], z[r][7])));
             m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
             m = fmaxf(m, mrun[r]);
             const float sub = m == -INFINITY ? 0.0f : m;
-            alpha[r] = m == -INFINITY ? 1.0f : exp2f(mrun[r] - m);
+            alpha[r] = m == -INFINITY ? 1.0f : kv8_ex2(mrun[r] - m);
             mrun[r] = m;
             float sum = 0.0f, top = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float p = exp2f(z[r][j] - sub);
+                const float p = kv8_ex2(z[r][j] - sub);
                 sum += p;
                 // a masked key's scale has no part in this, whatever it is
                 z[r][j] = z[r][j] == -INFINITY ? 0.0f : p * vs[j];
@@ -372,11 +434,14 @@ __global__ void __launch_bounds__(32 * NW) k_kv8_split(const __grid_constant__ K
             if constexpr (F32) {
                 split_f16(z[0][4 * kk], z[0][4 * kk + 1], pa[kk][0], pa[kk][1]);
                 split_f16(z[0][4 * kk + 2], z[0][4 * kk + 3], pa[kk][2], pa[kk][3]);
-            } else {
+            } else if constexpr (RM == 2) {
                 pa[kk][0] = pack_f16(z[0][4 * kk], z[0][4 * kk + 1]);
                 pa[kk][1] = pack_f16(z[RM - 1][4 * kk], z[RM - 1][4 * kk + 1]);
                 pa[kk][2] = pack_f16(z[0][4 * kk + 2], z[0][4 * kk + 3]);
                 pa[kk][3] = pack_f16(z[RM - 1][4 * kk + 2], z[RM - 1][4 * kk + 3]);
+            } else {
+                pa[kk][0] = pack_f16(z[0][4 * kk], z[0][4 * kk + 1]);
+                pa[kk][1] = pack_f16(z[0][4 * kk + 2], z[0][4 * kk + 3]);
             }
         }
         bool same = alpha[0] == 1.0f;
@@ -609,6 +674,7 @@ bool smem_opt_in(const void *fn, size_t bytes) {
 
 struct Split {
     bool wide;             // the tcgen05 kernel serves the call
+    int rm;                // query rows of a CTA / 8
     int n, tiles;          // spans, 32-row tiles per span
     int64_t rtiles;        // query tiles
     size_t part, scores, total;   // floats of the partial results / scores, bytes in all
@@ -617,16 +683,21 @@ struct Split {
 
 Split split_plan(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_score &s, int H, int q_dt, bool weights) {
     Split p{};
-    const int G = H / c.KV, rows = q_dt == TLMG_DT_F32 ? 8 : 16;
+    const int G = H / c.KV;
     p.wide = !weights && kv8_prefill_serves(c, b, H, q_dt);
     if (p.wide) return p;
+    // 16 query rows a CTA only where there are more than 8 (and 16-bit queries, whose fragments leave the room)
+    p.rm = q_dt != TLMG_DT_F32 && (int64_t)b.max_q * G > 8 ? 2 : 1;
+    const int rows = 8 * p.rm;
     p.rtiles = ((int64_t)b.max_q * G + rows - 1) / rows;
     // rows that a query tile can see at most (the prefix is only known to the device)
     int64_t vis = b.max_kv;
     if (s.window > 0 && s.causal && !c.pos && !s.prefix && !b.q_pos)
         vis = std::min<int64_t>(vis, (int64_t)s.window + (rows + G - 1) / G + TILE);
+    // Spans: one round of the CTAs that the SMs hold for one sequence; four for a batch, whose lengths differ.
+    const int64_t slots = (int64_t)sm_count() * (c.hd <= 128 ? 3 : 1) * (b.n_seq > 1 ? 4 : 1);
     const int64_t tiles = std::max<int64_t>(1, (vis + TILE - 1) / TILE), base = p.rtiles * c.KV * b.n_seq;
-    const int64_t want = std::max<int64_t>(1, (int64_t)sm_count() * 2 / base);
+    const int64_t want = std::max<int64_t>(1, slots / base);
     p.tiles = (int)std::max<int64_t>(NW, (tiles + want - 1) / want);
     p.n = (int)((tiles + p.tiles - 1) / p.tiles);
     const size_t rows_all = (size_t)b.total_q * H;
@@ -650,10 +721,10 @@ template <typename F> cudaError_t launch_dep(F fn, dim3 grid, int block, const K
     return cudaLaunchKernelEx(&cfg, fn, a);
 }
 
-template <int HD, int FMT, typename QT>
-int launch_split(const Kv8Attn &a, const Split &p, cudaStream_t st) {
-    auto fn = k_kv8_split<HD, FMT, QT>;
-    constexpr int ROWS = sizeof(QT) == 4 ? 8 : 16;
+template <int HD, int FMT, typename QT, int RM>
+int launch_split_rows(const Kv8Attn &a, const Split &p, cudaStream_t st) {
+    auto fn = k_kv8_split<HD, FMT, QT, RM>;
+    constexpr int ROWS = 8 * RM;
     constexpr size_t join = (size_t)NW * ROWS * (HD + 2) * 4, sm = std::max<size_t>(Plan<HD>::SMEM, join);
     if (!smem_opt_in((const void *)fn, sm)) return set_error(TLMG_EIO, "kv8_attend: shared memory opt-in failed");
     fn<<<dim3(p.n, (unsigned)(p.rtiles * a.c.KV), a.b.n_seq), 32 * NW, sm, st>>>(a);
@@ -670,6 +741,11 @@ int launch_split(const Kv8Attn &a, const Split &p, cudaStream_t st) {
     }
     if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? TLMG_OK : cuda_fail(e, "kv8_attend launch");
+}
+template <int HD, int FMT, typename QT> int launch_split(const Kv8Attn &a, const Split &p, cudaStream_t st) {
+    if constexpr (sizeof(QT) == 2)
+        if (p.rm == 2) return launch_split_rows<HD, FMT, QT, 2>(a, p, st);
+    return launch_split_rows<HD, FMT, QT, 1>(a, p, st);
 }
 
 template <int HD, int FMT> int launch_split_q(const Kv8Attn &a, const Split &p, int q_dt, cudaStream_t st) {

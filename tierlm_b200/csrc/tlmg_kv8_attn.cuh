@@ -27,6 +27,25 @@ struct Kv8Attn {
     int64_t s_stride;
 };
 
+// tanh(x) = x (c0 + c1 x^2 + .. + c5 x^10) for |x| < TANH_X within 2e-7: fitted (reweighted least squares towards the
+// smallest maximum) to tanh(x) / x over x^2 in [0, TANH_X^2]. Two issue slots and a half an element; the exponential
+// form takes two of the slower special-function results.
+constexpr float TANH_X = 0.8f;
+__device__ constexpr float TANH_C[6] = { 0.9999999403953552f, -0.33332714438438416f, 0.13321532309055328f, -0.05313541740179062f, 0.019130872562527657f, -0.004378729499876499f };
+
+__device__ __forceinline__ float kv8_tanh_small(float x) {
+    const float y = x * x;
+    float r = TANH_C[5];
+#pragma unroll
+    for (int k = 4; k >= 0; k--) r = __fmaf_rn(r, y, TANH_C[k]);
+    return r * x;
+}
+__device__ __forceinline__ float kv8_ex2(float x) {   // 2^x, results below 2^-126 as 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // The key tiles of TILE rows that a tile of queries at positions pmin ..
 // pmax may see. Rows are positions when the cache has no position pool: then
 // they are the rows below the prefix and those from the window's begin to

@@ -215,21 +215,11 @@ __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
+__device__ __forceinline__ float ex2(float x) { return kv8_ex2(x); }
 __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-
-// tanh(x) = x (c0 + c1 x^2 + .. + c5 x^10) for |x| < TANH_X within 2e-7: fitted (reweighted least squares towards the
-// smallest maximum) to tanh(x) / x over x^2 in [0, TANH_X^2]. Two issue slots and a half an element; the exponential
-// form takes two of the slower special-function results.
-constexpr float TANH_X = 0.8f;
-__device__ constexpr float TANH_C[6] = { 0.9999999403953552f, -0.33332714438438416f, 0.13321532309055328f, -0.05313541740179062f, 0.019130872562527657f, -0.004378729499876499f };
 
 // softcap * log2(e) * tanh(y) by the exponential
 __device__ __forceinline__ float cap_exp(float y, float capl) {
