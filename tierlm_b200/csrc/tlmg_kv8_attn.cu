@@ -51,6 +51,10 @@ template <int N> __device__ __forceinline__ void cpN(uint32_t dst, const void *s
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(src_bytes) : "memory");
 }
+template <int N> __device__ __forceinline__ void cpA(uint32_t dst, const void *src) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -65,6 +69,17 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                  "{%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the same with an accumulator that starts from zero
+__device__ __forceinline__ void mma_f16_0(float (&c)[4], const uint32_t (&a)[2], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%6,%5,%6}, {%7,%8}, {%9,%9,%9,%9};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(0u), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_f16_0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -154,8 +169,9 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
     const int32_t *docs = a.doc ? a.doc + (size_t)s * a.doc_stride : nullptr;
     uint8_t *ring = sm + (size_t)warp * NST * P::STAGE;
     int32_t te = -1;
-    // pages of 32 rows and more hold a tile whole: one entry, row offsets that the compiler knows
+    // pages of 32 rows and more hold a tile whole: one entry, offsets that the compiler knows
     const bool whole = a.c.lp >= 5;
+    const int k_lane = g * HD + 16 * t4, v_lane = 2 * t4 * HD + g * P::VB;   // this lane's first K and V bytes of a tile
     auto load_te = [&](int i) {
         if (i < n_my) {
             const int t = rg.t0(v0 + warp + NW * i) + (whole ? 0 : lane);
@@ -184,25 +200,19 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
                 else reinterpret_cast<int *>(st + P::META)[3 * TILE + lane] = -1;
             }
             const uint32_t kd = sb + lane * 16, vd = sb + TILE * HD + lane * P::CH;
-            if (whole) {
-                const int lim = a.c.ok(te) ? q.L - t0 : 0;   // rows of the tile that there are
-                const size_t r0 = lim > 0 ? (size_t)a.c.row(te, kvh, t0) * HD : 0;
-                const uint8_t *ks = a.c.k + r0 + (lim > g ? g * HD : 0) + 16 * t4, *vs = a.c.v + r0 + g * P::VB;
+            if (whole && a.c.ok(te) && t0 + TILE <= q.L) {
+                const uint8_t *ks = a.c.k + (size_t)a.c.row(te, kvh, t0) * HD, *vs = a.c.v + (ks - a.c.k) + v_lane;
+                ks += k_lane;
 #pragma unroll
-                for (int nt = 0; nt < 4; nt++) {
-                    const bool in = 8 * nt + g < lim;
+                for (int nt = 0; nt < 4; nt++)
 #pragma unroll
-                    for (int c = 0; c < KC; c++)
-                        cpN<16>(kd + (nt * KC + c) * 512, in ? ks + 8 * nt * HD + 64 * c : a.c.k, in ? 16 : 0);
-                }
+                    for (int c = 0; c < KC; c++) cpA<16>(kd + (nt * KC + c) * 512, ks + 8 * nt * HD + 64 * c);
 #pragma unroll
-                for (int kr = 0; kr < 8; kr++) {   // rows 16 (kr / 4) + 2 t4 + {0, 1, 8, 9}
-                    const int row = 16 * (kr >> 2) + (kr & 1) + 8 * ((kr >> 1) & 1) + 2 * t4;
-                    const bool in = row < lim;
+                for (int kr = 0; kr < 8; kr++)   // rows 16 (kr / 4) + 2 t4 + {0, 1, 8, 9}
 #pragma unroll
                     for (int c = 0; c < P::VP; c++)
-                        cpN<P::CH>(vd + (kr * P::VP + c) * 32 * P::CH, in ? vs + row * HD + 16 * c : a.c.v, in ? P::CH : 0);
-                }
+                        cpA<P::CH>(vd + (kr * P::VP + c) * 32 * P::CH,
+                                   vs + (16 * (kr >> 2) + (kr & 1) + 8 * ((kr >> 1) & 1)) * HD + 16 * c);
             } else {
 #pragma unroll
                 for (int nt = 0; nt < 4; nt++) {
@@ -237,58 +247,54 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
     float qs[RM], slope[RM];
     int qp[RM], qd[RM];
     {
-        float m[RM];
-        const QT *qr[RM];
-        bool live[RM];
+        float4 x[RM][4 * KC];   // this lane's elements of its rows
+        float up[RM];
 #pragma unroll
         for (int r = 0; r < RM; r++) {
             const int R = R0 + g + 8 * r, tok = R / G, h = kvh * G + R % G;
-            live[r] = R < n_rows;
-            qr[r] = static_cast<const QT *>(a.q) + (live[r] ? (q.q0 + (int64_t)tok) * a.q_stride + (int64_t)h * HD : 0);
-            const int at = live[r] ? tok : i0;   // a row past the end takes the first token's place
-            qp[r] = a.b.q_pos ? a.b.q_pos[q.q0 + at] : q.L - q.n + at;
-            qd[r] = docs && live[r] ? (qp[r] >= 0 && qp[r] < a.doc_stride ? docs[qp[r]] : -1) : -1;
-            slope[r] = a.slopes && live[r] ? a.slopes[h] : 0.0f;
-            m[r] = 0.0f;
-            for (int c = 0; c < 4 * KC; c++) {
-                const float4 x = live[r] ? kv8_ld4(qr[r] + 64 * (c >> 2) + 16 * t4 + 4 * (c & 3)) : make_float4(0, 0, 0, 0);
-                m[r] = fmaxf(m[r], fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-            }
-            m[r] = fmaxf(m[r], __shfl_xor_sync(0xFFFFFFFFu, m[r], 1));
-            m[r] = fmaxf(m[r], __shfl_xor_sync(0xFFFFFFFFu, m[r], 2));
-        }
-        float up[RM];
+            const bool live = R < n_rows;
+            const int at = live ? tok : i0;   // a row past the end takes the first token's place
+            const QT *qr = static_cast<const QT *>(a.q) + (q.q0 + (int64_t)at) * a.q_stride + (int64_t)(live ? h : kvh * G) * HD + 16 * t4;
 #pragma unroll
-        for (int r = 0; r < RM; r++) {   // the row's largest element to 2^9 .. 2^10
-            const int e = min(max(exp_above(m[r]) - 10, -100), 100);
-            up[r] = pow2i(-e);
-            qs[r] = pow2i(e) * a.scale * kv8_f16_unit<FMT>();
+            for (int c = 0; c < 4 * KC; c++) x[r][c] = kv8_ld4(qr + 64 * (c >> 2) + 4 * (c & 3));
+            qp[r] = a.b.q_pos ? a.b.q_pos[q.q0 + at] : q.L - q.n + at;
+            qd[r] = docs && live ? (qp[r] >= 0 && qp[r] < a.doc_stride ? docs[qp[r]] : -1) : -1;
+            slope[r] = a.slopes && live ? a.slopes[h] * LOG2E : 0.0f;
+            float m = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4 * KC; c++)
+                m = fmaxf(m, fmaxf(fmaxf(fabsf(x[r][c].x), fabsf(x[r][c].y)), fmaxf(fabsf(x[r][c].z), fabsf(x[r][c].w))));
+            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+            // the row's largest element to 2^9 .. 2^10
+            const int e = min(max(exp_above(m) - 10, -100), 100);
+            up[r] = live ? pow2i(-e) : 0.0f;
+            qs[r] = pow2i(e) * a.scale * kv8_f16_unit<FMT>() * (a.softcap > 0.0f ? a.inv_cap : LOG2E);
         }
 #pragma unroll
         for (int c = 0; c < 4 * KC; c++) {
-            float4 x[RM];
 #pragma unroll
             for (int r = 0; r < RM; r++) {
-                x[r] = live[r] ? kv8_ld4(qr[r] + 64 * (c >> 2) + 16 * t4 + 4 * (c & 3)) : make_float4(0, 0, 0, 0);
-                x[r].x *= up[r];
-                x[r].y *= up[r];
-                x[r].z *= up[r];
-                x[r].w *= up[r];
+                x[r][c].x *= up[r];
+                x[r][c].y *= up[r];
+                x[r][c].z *= up[r];
+                x[r][c].w *= up[r];
             }
             if constexpr (F32) {
-                split_f16(x[0].x, x[0].y, qa[c][0], qa[c][1]);
-                split_f16(x[0].z, x[0].w, qa[c][2], qa[c][3]);
+                split_f16(x[0][c].x, x[0][c].y, qa[c][0], qa[c][1]);
+                split_f16(x[0][c].z, x[0][c].w, qa[c][2], qa[c][3]);
             } else if constexpr (RM == 2) {
-                qa[c][0] = pack_f16(x[0].x, x[0].y);
-                qa[c][1] = pack_f16(x[1].x, x[1].y);
-                qa[c][2] = pack_f16(x[0].z, x[0].w);
-                qa[c][3] = pack_f16(x[1].z, x[1].w);
+                qa[c][0] = pack_f16(x[0][c].x, x[0][c].y);
+                qa[c][1] = pack_f16(x[1][c].x, x[1][c].y);
+                qa[c][2] = pack_f16(x[0][c].z, x[0][c].w);
+                qa[c][3] = pack_f16(x[1][c].z, x[1][c].w);
             } else {
-                qa[c][0] = pack_f16(x[0].x, x[0].y);
-                qa[c][1] = pack_f16(x[0].z, x[0].w);
+                qa[c][0] = pack_f16(x[0][c].x, x[0][c].y);
+                qa[c][1] = pack_f16(x[0][c].z, x[0][c].w);
             }
         }
     }
+    const float capl = a.softcap * LOG2E;
     const int pre = a.prefix ? a.prefix[s] : 0;
     int pmin = qp[0], pmax = qp[0];
     if constexpr (RM == 2) {
@@ -311,17 +317,19 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
         const int t0 = rg.t0(v0 + warp + NW * i);
         float sc[4][4];
 #pragma unroll
-        for (int nt = 0; nt < 4; nt++) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
-#pragma unroll
         for (int c = 0; c < KC; c++)
 #pragma unroll
             for (int nt = 0; nt < 4; nt++) {
                 const uint4 w = *reinterpret_cast<const uint4 *>(st + ((nt * KC + c) * 32 + lane) * 16);
                 const uint32_t x[4] = { kv8_bias<FMT>(w.x), kv8_bias<FMT>(w.y), kv8_bias<FMT>(w.z), kv8_bias<FMT>(w.w) };
 #pragma unroll
-                for (int j = 0; j < 4; j++) mma_f16(sc[nt], qa[4 * c + j], kv8_half2<FMT, 0>(x[j]), kv8_half2<FMT, 1>(x[j]));
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t b0 = kv8_half2<FMT, 0>(x[j]), b1 = kv8_half2<FMT, 1>(x[j]);
+                    if (c == 0 && j == 0) mma_f16_0(sc[nt], qa[0], b0, b1);
+                    else mma_f16(sc[nt], qa[4 * c + j], b0, b1);
+                }
             }
-        // scores in log2 units; masked ones -inf
+        // scores in log2 units (with a cap: over it, until the tanh), masked ones -inf
         const float *ms = reinterpret_cast<const float *>(st + P::META);
         const int *mi = reinterpret_cast<const int *>(ms);
         const bool full = !docs && !a.c.pos && t0 + TILE <= q.L &&
@@ -346,20 +354,17 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
 #pragma unroll
             for (int r = 0; r < RM; r++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    z[r][j] *= a.inv_cap;
-                    big = fmaxf(big, fabsf(z[r][j]));
-                }
+                for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(z[r][j]));
             if (__all_sync(0xFFFFFFFFu, big < TANH_X)) {   // (a NaN may pass: the polynomial keeps it)
 #pragma unroll
                 for (int r = 0; r < RM; r++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) z[r][j] = a.softcap * kv8_tanh_small(z[r][j]);
+                    for (int j = 0; j < 8; j++) z[r][j] = capl * kv8_tanh_small(z[r][j]);
             } else {
 #pragma unroll
                 for (int r = 0; r < RM; r++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) z[r][j] = a.softcap * tanhf(z[r][j]);
+                    for (int j = 0; j < 8; j++) z[r][j] = capl * tanhf(z[r][j]);
             }
         }
         if (a.slopes) {
@@ -370,10 +375,6 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
                 for (int r = 0; r < RM; r++) z[r][j] = z[r][j] - slope[r] * fabsf((float)(qp[r] - kp));
             }
         }
-#pragma unroll
-        for (int r = 0; r < RM; r++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) z[r][j] *= LOG2E;
         if (!full) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -483,13 +484,14 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
                 }
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    float acc[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+                    float acc[4];
 #pragma unroll
                     for (int kk = 0; kk < 2; kk++) {
                         const uint32_t *u = y < 2 ? ev : od;
                         const uint32_t b0 = (y & 1) ? kv8_half2<FMT, 1>(u[2 * kk]) : kv8_half2<FMT, 0>(u[2 * kk]);
                         const uint32_t b1 = (y & 1) ? kv8_half2<FMT, 1>(u[2 * kk + 1]) : kv8_half2<FMT, 0>(u[2 * kk + 1]);
-                        mma_f16(acc, pa[kk], b0, b1);
+                        if (kk == 0) mma_f16_0(acc, pa[kk], b0, b1);
+                        else mma_f16(acc, pa[kk], b0, b1);
                     }
                     float (&oj)[2 * RM] = o[16 * c + 4 * x + y];
                     if constexpr (F32) {
@@ -508,19 +510,21 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
     }
     cp_wait<0>();
     __syncthreads();
-    // join the warps: per row weights 2^(m_w - M)
-    float *wo = reinterpret_cast<float *>(sm);                 // [NW][ROWS][HD]
-    float *wm = wo + NW * ROWS * HD, *wl = wm + NW * ROWS;     // [NW][ROWS]
+    // join the warps: per row weights 2^(m_w - M). A row's HD columns lie in four runs (one per t4) of HD / 4 + 4
+    // floats, HD + 16 in all, so that the eight lanes of a 16-byte store phase take different banks.
+    constexpr int RUN = HD / 4 + 4, ROW = HD + 16;
+    float *wo = reinterpret_cast<float *>(sm);                  // [NW][ROWS][ROW]
+    float *wm = wo + NW * ROWS * ROW, *wl = wm + NW * ROWS;     // [NW][ROWS]
 #pragma unroll
     for (int r = 0; r < RM; r++) {
         float l = lrun[r];
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-        float *d = wo + (warp * ROWS + g + 8 * r) * HD + 2 * t4 * P::VB;
+        float *d = wo + (warp * ROWS + g + 8 * r) * ROW + t4 * RUN;
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            d[j] = o[j][2 * r];
-            d[P::VB + j] = o[j][2 * r + 1];
+        for (int j = 0; j < NT; j += 4) {
+            kv8_st4(d + j, make_float4(o[j][2 * r], o[j + 1][2 * r], o[j + 2][2 * r], o[j + 3][2 * r]));
+            kv8_st4(d + P::VB + j, make_float4(o[j][2 * r + 1], o[j + 1][2 * r + 1], o[j + 2][2 * r + 1], o[j + 3][2 * r + 1]));
         }
         if (t4 == 0) {
             wm[warp * ROWS + g + 8 * r] = mrun[r];
@@ -528,39 +532,42 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
         }
     }
     __syncthreads();
-    for (int idx = tid; idx < ROWS * HD / 4; idx += 32 * NW) {
-        const int r = idx / (HD / 4), d = 4 * (idx % (HD / 4)), R = R0 + r;
-        if (R >= n_rows) continue;
-        float M = -INFINITY, L = 0.0f;
+    constexpr int TR = 32 * NW / ROWS;      // threads of a row, 4 columns each and TR * 4 further
+    const int r = tid / TR, R = R0 + r, c0 = 4 * (tid % TR);
+    if (R >= n_rows) return;
+    float M = -INFINITY, L = 0.0f, f[NW];
 #pragma unroll
-        for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w * ROWS + r]);
+    for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w * ROWS + r]);
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        const float mw = wm[w * ROWS + r];
+        f[w] = mw == -INFINITY ? 1.0f : kv8_ex2(mw - M);   // an empty warp holds zeros
+        L = __fmaf_rn(wl[w * ROWS + r], f[w], L);
+    }
+    const int64_t row = (q.q0 + (int64_t)(R / G)) * H + kvh * G + R % G;
+    const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+#pragma unroll 2
+    for (int d = c0; d < HD; d += 4 * TR) {
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float mw = wm[w * ROWS + r], f = mw == -INFINITY ? 1.0f : exp2f(mw - M);   // an empty warp holds zeros
-            const float4 u = *reinterpret_cast<const float4 *>(wo + (w * ROWS + r) * HD + d);
-            L = __fmaf_rn(wl[w * ROWS + r], f, L);
-            v.x = __fmaf_rn(u.x, f, v.x);
-            v.y = __fmaf_rn(u.y, f, v.y);
-            v.z = __fmaf_rn(u.z, f, v.z);
-            v.w = __fmaf_rn(u.w, f, v.w);
+            const float4 u = *reinterpret_cast<const float4 *>(wo + (w * ROWS + r) * ROW + d + 4 * (d / (HD / 4)));
+            v.x = __fmaf_rn(u.x, f[w], v.x);
+            v.y = __fmaf_rn(u.y, f[w], v.y);
+            v.z = __fmaf_rn(u.z, f[w], v.z);
+            v.w = __fmaf_rn(u.w, f[w], v.w);
         }
-        const int64_t row = (q.q0 + (int64_t)(R / G)) * H + kvh * G + R % G;
+        if (a.n_split > 1) kv8_st4(a.po + (row * a.n_split + split) * HD + d, v);
+        else kv8_st4(out + row * HD + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    }
+    if (c0 == 0) {
         if (a.n_split > 1) {
-            const int64_t p = row * a.n_split + split;
-            kv8_st4(a.po + p * HD + d, v);
-            if (d == 0) {
-                a.pm[p] = M;
-                a.pl[p] = L;
-            }
+            a.pm[row * a.n_split + split] = M;
+            a.pl[row * a.n_split + split] = L;
         } else {
-            const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
-            kv8_st4(out + row * HD + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-            if (d == 0) {
-                const float l2 = M + log2f(L);
-                if (a.lse) a.lse[row] = l2 * LN2;
-                if (a.lse2) a.lse2[row] = l2;
-            }
+            const float l2 = M + log2f(L);
+            if (a.lse) a.lse[row] = l2 * LN2;
+            if (a.lse2) a.lse2[row] = l2;
         }
     }
 }
@@ -581,7 +588,7 @@ __global__ void __launch_bounds__(HD) k_kv8_join(const __grid_constant__ Kv8Attn
     for (int i = sl; i < n; i += 4) {
         const float mi = m[i], li = l[i];
         if (mi == -INFINITY && li == 0.0f) continue;            // a span without visible keys
-        const float f = mi == -INFINITY ? 1.0f : exp2f(mi - M);  // -inf with a sum: a NaN, which stays
+        const float f = mi == -INFINITY ? 1.0f : kv8_ex2(mi - M);  // -inf with a sum: a NaN, which stays
         const float4 u = *reinterpret_cast<const float4 *>(a.po + (row * n + i) * HD + d);
         L = __fmaf_rn(li, f, L);
         v.x = __fmaf_rn(u.x, f, v.x);
@@ -638,7 +645,7 @@ __global__ void __launch_bounds__(WG_THREADS) k_kv8_weights(const __grid_constan
         const int R1 = min(n_rows, (r + 1) * ROWS);
         for (int R = r * ROWS; R < R1; R++) {
             const float z = a.scores[((q.q0 + (int64_t)(R / a.G)) * a.H + kvh * a.G + R % a.G) * a.s_stride + t];
-            sum += z == -INFINITY ? 0.0f : exp2f(z - l2[R]);
+            sum += z == -INFINITY ? 0.0f : kv8_ex2(z - l2[R]);
         }
     }
     a.weights[((int64_t)s * a.c.KV + kvh) * a.w_stride + t] += sum;
@@ -725,7 +732,7 @@ template <int HD, int FMT, typename QT, int RM>
 int launch_split_rows(const Kv8Attn &a, const Split &p, cudaStream_t st) {
     auto fn = k_kv8_split<HD, FMT, QT, RM>;
     constexpr int ROWS = 8 * RM;
-    constexpr size_t join = (size_t)NW * ROWS * (HD + 2) * 4, sm = std::max<size_t>(Plan<HD>::SMEM, join);
+    constexpr size_t join = (size_t)NW * ROWS * (HD + 18) * 4, sm = std::max<size_t>(Plan<HD>::SMEM, join);
     if (!smem_opt_in((const void *)fn, sm)) return set_error(TLMG_EIO, "kv8_attend: shared memory opt-in failed");
     fn<<<dim3(p.n, (unsigned)(p.rtiles * a.c.KV), a.b.n_seq), 32 * NW, sm, st>>>(a);
     count_launch();
