@@ -73,10 +73,29 @@ __device__ __forceinline__ float warp_max(float a) {
 template <int FMT> __device__ __forceinline__ float scale_of(float amax) {
     return amax < INFINITY ? __fmul_rn(fmaxf(amax, KV8_FLOOR), 1.0f / kv8_qmax<FMT>()) : __uint_as_float(0x7FC00000u);
 }
-template <int FMT> __device__ __forceinline__ uint32_t codes4(float4 v, float d) {
+// The codes of x / d for four values. The quotient by the rounded reciprocal is within 2^-22 of the IEEE one; where
+// 2^-21 more and less of it round to the same code, that is the code, else (one value in some ten thousand) the
+// divisions are carried out.
+template <int FMT> __device__ __noinline__ uint32_t codes4_div(float4 v, float d) {
+    return kv8_code<FMT>(__fdiv_rn(v.x, d)) | (kv8_code<FMT>(__fdiv_rn(v.y, d)) << 8) | (kv8_code<FMT>(__fdiv_rn(v.z, d)) << 16) |
+           (kv8_code<FMT>(__fdiv_rn(v.w, d)) << 24);
+}
+template <int FMT> __device__ __forceinline__ uint32_t pack4(float x, float y, float z, float w) {
+    if constexpr (FMT == TLMG_KV8_INT8) {
+        return __byte_perm(__byte_perm((uint32_t)__float2int_rn(x), (uint32_t)__float2int_rn(y), 0x0040),
+                           __byte_perm((uint32_t)__float2int_rn(z), (uint32_t)__float2int_rn(w), 0x0040), 0x5410);
+    } else {
+        return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3) |
+               ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(z, w), __NV_SATFINITE, __NV_E4M3) << 16);
+    }
+}
+template <int FMT> __device__ __forceinline__ uint32_t codes4(float4 v, float d, float inv) {
     if (!(d == d)) return 0u;
-    return kv8_code<FMT>(__fdiv_rn(v.x, d)) | (kv8_code<FMT>(__fdiv_rn(v.y, d)) << 8) |
-           (kv8_code<FMT>(__fdiv_rn(v.z, d)) << 16) | (kv8_code<FMT>(__fdiv_rn(v.w, d)) << 24);
+    const float x = v.x * inv, y = v.y * inv, z = v.z * inv, w = v.w * inv;
+    constexpr float lo = 1.0f - 0x1p-21f, hi = 1.0f + 0x1p-21f;
+    const uint32_t c = pack4<FMT>(x * lo, y * lo, z * lo, w * lo);
+    if (c != pack4<FMT>(x * hi, y * hi, z * hi, w * hi)) return codes4_div<FMT>(v, d);
+    return c;
 }
 template <int FMT> __device__ __forceinline__ float4 values4(uint32_t w, float d) {
     return make_float4(__fmul_rn(kv8_value<FMT>(w & 255u), d), __fmul_rn(kv8_value<FMT>((w >> 8) & 255u), d),
@@ -108,19 +127,23 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_append(const Kv8View c, c
     float a = 0.0f;
     for (int i = lane; i < n4; i += 32) a = amax4(a, kv8_ld4(x + (int64_t)(i >> lper) * x_stride + 4 * (i & (per - 1))));
     float d = scale_of<FMT>(warp_max(a));
+    float old = 0.0f;
     if (t0 < ta) {   // rows of an earlier call
-        const float old = *scale;
+        old = *scale;
         if (!(old <= d)) d = d == d ? old : d;     // max(old, d); a NaN of either side stays
+    }
+    const float inv = __frcp_rn(d);
+    if (t0 < ta) {
         if (!(old == d)) {
             uint32_t *w = reinterpret_cast<uint32_t *>(codes);
-            for (int i = lane; i < (ta - t0) << lper; i += 32) w[i] = codes4<FMT>(values4<FMT>(w[i], old), d);
+            for (int i = lane; i < (ta - t0) << lper; i += 32) w[i] = codes4<FMT>(values4<FMT>(w[i], old), d, inv);
         }
         __syncwarp();                              // every lane has read the old scale
     }
     if (lane == 0) *scale = d;
     uint32_t *w = reinterpret_cast<uint32_t *>(codes + (size_t)(ta - t0) * c.hd);
     for (int i = lane; i < n4; i += 32)
-        w[i] = codes4<FMT>(kv8_ld4(x + (int64_t)(i >> lper) * x_stride + 4 * (i & (per - 1))), d);
+        w[i] = codes4<FMT>(kv8_ld4(x + (int64_t)(i >> lper) * x_stride + 4 * (i & (per - 1))), d, inv);
     if (c.pos && !is_v)
         for (int t = ta + lane; t < t1; t += 32)
             c.pos[r0 + (uint32_t)(t - t0)] = b.q_pos ? b.q_pos[q.q0 + (t - t_new)] : t;
@@ -166,53 +189,93 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 constexpr int SEL_THREADS = 1024;
 constexpr int SEL_BINS = 2048;
+constexpr int SEL_CLUSTER = 8;
+constexpr int SEL_ALONE = 8192;   // rows up to which one CTA is as fast as a cluster
 
-// One CTA per (sequence, KV head). The m-th largest key of the rows between
-// the first `sink` and the last `recent` is found digit by digit (11, 11 and
-// 10 bits, a shared-memory count of each digit), then one ordered pass
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+template <int CS> __device__ __forceinline__ void sync_all() {
+    if constexpr (CS == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ uint32_t ld_cluster(const uint32_t *p, uint32_t rank) {   // the word p of CTA `rank`'s shared memory
+    uint32_t a, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// One CTA, or a cluster of CS over long caches, per (sequence, KV head). The
+// m-th largest key of the rows between the first `sink` and the last `recent`
+// is found digit by digit (11, 11 and 10 bits, a shared-memory count of each
+// digit in every CTA's part, summed over the cluster), then one ordered pass
 // writes the rows above it and as many rows equal to it, lowest first, as m
-// leaves.
+// leaves. Latency-bound: the weights are 4 bytes a row; 32,768 rows took 61 us
+// with one CTA a head.
+template <int CS>
 __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_t *__restrict__ kv_len, int max_kv,
                                                             const float *__restrict__ weights, int64_t w_stride,
                                                             int n_keep, int sink, int recent, int32_t *__restrict__ rows,
                                                             int32_t *__restrict__ lens) {
-    __shared__ uint32_t hist[SEL_BINS];
-    __shared__ uint32_t wsum[2][32];
+    __shared__ uint32_t hist[2][SEL_BINS];
+    __shared__ uint32_t wsum[2][32], mine[2];
     __shared__ uint32_t pick_s, left_s;
-    const int kv = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int kv = blockIdx.x / CS, s = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t rank = CS > 1 ? cluster_rank() : 0u;
     const int L = min(max(kv_len[s], 0), max_kv);
     int32_t *out = rows + ((size_t)s * KV + kv) * n_keep;
     const float *w = weights + ((size_t)s * KV + kv) * w_stride;
-    if (kv == 0 && tid == 0 && lens) lens[s] = min(L, n_keep);
-    if (L <= n_keep) {
-        for (int j = tid; j < n_keep; j += SEL_THREADS) out[j] = j < L ? j : -1;
+    const int first = (int)rank * SEL_THREADS + tid, step = CS * SEL_THREADS;
+    if (kv == 0 && first == 0 && lens) lens[s] = min(L, n_keep);
+    if (L <= n_keep) {   // the same for the whole cluster
+        for (int j = first; j < n_keep; j += step) out[j] = j < L ? j : -1;
         return;
     }
-    const int lo = sink, hi = L - recent, m = n_keep - sink - recent;
-    for (int j = tid; j < sink; j += SEL_THREADS) out[j] = j;
-    for (int j = tid; j < recent; j += SEL_THREADS) out[n_keep - recent + j] = hi + j;
+    const int m = n_keep - sink - recent;
+    for (int j = first; j < sink; j += step) out[j] = j;
+    for (int j = first; j < recent; j += step) out[n_keep - recent + j] = L - recent + j;
     if (m == 0) return;
+    // this CTA's part of the rows between, a multiple of the warp
+    const int mid = L - recent - sink, part = ((mid + CS - 1) / CS + 31) / 32 * 32;
+    const int lo = sink + min(mid, (int)rank * part), hi = sink + min(mid, ((int)rank + 1) * part);
     uint32_t prefix = 0, left = (uint32_t)m;   // key bits found so far; rows still to take below them
     for (int pass = 0; pass < 3; pass++) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-        for (int i = tid; i < bins; i += SEL_THREADS) hist[i] = 0;
+        uint32_t *h = hist[pass & 1];          // the other one may still be read by the cluster
+        for (int i = tid; i < bins; i += SEL_THREADS) h[i] = 0;
         __syncthreads();
-        for (int t0 = lo; t0 < hi; t0 += SEL_THREADS) {
-            const int t = t0 + tid;
-            const uint32_t key = t < hi ? weight_key(w[t]) : 0u;
-            const bool in = t < hi && (pass == 0 || (key >> (shift + (pass == 2 ? 10 : 11))) == prefix);
-            const uint32_t bin = (key >> shift) & (uint32_t)(bins - 1);
-            // equal digits of a warp are counted once: accumulated weights hold many equal values
-            const uint32_t act = __ballot_sync(0xFFFFFFFFu, in);
-            if (in) {
-                const uint32_t peers = __match_any_sync(act, bin);
-                if (lane == __ffs(peers) - 1) atomicAdd(&hist[bin], (uint32_t)__popc(peers));
+        for (int t0 = lo; t0 < hi; t0 += 4 * SEL_THREADS) {
+            uint32_t key[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int t = t0 + u * SEL_THREADS + tid;
+                key[u] = t < hi ? weight_key(w[t]) : 0u;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const bool in = t0 + u * SEL_THREADS + tid < hi && (pass == 0 || (key[u] >> (shift + (pass == 2 ? 10 : 11))) == prefix);
+                const uint32_t bin = (key[u] >> shift) & (uint32_t)(bins - 1);
+                // equal digits of a warp are counted once: accumulated weights hold many equal values
+                const uint32_t act = __ballot_sync(0xFFFFFFFFu, in);
+                if (in) {
+                    const uint32_t peers = __match_any_sync(act, bin);
+                    if (lane == __ffs(peers) - 1) atomicAdd(&h[bin], (uint32_t)__popc(peers));
+                }
             }
         }
-        __syncthreads();
-        // suffix counts: thread i covers the bins / 1024 bins from the top
-        const int per = bins / SEL_THREADS;
-        uint32_t c0 = hist[bins - 1 - per * tid], c1 = per == 2 ? hist[bins - 2 - per * tid] : 0u, sum = c0 + c1;
+        sync_all<CS>();
+        // counts from the top: thread i covers the bins / 1024 bins there
+        const int per = bins / SEL_THREADS, b0 = bins - 1 - per * tid;
+        uint32_t c0 = 0, c1 = 0;
+#pragma unroll
+        for (int r = 0; r < CS; r++) {
+            c0 += CS == 1 ? h[b0] : ld_cluster(&h[b0], r);
+            if (per == 2) c1 += CS == 1 ? h[b0 - 1] : ld_cluster(&h[b0 - 1], r);
+        }
+        const uint32_t sum = c0 + c1;
         uint32_t inc = sum;
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
@@ -220,20 +283,12 @@ __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_
         }
         if (lane == 31) wsum[0][warp] = inc;
         __syncthreads();
-        if (warp == 0) {
-            uint32_t v = wsum[0][lane];
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, v, o);
-                if (lane >= o) v += u;
-            }
-            wsum[1][lane] = v;
-        }
-        __syncthreads();
-        const uint32_t upto = inc + (warp ? wsum[1][warp - 1] : 0u), before = upto - sum;
+        const uint32_t a = wsum[0][lane];
+        const uint32_t upto = inc + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? a : 0u), before = upto - sum;
         if (before < left && upto >= left) {       // exactly one thread
-            const bool first = before + c0 >= left;
-            pick_s = (uint32_t)(bins - 1 - per * tid) - (first ? 0u : 1u);
-            left_s = left - before - (first ? 0u : c0);
+            const bool hit = before + c0 >= left;
+            pick_s = (uint32_t)b0 - (hit ? 0u : 1u);
+            left_s = left - before - (hit ? 0u : c0);
         }
         __syncthreads();
         prefix = (prefix << (pass == 2 ? 10 : 11)) | pick_s;
@@ -242,6 +297,29 @@ __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_
     }
     // prefix is now the m-th largest key; `left` rows equal to it are taken
     uint32_t n_out = 0, n_eq = 0;
+    if constexpr (CS > 1) {   // rows larger and equal in the parts before this one
+        uint32_t g = 0, e = 0;
+        for (int t = lo + tid; t < hi; t += SEL_THREADS) {
+            const uint32_t key = weight_key(w[t]);
+            g += key > prefix;
+            e += key == prefix;
+        }
+        g = __reduce_add_sync(0xFFFFFFFFu, g);
+        e = __reduce_add_sync(0xFFFFFFFFu, e);
+        if (tid < 2) mine[tid] = 0;
+        __syncthreads();
+        if (lane == 0) {
+            atomicAdd(&mine[0], g);
+            atomicAdd(&mine[1], e);
+        }
+        sync_all<CS>();
+#pragma unroll
+        for (uint32_t r = 0; r < CS; r++)
+            if (r < rank) {
+                n_out += ld_cluster(&mine[0], r);
+                n_eq += ld_cluster(&mine[1], r);
+            }
+    }
     for (int t0 = lo; t0 < hi; t0 += SEL_THREADS) {
         const int t = t0 + tid;
         const uint32_t key = t < hi ? weight_key(w[t]) : 0u;
@@ -252,22 +330,17 @@ __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_
             wsum[1][warp] = __popc(be);
         }
         __syncthreads();
-        uint32_t g0 = n_out, e0 = n_eq, gt_all = 0, eq_all = 0;
-        {
-            const uint32_t a = wsum[0][lane], bq = wsum[1][lane];
-            uint32_t ga = lane < warp ? a : 0u, ea = lane < warp ? bq : 0u;
-            g0 += __reduce_add_sync(0xFFFFFFFFu, ga);
-            e0 += __reduce_add_sync(0xFFFFFFFFu, ea);
-            gt_all = __reduce_add_sync(0xFFFFFFFFu, a);
-            eq_all = __reduce_add_sync(0xFFFFFFFFu, bq);
-        }
+        const uint32_t a = wsum[0][lane], b = wsum[1][lane];
+        const uint32_t g0 = n_out + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? a : 0u);
+        const uint32_t e0 = n_eq + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? b : 0u);
         const uint32_t below = (1u << lane) - 1u;
         const uint32_t g = g0 + __popc(bg & below), q = e0 + __popc(be & below);   // larger / equal rows before t
         if (gt || (eq && q < left)) out[sink + (int)(g + min(q, left))] = t;
-        n_out += gt_all;
-        n_eq += eq_all;
+        n_out += __reduce_add_sync(0xFFFFFFFFu, a);
+        n_eq += __reduce_add_sync(0xFFFFFFFFu, b);
         __syncthreads();
     }
+    if constexpr (CS > 1) sync_all<CS>();   // no CTA leaves while another may read its shared memory
 }
 
 // One warp per (destination block, KV head, K or V).
@@ -289,36 +362,50 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_compact(const Kv8View c, 
     const int32_t de = (j0 >> d.lp) < dstride ? dtable[(size_t)s * dstride + (j0 >> d.lp)] : -1;
     const bool dok = d.ok(de);
     const uint32_t dr = dok ? d.row(de, kv, (int)j0) : 0u;
-    const int per = c.hd >> 2, lper = 31 - __clz(per);
     const uint8_t *pool = is_v ? c.v : c.k;
     const float *sc = is_v ? c.vs : c.ks;
-    // source row number of entry j, or -1; uniform over the lanes that share a row
+    // source row number of entry j
     auto source = [&](int j, uint32_t &r) {
-        const int32_t t = src[j];
+        const int32_t t = j < nj ? src[j] : -1;
         if (t < 0 || t >= L || (t >> c.lp) >= stride) return false;
         const int32_t e = table[(size_t)s * stride + (t >> c.lp)];
         if (!c.ok(e)) return false;
         r = c.row(e, kv, t);
         return true;
     };
+    // 32 rows a round: lane j finds row j's number and scale, then hd / 16 lanes share a row, 16 codes each
+    const int lpr = c.hd >> 4, rpi = 32 / lpr, sub = lane / lpr, at = 16 * (lane - sub * lpr);
+    auto rounds = [&](auto &&f) {
+        for (int j0 = 0; j0 < nj; j0 += 32) {
+            uint32_t r = 0;
+            const bool ok = source(j0 + lane, r);
+            const float v = ok ? sc[r >> c.lb] : 0.0f;
+            const int left = min(32, nj - j0);
+#pragma unroll 4
+            for (int i = 0; i < left; i += rpi) {
+                const uint32_t rr = __shfl_sync(0xFFFFFFFFu, r, i + sub);
+                const float vv = __shfl_sync(0xFFFFFFFFu, v, i + sub);
+                if (__shfl_sync(0xFFFFFFFFu, (int)ok, i + sub))
+                    f(j0 + i + sub, *reinterpret_cast<const uint4 *>(pool + (size_t)rr * c.hd + at), vv);
+            }
+        }
+    };
     float a = 0.0f;
     bool any = false;
-    for (int i = lane; i < nj << lper; i += 32) {
-        uint32_t r;
-        if (!source(i >> lper, r)) continue;
+    rounds([&](int, uint4 w, float v) {
         any = true;
-        a = amax4(a, values4<FS>(reinterpret_cast<const uint32_t *>(pool + (size_t)r * c.hd)[i & (per - 1)], sc[r >> c.lb]));
-    }
+        a = amax4(amax4(amax4(amax4(a, values4<FS>(w.x, v)), values4<FS>(w.y, v)), values4<FS>(w.z, v)), values4<FS>(w.w, v));
+    });
     any = __any_sync(0xFFFFFFFFu, any);
-    const float q = scale_of<FD>(warp_max(a));
+    const float q = scale_of<FD>(warp_max(a)), inv = __frcp_rn(q);
     if (dok && any) {
         if (lane == 0) (is_v ? d.vs : d.ks)[dr >> d.lb] = q;
-        uint32_t *w = reinterpret_cast<uint32_t *>((is_v ? d.v : d.k) + (size_t)dr * d.hd);
-        for (int i = lane; i < nj << lper; i += 32) {
-            uint32_t r;
-            if (!source(i >> lper, r)) continue;
-            w[i] = codes4<FD>(values4<FS>(reinterpret_cast<const uint32_t *>(pool + (size_t)r * c.hd)[i & (per - 1)], sc[r >> c.lb]), q);
-        }
+        uint8_t *to = (is_v ? d.v : d.k) + (size_t)dr * d.hd + at;
+        rounds([&](int j, uint4 w, float v) {
+            *reinterpret_cast<uint4 *>(to + (size_t)j * d.hd) =
+                make_uint4(codes4<FD>(values4<FS>(w.x, v), q, inv), codes4<FD>(values4<FS>(w.y, v), q, inv),
+                           codes4<FD>(values4<FS>(w.z, v), q, inv), codes4<FD>(values4<FS>(w.w, v), q, inv));
+        });
     }
     if (!is_v)
         for (int j = lane; j < nj; j += 32) {
@@ -405,8 +492,25 @@ extern "C" int tlmg_kv8_select(int n_seq, int KV, const int32_t *kv_len, int max
         return set_error(TLMG_EINVAL, "kv8_select: %d sequences x %d heads, max_kv %d, weight stride %lld, keep %d (%d first, %d last)",
                          n_seq, KV, max_kv, (long long)w_stride, n_keep, sink, recent);
     if (!kv_len || !weights || !rows) return set_error(TLMG_EINVAL, "kv8_select: null pointer");
-    k_kv8_select<<<dim3(KV, n_seq), SEL_THREADS, 0, pick_stream(stream)>>>(KV, kv_len, max_kv, weights, w_stride, n_keep, sink,
-                                                                          recent, rows, lens);
+    cudaStream_t st = pick_stream(stream);
+    if (max_kv <= SEL_ALONE) {
+        k_kv8_select<1><<<dim3(KV, n_seq), SEL_THREADS, 0, st>>>(KV, kv_len, max_kv, weights, w_stride, n_keep, sink, recent, rows, lens);
+    } else {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)KV * SEL_CLUSTER, n_seq);
+        cfg.blockDim = dim3(SEL_THREADS);
+        cfg.stream = st;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = SEL_CLUSTER;
+        at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, k_kv8_select<SEL_CLUSTER>, KV, kv_len, max_kv, weights, w_stride, n_keep, sink, recent,
+                                                 rows, lens);
+        if (e != cudaSuccess) return cuda_fail(e, "kv8_select launch");
+    }
     return launched("kv8_select launch");
 }
 

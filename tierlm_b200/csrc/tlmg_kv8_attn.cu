@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
     }
     __syncthreads();
     constexpr int TR = 32 * NW / ROWS;      // threads of a row, 4 columns each and TR * 4 further
-    const int r = tid / TR, R = R0 + r, c0 = 4 * (tid % TR);
+    const int r = tid / TR, R = R0 + r, col0 = 4 * (tid % TR);
     if (R >= n_rows) return;
     float M = -INFINITY, L = 0.0f, f[NW];
 #pragma unroll
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
     const int64_t row = (q.q0 + (int64_t)(R / G)) * H + kvh * G + R % G;
     const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
 #pragma unroll 2
-    for (int d = c0; d < HD; d += 4 * TR) {
+    for (int d = col0; d < HD; d += 4 * TR) {
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < NW; w++) {
@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
         if (a.n_split > 1) kv8_st4(a.po + (row * a.n_split + split) * HD + d, v);
         else kv8_st4(out + row * HD + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
     }
-    if (c0 == 0) {
+    if (col0 == 0) {
         if (a.n_split > 1) {
             a.pm[row * a.n_split + split] = M;
             a.pl[row * a.n_split + split] = L;
@@ -572,24 +572,31 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
     }
 }
 
-// out[row] = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M): one CTA of HD threads per output row
-// (HD / 4 column groups x 4 span slices).
+// out[row] = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M): one CTA per output row, HD / 4 column groups times the
+// slices of the spans that 256 threads leave. Every warp finds M by itself. (111 spans of one long sequence: one
+// slice of 4 with a serial maximum took 22 us.)
+constexpr int JOIN_THREADS = 256;
 template <int HD, typename QT>
-__global__ void __launch_bounds__(HD) k_kv8_join(const __grid_constant__ Kv8Attn a) {
+__global__ void __launch_bounds__(JOIN_THREADS) k_kv8_join(const __grid_constant__ Kv8Attn a) {
+    constexpr int CG = HD / 4, SL = JOIN_THREADS / CG;
     pdl_enter();
-    __shared__ float ro[4][HD], rl[4];
+    __shared__ __align__(16) float ro[SL][HD];
+    __shared__ float rl[SL];
     const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, sl = tid / (HD / 4), d = 4 * (tid % (HD / 4)), n = a.n_split;
-    const float *m = a.pm + row * n, *l = a.pl + row * n;
+    const int tid = threadIdx.x, sl = tid / CG, d = 4 * (tid % CG), n = a.n_split;
+    const float *m = a.pm + row * n, *l = a.pl + row * n, *po = a.po + row * n * HD + d;
     float M = -INFINITY;
-    for (int i = 0; i < n; i++) M = fmaxf(M, m[i]);
+    for (int i = tid & 31; i < n; i += 32) M = fmaxf(M, m[i]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
     float L = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i = sl; i < n; i += 4) {
+#pragma unroll 4
+    for (int i = sl; i < n; i += SL) {
         const float mi = m[i], li = l[i];
-        if (mi == -INFINITY && li == 0.0f) continue;            // a span without visible keys
-        const float f = mi == -INFINITY ? 1.0f : kv8_ex2(mi - M);  // -inf with a sum: a NaN, which stays
-        const float4 u = *reinterpret_cast<const float4 *>(a.po + (row * n + i) * HD + d);
+        if (mi == -INFINITY && li == 0.0f) continue;                // a span without visible keys
+        const float f = mi == -INFINITY ? 1.0f : kv8_ex2(mi - M);   // -inf with a sum: a NaN, which stays
+        const float4 u = *reinterpret_cast<const float4 *>(po + (size_t)i * HD);
         L = __fmaf_rn(li, f, L);
         v.x = __fmaf_rn(u.x, f, v.x);
         v.y = __fmaf_rn(u.y, f, v.y);
@@ -600,11 +607,13 @@ __global__ void __launch_bounds__(HD) k_kv8_join(const __grid_constant__ Kv8Attn
     if (d == 0) rl[sl] = L;
     __syncthreads();
     if (sl) return;
-    for (int k = 1; k < 4; k++) {
-        v.x += ro[k][d];
-        v.y += ro[k][d + 1];
-        v.z += ro[k][d + 2];
-        v.w += ro[k][d + 3];
+#pragma unroll
+    for (int k = 1; k < SL; k++) {
+        const float4 u = *reinterpret_cast<const float4 *>(&ro[k][d]);
+        v.x += u.x;
+        v.y += u.y;
+        v.z += u.z;
+        v.w += u.w;
         L += rl[k];
     }
     const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
@@ -738,7 +747,7 @@ int launch_split_rows(const Kv8Attn &a, const Split &p, cudaStream_t st) {
     count_launch();
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess && p.n > 1) {
-        e = launch_dep(k_kv8_join<HD, QT>, dim3((unsigned)((int64_t)a.b.total_q * a.H)), HD, a, st);
+        e = launch_dep(k_kv8_join<HD, QT>, dim3((unsigned)((int64_t)a.b.total_q * a.H)), JOIN_THREADS, a, st);
         count_launch();
     }
     if (e == cudaSuccess && a.weights) {

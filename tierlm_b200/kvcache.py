@@ -17,9 +17,18 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import BF16, F16, F32, TlmError, check, load
-from .quant import _dev, stream_handle
+from .quant import CUDA_STREAM_LEGACY, _dev
 
 INT8, E4M3 = 1, 2
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(index: int) -> int:
+    """The current stream of a device for the C calls (see quant.stream_handle; without building a Stream object)."""
+    s = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+    return s if s else CUDA_STREAM_LEGACY
+
+
 _FMT = {torch.int8: INT8, torch.float8_e4m3fn: E4M3}
 _X_DT = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
@@ -64,22 +73,23 @@ def _f32(t: torch.Tensor | None, what: str, shape: tuple | None = None) -> int |
     return _dev(t, what)
 
 
-def _rows(t: torch.Tensor, what: str, heads: int, hd: int) -> tuple[torch.Tensor, int]:
-    """[n][heads][hd] rows and their stride in elements; a copy where the
-    library cannot read them in place (heads apart, rows off 16 bytes)."""
+def _rows(t: torch.Tensor, what: str, heads: int, hd: int) -> tuple[torch.Tensor, int, int]:
+    """[n][heads][hd] rows, their stride in elements and their address; a copy
+    where the library cannot read them in place (heads apart, rows off 16 bytes)."""
     if t.dtype not in _X_DT:
         raise TlmError(-3, f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
     if t.dim() != 3 or t.shape[1:] != (heads, hd):
         raise TlmError(-3, f"{what} has shape {tuple(t.shape)}, not [n][{heads}][{hd}]")
     if not t.is_cuda:
         raise TlmError(-3, f"{what} must be a CUDA tensor")
-    st = t.stride(0)
-    if t.stride(2) != 1 or t.stride(1) != hd or st < heads * hd or st * t.element_size() % 16 or t.data_ptr() % 16:
+    st, sh, sd = t.stride()
+    at = t.data_ptr()
+    if sd != 1 or sh != hd or st < heads * hd or st * (4 if t.dtype is torch.float32 else 2) % 16 or at % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-        st = heads * hd
-    return t, st
+        st, at = heads * hd, t.data_ptr()
+    return t, st, at
 
 
 class Kv8Batch:
@@ -99,12 +109,14 @@ class Kv8Batch:
         self.max_q, self.max_kv = max_q, max_kv
         self._c = _Batch(_i32(page_table, "page_table"), _i32(q_start, "q_start", (n_seq + 1,)),
                          _i32(kv_len, "kv_len", (n_seq,)), _i32(q_pos, "q_pos"), n_seq, stride, 0, max_q, max_kv)
+        self._p = C.addressof(self._c)
 
-    def _at(self, total: int) -> _Batch:
+    def _at(self, total: int) -> int:
+        """The address of the C struct for a call on `total` tokens."""
         if self.q_pos is not None and self.q_pos.numel() < total:
             raise TlmError(-3, f"q_pos has {self.q_pos.numel()} entries for {total} tokens")
         self._c.total_q = total
-        return self._c
+        return self._p
 
 
 @dataclass(frozen=True)
@@ -121,17 +133,20 @@ class Score:
     prefix: torch.Tensor | None = None
     doc: torch.Tensor | None = None
 
-    def _at(self, n_seq: int, H: int) -> _Score:
+    def _at(self, n_seq: int, H: int) -> int:
+        """The address of the C struct for a call on n_seq sequences and H heads."""
         key = (n_seq, H)
-        if getattr(self, "_made", None) != key:
+        if self.__dict__.get("_made") != key:
             if self.doc is not None and (self.doc.dim() != 2 or self.doc.shape[0] != n_seq):
                 raise TlmError(-3, f"doc has shape {tuple(self.doc.shape)}, not [{n_seq}][positions]")
             c = _Score(self.scale, self.softcap, _f32(self.slopes, "slopes", (H,)),
                        _i32(self.prefix, "prefix", (n_seq,)), _i32(self.doc, "doc"),
                        self.doc.shape[1] if self.doc is not None else 0, 1 if self.causal else 0, self.window)
-            object.__setattr__(self, "_c", c)   # built once: the fields never change
-            object.__setattr__(self, "_made", key)
-        return self._c
+            self.__dict__.update(_c=c, _p=C.addressof(c), _made=key)   # built once: the fields never change
+        return self._p
+
+
+_PLAIN = Score()
 
 
 class Kv8Cache:
@@ -174,21 +189,24 @@ class Kv8Cache:
         self._c = _Cache(_dev(k, "k"), _dev(v, "v"), _f32(k_scale, "k_scale", (n_pages, KV, blocks)),
                          _f32(v_scale, "v_scale", (n_pages, KV, blocks)), _i32(pos, "pos", (n_pages, KV, page)),
                          self.fmt, n_pages, KV, page, self.block, hd)
-        self._lib = load()
-        self._work: dict[int, torch.Tensor] = {}
+        self._p = C.addressof(self._c)
+        self._dev = k.device.index or 0
+        lib = load()
+        self._append, self._read, self._attend = lib.tlmg_kv8_append, lib.tlmg_kv8_read, lib.tlmg_kv8_attend
+        self._need, self._select, self._compact = lib.tlmg_kv8_attend_work_bytes, lib.tlmg_kv8_select, lib.tlmg_kv8_compact
+        self._work: dict[int, tuple[int, int, torch.Tensor]] = {}    # stream -> size, address, scratch
 
     def append(self, k: torch.Tensor, v: torch.Tensor, batch: Kv8Batch) -> None:
         """Stores the batch's new rows k, v [n][KV][hd] (float32, float16 or
         bfloat16)."""
-        k, sk = _rows(k, "k", self.KV, self.hd)
-        v, sv = _rows(v, "v", self.KV, self.hd)
+        k, sk, kp = _rows(k, "k", self.KV, self.hd)
+        v, sv, vp = _rows(v, "v", self.KV, self.hd)
         if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
             raise TlmError(-3, f"k and v differ: {k.dtype} x {k.shape[0]} rows, {v.dtype} x {v.shape[0]} rows")
         if sk != sv:
             k, v = k.contiguous(), v.contiguous()
-            sk = self.KV * self.hd
-        check(self._lib.tlmg_kv8_append(C.byref(self._c), C.byref(batch._at(k.shape[0])), _X_DT[k.dtype], k.data_ptr(),
-                                        v.data_ptr(), sk, stream_handle()))
+            sk, kp, vp = self.KV * self.hd, k.data_ptr(), v.data_ptr()
+        check(self._append(self._p, batch._at(k.shape[0]), _X_DT[k.dtype], kp, vp, sk, _stream(self._dev)))
 
     def read(self, page_table: torch.Tensor, row0: torch.Tensor, start: torch.Tensor, total: int,
              k: torch.Tensor | None = None, v: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -196,11 +214,11 @@ class Kv8Cache:
         start[s + 1] - 1 of the results [total][KV][hd])."""
         n_seq, stride = page_table.shape
         shape = (total, self.KV, self.hd)
-        k = torch.empty(shape, device=self.k.device) if k is None else k
-        v = torch.empty(shape, device=self.k.device) if v is None else v
-        check(self._lib.tlmg_kv8_read(C.byref(self._c), n_seq, _i32(page_table, "page_table"), stride,
-                                      _i32(row0, "row0", (n_seq,)), _i32(start, "start", (n_seq + 1,)), total,
-                                      _f32(k, "k", shape), _f32(v, "v", shape), stream_handle()))
+        k = torch.empty(shape, dtype=torch.float32, device=self.k.device) if k is None else k
+        v = torch.empty_like(k) if v is None else v
+        check(self._read(self._p, n_seq, _i32(page_table, "page_table"), stride, _i32(row0, "row0", (n_seq,)),
+                         _i32(start, "start", (n_seq + 1,)), total, _f32(k, "k", shape), _f32(v, "v", shape),
+                         _stream(self._dev)))
         return k, v
 
     def attend(self, q: torch.Tensor, batch: Kv8Batch, score: Score | None = None, out: torch.Tensor | None = None,
@@ -209,34 +227,35 @@ class Kv8Cache:
         rows -> out (q's dtype), or (out, lse) with lse. weights float32
         [n_seq][KV][rows >= max_kv] accumulates every row's softmax weights
         (what evict goes by); max_q <= 64 then."""
-        if q.dim() != 3:
-            raise TlmError(-3, f"q has shape {tuple(q.shape)}, not [n][H][{self.hd}]")
-        H = q.shape[1]
-        q, sq = _rows(q, "q", H, self.hd)
-        b = batch._at(q.shape[0])
-        s = (score or Score())._at(batch.n_seq, H)
+        shape = q.shape
+        if len(shape) != 3:
+            raise TlmError(-3, f"q has shape {tuple(shape)}, not [n][H][{self.hd}]")
+        n, H = shape[0], shape[1]
+        q, sq, qp = _rows(q, "q", H, self.hd)
+        b = batch._at(n)
+        s = (score or _PLAIN)._at(batch.n_seq, H)
         dt = _X_DT[q.dtype]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            raise TlmError(-3, f"out is {out.dtype} {tuple(out.shape)}, q {q.dtype} {tuple(q.shape)}")
-        want = lse is True or isinstance(lse, torch.Tensor)
-        lse_t = lse if isinstance(lse, torch.Tensor) else torch.empty(q.shape[:2], device=q.device) if want else None
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        elif out.shape != shape or out.dtype != q.dtype:
+            raise TlmError(-3, f"out is {out.dtype} {tuple(out.shape)}, q {q.dtype} {tuple(shape)}")
+        lse_t = None
+        if lse is not False and lse is not None:
+            lse_t = torch.empty((n, H), dtype=torch.float32, device=q.device) if lse is True else lse
         w_stride = 0
         if weights is not None:
             if weights.dim() != 3 or weights.shape[:2] != (batch.n_seq, self.KV):
                 raise TlmError(-3, f"weights have shape {tuple(weights.shape)}, not [{batch.n_seq}][{self.KV}][rows]")
             w_stride = weights.shape[2]
-        st = stream_handle()
-        need = self._lib.tlmg_kv8_attend_work_bytes(C.byref(self._c), C.byref(b), C.byref(s), H, dt,
-                                                    0 if weights is None else 1)
-        work = self._work.get(st)
-        if work is None or work.numel() < need:
-            work = self._work[st] = torch.empty(max(need, 1 << 20), dtype=torch.uint8, device=q.device)
-        check(self._lib.tlmg_kv8_attend(C.byref(self._c), C.byref(b), C.byref(s), H, dt, q.data_ptr(), sq,
-                                        _dev(out, "out"), _f32(lse_t, "lse", tuple(q.shape[:2])),
-                                        _f32(weights, "weights"), w_stride, work.data_ptr(), work.numel(), st))
-        return (out, lse_t) if want else out
+        st = _stream(self._dev)
+        need = self._need(self._p, b, s, H, dt, 0 if weights is None else 1)
+        have = self._work.get(st)
+        if have is None or have[0] < need:
+            work = torch.empty(max(need, 1 << 20), dtype=torch.uint8, device=q.device)
+            have = self._work[st] = (work.numel(), work.data_ptr(), work)
+        check(self._attend(self._p, b, s, H, dt, qp, sq, _dev(out, "out"), _f32(lse_t, "lse", (n, H)),
+                           _f32(weights, "weights"), w_stride, have[1], have[0], st))
+        return out if lse_t is None else (out, lse_t)
 
     def evict(self, weights: torch.Tensor, batch: Kv8Batch, dst_table: torch.Tensor, n_keep: int, sink: int = 0,
               recent: int = 0, dst: "Kv8Cache | None" = None, weights_out: torch.Tensor | None = None,
@@ -257,12 +276,12 @@ class Kv8Cache:
             raise TlmError(-3, f"weights_out has shape {tuple(weights_out.shape)}, not [{n}][{self.KV}][rows]")
         rows = torch.empty((n, self.KV, max(n_keep, 0)), dtype=torch.int32, device=dev) if rows is None else rows
         lens = torch.empty((n,), dtype=torch.int32, device=dev) if lens is None else lens
-        st = stream_handle()
+        st = _stream(self._dev)
         w = _f32(weights, "weights")
         r = _i32(rows, "rows", (n, self.KV, n_keep))
-        check(self._lib.tlmg_kv8_select(n, self.KV, batch._c.kv_len, batch.max_kv, w, weights.shape[2], n_keep, sink,
+        check(self._select(n, self.KV, batch._c.kv_len, batch.max_kv, w, weights.shape[2], n_keep, sink,
                                         recent, r, _i32(lens, "lens", (n,)), st))
-        check(self._lib.tlmg_kv8_compact(C.byref(self._c), C.byref(d._c), n, batch._c.page_table, batch._c.table_stride,
+        check(self._compact(self._p, d._p, n, batch._c.page_table, batch._c.table_stride,
                                          batch._c.kv_len, _i32(dst_table, "dst_table"), dst_table.shape[1], r, n_keep, w,
                                          weights.shape[2], _f32(weights_out, "weights_out"),
                                          0 if weights_out is None else weights_out.shape[2], st))
