@@ -1,9 +1,9 @@
 // tlmg_kv8_prefill.cu - attention over the 8-bit KV cache for many query rows,
-// on tcgen05 (16-bit queries, head_dim 64 and 128).
+// on tcgen05 (head_dim 64 and 128).
 //
-// One CTA per SM takes 256 query rows (token, head of the group) of one KV
-// head in two tiles A and B of 128, and walks the visible keys in tiles of
-// 128. Roles, 28 warps:
+// 16-bit queries: one CTA per SM takes 256 query rows (token, head of the
+// group) of one KV head in two tiles A and B of 128, and walks the visible keys
+// in tiles of 128. Roles, 28 warps:
 //   warps 0-7, 8-15  softmax of tile A, B: two threads per query row (= TMEM lane), each with half of the keys
 //   warps 16-23      K and V codes -> f16 in shared memory, once for both tiles
 //   warps 24-27      the first issues the MMAs (a warpgroup, for its share of the registers)
@@ -28,6 +28,11 @@
 // bytes are K as a K-major B operand (contraction over dims) and V as an
 // MN-major one (contraction over keys).
 //
+// f32 queries (one query tile a CTA): Q and P are two f16 each, the high part and the remainder (P's times 2^11); S
+// sums the two products of Q, O's two products stay apart, start from zero at every key tile and are added to f32
+// registers a tile later, since the tensor core's sums truncate. S has two buffers, so the next tile's scores form
+// while this one's are weighed.
+//
 // Every wait is bounded: a role whose wait runs out sets a flag, all roles
 // leave, and the CTA's outputs are NaN.
 #include <cstdint>
@@ -44,12 +49,18 @@ namespace {
 
 constexpr int TK = 128;           // keys of a tile
 constexpr int TQ = 128;           // query rows of a tile
-constexpr int THREADS = 28 * 32;
 constexpr int CK = 16;            // columns of a round of the softmax loops: few registers, four warps a scheduler
 constexpr int HC = TK / 2;        // keys of a softmax thread: two threads share a query row
 constexpr int CV = 256;           // converting threads
-// Registers a thread: 72 at launch (896 x 72 = 64,512), then 512 x 80 + 256 x 56 + 128 x 72 = 64,512.
-constexpr int REGS_SOFTMAX = 80, REGS_CONVERT = 56, REGS_MMA = 72;
+// What differs between 16-bit queries (two query tiles in turn) and f32 ones (one tile of which every operand but K and V
+// has a high and a low part). Registers a thread: 16-bit 72 at launch (896 x 72 = 64,512), then 512 x 80 + 256 x 56 +
+// 128 x 72 = 64,512; f32 96 at launch (640 x 96 = 61,440), then 256 x 144 + 256 x 56 + 128 x 72 = 60,416.
+template <bool F32> struct Role {
+    static constexpr int TILES = F32 ? 1 : 2;                 // query tiles of a CTA
+    static constexpr int SW = 8 * TILES;                      // softmax warps; then 8 that convert and 4 for the MMAs
+    static constexpr int THREADS = 32 * (SW + 12);
+    static constexpr int REGS_SOFTMAX = F32 ? 144 : 80, REGS_CONVERT = 56, REGS_MMA = 72;
+};
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int META = 4;           // buffers of per-key scales
@@ -221,6 +232,12 @@ __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// what the f16 pair h leaves of x, y, times `mul`, as f16
+__device__ __forceinline__ uint32_t rest_f16(float x, float y, uint32_t h, float mul) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+    return pack_f16((x - f.x) * mul, (y - f.y) * mul);
+}
+
 // softcap * log2(e) * tanh(y) by the exponential
 __device__ __forceinline__ float cap_exp(float y, float capl) {
     return __fmaf_rn(-2.0f * capl, __fdividef(1.0f, ex2(y * (2.0f * LOG2E)) + 1.0f), capl);
@@ -231,9 +248,12 @@ constexpr float TOP = 14.0f;   // log2 of the largest p * v_scale right after a 
 // SHAPED: softcap, slopes, documents or a position pool; without them the code is half the size, and the instruction
 // cache is what these roles share most tightly.
 template <int HD, int FMT, typename QT, bool SHAPED>
-__global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constant__ Kv8Attn a) {
+__global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefill(const __grid_constant__ Kv8Attn a) {
     extern __shared__ __align__(128) uint8_t raw[];
     Smem<HD> &sm = *reinterpret_cast<Smem<HD> *>(raw);
+    constexpr bool F32 = sizeof(QT) == 4;
+    using RL = Role<F32>;
+    constexpr int THREADS = RL::THREADS, SW = RL::SW, RPC = RL::TILES * TQ;   // query rows of the CTA
     constexpr int SBO = HD * 16;              // bytes between 8-row groups of an operand
     constexpr int PC = HD / 16;               // 16-byte pieces of a code row
     constexpr int NP = TK * PC / CV;          // pieces of half a tile per converting thread
@@ -254,10 +274,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     }
     // R / G for the rows of a call (fewer than 2^20): the division's own code would be a good part of the start
     auto token_of = [&](int R) { return (int)__umulhi((uint32_t)R, a.inv_g) + (a.G == 1 ? R : 0); };
-    const int n_rows = q.n * a.G, R0 = rt * 2 * TQ;
+    const int n_rows = q.n * a.G, R0 = rt * RPC;
     if (R0 >= n_rows) return;
-    const bool two = R0 + TQ < n_rows;
-    const int i0 = token_of(R0), i1 = min(q.n, token_of(R0 + 2 * TQ - 1) + 1);
+    const bool two = !F32 && R0 + TQ < n_rows;
+    const int i0 = token_of(R0), i1 = min(q.n, token_of(R0 + RPC - 1) + 1);
     if (tid == 0) {
         sm.abort = 0;
         sm.pmin = INT32_MAX;
@@ -277,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
         mbar_init(&sm.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 24) {
+    if (warp == SW + 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -296,9 +316,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     const int32_t *docs = a.doc ? a.doc + (size_t)s * a.doc_stride : nullptr;
     const int n = rg.n;
 
-    if (warp < 16) {
+    if (warp < SW) {
         // ---- softmax of one query tile ----
-        regs_up<REGS_SOFTMAX>();
+        regs_up<RL::REGS_SOFTMAX>();
         const int w = warp >> 3, half = (warp >> 2) & 1, r = tid & (TQ - 1), k0 = half * HC;
         if (w == 0 || two) {
             const int R = R0 + w * TQ + r;
@@ -314,17 +334,27 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                 const int r8 = lane & 7, cq = lane >> 3;
 #pragma unroll 1
                 for (int g = 0; g < 2; g++) {
-                    uint4 x[HD / 32];
+                    float4 x[F32 ? HD / 32 : 1][2];
+                    uint4 x16[HD / 32];
                     const int rr = R0 + w * TQ + (warp & 7) * 16 + 8 * g + r8;
                     const int tk = rr < n_rows ? token_of(rr) : i0, hh = kvh * a.G + (rr < n_rows ? rr - tk * a.G : 0);
                     const QT *src = static_cast<const QT *>(a.q) + (q.q0 + (int64_t)tk) * a.q_stride + hh * HD + 8 * cq;
+                    // elements 8 i .. of chunk i
+                    auto get = [&](int i, float4 &u, float4 &v) {
+                        if constexpr (F32) u = x[i][0], v = x[i][1];
+                        else u = kv8_ld4(reinterpret_cast<const QT *>(&x16[i])), v = kv8_ld4(reinterpret_cast<const QT *>(&x16[i]) + 4);
+                    };
 #pragma unroll
-                    for (int i = 0; i < HD / 32; i++) x[i] = *reinterpret_cast<const uint4 *>(src + 32 * i);
+                    for (int i = 0; i < HD / 32; i++) {
+                        if constexpr (F32) x[i][0] = kv8_ld4(src + 32 * i), x[i][1] = kv8_ld4(src + 32 * i + 4);
+                        else x16[i] = *reinterpret_cast<const uint4 *>(src + 32 * i);
+                    }
                     const int row = (warp & 7) * 16 + 8 * g + r8;
                     float m = 0.0f;
 #pragma unroll
                     for (int i = 0; i < HD / 32; i++) {
-                        const float4 u = kv8_ld4(reinterpret_cast<const QT *>(&x[i])), v = kv8_ld4(reinterpret_cast<const QT *>(&x[i]) + 4);
+                        float4 u, v;
+                        get(i, u, v);
                         m = fmaxf(m, fmaxf(fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))),
                                            fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)))));
                     }
@@ -336,9 +366,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                     uint8_t *dst = sm.q[w] + (row >> 3) * SBO + (row & 7) * 16 + cq * 128;
 #pragma unroll
                     for (int i = 0; i < HD / 32; i++) {
-                        const float4 u = kv8_ld4(reinterpret_cast<const QT *>(&x[i])), v = kv8_ld4(reinterpret_cast<const QT *>(&x[i]) + 4);
-                        *reinterpret_cast<uint4 *>(dst + 512 * i) = make_uint4(pack_f16(u.x * up, u.y * up), pack_f16(u.z * up, u.w * up),
-                                                                             pack_f16(v.x * up, v.y * up), pack_f16(v.z * up, v.w * up));
+                        float4 u, v;
+                        get(i, u, v);
+                        const uint4 hi = make_uint4(pack_f16(u.x * up, u.y * up), pack_f16(u.z * up, u.w * up),
+                                                    pack_f16(v.x * up, v.y * up), pack_f16(v.z * up, v.w * up));
+                        *reinterpret_cast<uint4 *>(dst + 512 * i) = hi;
+                        if constexpr (F32)
+                            *reinterpret_cast<uint4 *>(dst + TQ * HD * 2 + 512 * i) =
+                                make_uint4(rest_f16(u.x * up, u.y * up, hi.x, 1.0f), rest_f16(u.z * up, u.w * up, hi.y, 1.0f),
+                                           rest_f16(v.x * up, v.y * up, hi.z, 1.0f), rest_f16(v.z * up, v.w * up, hi.w, 1.0f));
                     }
                 }
                 fence_async_smem();
@@ -347,15 +383,34 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             bool ok = mbar_wait_warp(&sm.q_full, 0, &sm.abort);
             const float qsc = sm.qs[w][r];
             const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // this warp's 32 TMEM lanes
-            const uint32_t ts = tmem + lanes + w * TK, to = tmem + lanes + 2 * TK + w * HD;
+            const uint32_t to = tmem + lanes + 2 * TK + w * HD;          // O (f32 queries: then O of the remainders)
             const bool lists = SHAPED && (docs || a.c.pos);        // masks that go by a table
             const float qs2 = qsc * LOG2E, capl = a.softcap * LOG2E, capx = qsc * a.inv_cap;
             const float mul = SHAPED && a.softcap > 0.0f ? capx : qs2;
             float wref = -INFINITY, lsum = 0.0f;
+            // f32 queries: this thread's half of the row's output, and what the reference's last move multiplies it by
+            float o[F32 ? HD / 2 : 1], fo = 1.0f;
+            auto add_o = [&] {
+#pragma unroll
+                for (int c = 0; c < (F32 ? HD / 2 : 0); c += 16) {
+                    uint32_t hi[16], lo[16];
+                    tmem_ldc(to + half * (HD / 2) + c, hi);
+                    tmem_ldc(to + HD + half * (HD / 2) + c, lo);
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        o[c + i] = __fmaf_rn(o[c + i], fo, __fmaf_rn(__uint_as_float(lo[i]), 0x1p-11f, __uint_as_float(hi[i])));
+                }
+            };
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < HD / 2; i++) o[i] = 0.0f;
+            }
 #pragma unroll 1
             for (int j = 0; ok && j < n; j++) {
                 const int t0 = rg.t0(j), mb = j & (META - 1);
-                ok = mbar_wait_warp(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait_warp(&sm.s_full[w], j & 1, &sm.abort);
+                const int sb = F32 ? j & 1 : w;                     // buffer of S
+                const uint32_t ts = tmem + lanes + sb * TK;
+                ok = mbar_wait_warp(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait_warp(&sm.s_full[sb], F32 ? (j >> 1) & 1 : j & 1, &sm.abort);
                 if (!ok) break;
                 tc_after();
                 const float *ks = sm.ks[mb], *vs = sm.vs[mb], *lv = sm.lv[mb];
@@ -494,11 +549,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                 if (!ok) break;
                 m0 = fmaxf(m0, sm.part[w][half ^ 1][r]);
                 const bool grow = m0 > wref + 1.0f;
+                float fnew = 1.0f;
                 if (__any_sync(0xFFFFFFFFu, grow)) {
                     const float f = grow && wref != -INFINITY ? ex2(wref - m0) : 1.0f;
                     if (grow) wref = m0;
                     lsum *= f;
-                    if (j > 0) {
+                    fnew = f;
+                    if (!F32 && j > 0) {
 #pragma unroll 1
                         for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += CK) {
                             tmem_ldc(to + c, xa);
@@ -526,12 +583,38 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                                 upk(fma2(pku(xa[g + i], xa[g + i + 1]), k2, o2), y[i], y[i + 1]);
                                 y[i] = ex2(y[i]), y[i + 1] = ex2(y[i + 1]);
                                 p[(g + i) / 2] = pack_f16(y[i], y[i + 1]);
+                                if constexpr (F32) xa[(g + i) / 2] = rest_f16(y[i], y[i + 1], p[(g + i) / 2], 0x1p11f);
                             }
                             float u0, u1;
                             upk(add2(add2(pk(y[0], y[1]), pk(y[2], y[3])), add2(pk(y[4], y[5]), pk(y[6], y[7]))), u0, u1);
                             lsum = __fmaf_rn(u0 + u1, sm.rv[mb][c + g], lsum);
                         }
-                        tmem_st8(ts + (c + k0) / 2, p);   // columns whose scores are read already
+                        if constexpr (F32) {   // high parts and remainders of 16 keys over their 16 scores
+                            tmem_st8(ts + c, p);
+#pragma unroll
+                            for (int i = 0; i < CK / 2; i++) p[i] = xa[i];
+                            tmem_st8(ts + c + 8, p);
+                        } else {
+                            tmem_st8(ts + (c + k0) / 2, p);   // columns whose scores are read already
+                        }
+                    }
+                } else if constexpr (F32) {
+#pragma unroll 1
+                    for (int c = k0; c < k0 + HC; c += CK) {
+                        uint32_t p[CK / 2];
+                        tmem_ldc(ts + c, xa);
+#pragma unroll
+                        for (int i = 0; i < CK; i += 2) {
+                            const float y0 = __uint_as_float(xa[i]), y1 = __uint_as_float(xa[i + 1]), e0 = ex2(y0 + sub), e1 = ex2(y1 + sub);
+                            lsum += e0 + e1;
+                            const float u0 = y0 == -INFINITY ? 0.0f : e0 * vs[c + i], u1 = y1 == -INFINITY ? 0.0f : e1 * vs[c + i + 1];
+                            p[i / 2] = pack_f16(u0, u1);
+                            xa[i / 2] = rest_f16(u0, u1, p[i / 2], 0x1p11f);
+                        }
+                        tmem_st8(ts + c, p);
+#pragma unroll
+                        for (int i = 0; i < CK / 2; i++) p[i] = xa[i];
+                        tmem_st8(ts + c + 8, p);
                     }
                 } else {
 #pragma unroll 1
@@ -551,6 +634,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                     }
                 }
                 tmem_wait_st();
+                if constexpr (F32) {   // the last tile's product: the next one starts over it
+                    if (j > 0) {
+                        ok = mbar_wait_warp(&sm.o_full[0], (j - 1) & 1, &sm.abort);
+                        if (!ok) break;
+                        tc_after();
+                        add_o();
+                    }
+                    fo = fnew;
+                }
                 tc_before();
                 mbar_arrive(&sm.p_full[w]);
             }
@@ -558,13 +650,20 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             if (ok && n > 0) {
                 sm.sums[w][half][r] = lsum;
                 mbar_arrive(&sm.x_full[w]);
-                ok = mbar_wait_warp(&sm.x_full[w], n & 1, &sm.abort) && mbar_wait_warp(&sm.o_full[w], 0, &sm.abort);
+                ok = mbar_wait_warp(&sm.x_full[w], n & 1, &sm.abort) && mbar_wait_warp(&sm.o_full[w], F32 ? (n - 1) & 1 : 0, &sm.abort);
                 l = lsum + sm.sums[w][half ^ 1][r];
             }
             tc_after();
             const float inv = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? 0.0f : __fdividef(kv8_f16_unit<FMT>(), l);
+            if constexpr (F32) {
+                if (ok && n > 0) add_o();
+                if (live)
+#pragma unroll
+                    for (int i = 0; i < HD / 2; i += 4)
+                        kv8_st4(out + orow * HD + half * (HD / 2) + i, make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
+            }
 #pragma unroll 1
-            for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+            for (int c = half * (HD / 2); !F32 && c < (half + 1) * (HD / 2); c += 32) {
                 uint32_t x[32];
                 if (ok && n > 0) {
                     tmem_ld32(to + c, x);
@@ -586,10 +685,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             if (live && half == 0 && a.lse)
                 a.lse[orow] = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? -INFINITY : (log2f(l) - (wref == -INFINITY ? 0.0f : TOP - wref)) * LN2;
         }
-    } else if (warp < 24) {
+    } else if (warp < SW + 8) {
         // ---- codes to f16 ----
-        regs_down<REGS_CONVERT>();
-        const int c = tid - 512;
+        regs_down<RL::REGS_CONVERT>();
+        const int c = tid - 32 * SW;
         const bool is_v = c >= CV / 2;            // half of the warps convert K, half V: the same code
         const int h = c & (CV / 2 - 1);
         const int prow = (h & 7) + 8 * (h / (8 * PC)), piece = (h >> 3) % PC;   // first row and piece of this thread
@@ -602,18 +701,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
         uint4 xa[NP], xb[NP];
         int32_t te = -1, te_next = -1;
         auto entry = [&](int j) {
-            if (j >= n || c >= TK) return -1;
-            const int t = rg.t0(j) + c;
+            if (j >= n || !is_v) return -1;
+            const int t = rg.t0(j) + h;
             return t < q.L ? __ldg(table + (t >> a.c.lp)) : -1;
         };
         float mk = 0.0f, mv = 0.0f;
         int mp = 0, md = -1;
         auto rows_of = [&](int j, int32_t e) {   // row numbers of tile j; its scales into registers
-            if (c >= TK) return;
-            const int t = rg.t0(j) + c;
+            if (!is_v) return;   // (V's threads: what they wait for covers the last use of a buffer of scales)
+            const int t = rg.t0(j) + h;
             const bool have = t < q.L && a.c.ok(e);
             const uint32_t rid = have ? a.c.row(e, kvh, t) : 0xFFFFFFFFu;
-            sm.row[j & 1][c] = rid;
+            sm.row[j & 1][h] = rid;
             const float none = t < q.L ? nan : 1.0f;   // a bad page: NaN for whoever sees it
             mk = have ? __ldg(a.c.ks + (rid >> a.c.lb)) : none;
             mv = have ? __ldg(a.c.vs + (rid >> a.c.lb)) : none;
@@ -624,16 +723,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             }
         };
         auto put_meta = [&](int j) {
-            if (c >= TK) return;
+            if (!is_v) return;
             const int mb = j & (META - 1);
-            sm.ks[mb][c] = mk;
-            sm.vs[mb][c] = mv;
-            sm.lv[mb][c] = fmaxf(__log2f(mv), -60.0f);
-            sm.rv[mb][c] = __fdividef(1.0f, mv);
+            sm.ks[mb][h] = mk;
+            sm.vs[mb][h] = mv;
+            sm.lv[mb][h] = fmaxf(F32 ? log2f(mv) : __log2f(mv), -60.0f);
+            sm.rv[mb][h] = F32 ? __frcp_rn(mv) : __fdividef(1.0f, mv);
             const bool tame = __all_sync(0xFFFFFFFFu, mv > 0x1p-60f && mv < 0x1p60f);
-            if (lane == 0) sm.tame[mb][warp - 16] = tame;
-            sm.pos[mb][c] = mp;
-            sm.doc[mb][c] = md;
+            if (lane == 0) sm.tame[mb][warp - SW - 4] = tame;
+            sm.pos[mb][h] = mp;
+            sm.doc[mb][h] = md;
             mbar_arrive(&sm.meta_full[mb]);
         };
         auto load = [&](int j, int i0, uint4 (&x)[NP]) {   // pieces i0 .. i0 + NP - 1 of the thread
@@ -685,8 +784,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
         }
     } else {
         // ---- MMAs ----
-        regs_down<REGS_MMA>();
-        if (warp == 24) {
+        regs_down<RL::REGS_MMA>();
+        if (warp == SW + 8) {
             constexpr uint32_t id_qk = idesc(TK, false), id_pv = idesc(HD, true);
             const uint32_t lead = lane == 0, tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
             const int nt = __shfl_sync(0xFFFFFFFFu, n, 0), nw = __shfl_sync(0xFFFFFFFFu, two ? 2 : 1, 0);
@@ -696,15 +795,28 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
             constexpr int BUF = TK * HD * 2 / 16;   // from a first buffer to its second
             auto qk = [&](int w, int j) {
                 const uint64_t qa = dq + w * BUF, ka = dk + (j & 1) * BUF;
+                const int sb = F32 ? j & 1 : w;
 #pragma unroll
-                for (int k = 0; k < HD / 16; k++) umma_ss(tm + w * TK, qa + 16 * k, ka + 16 * k, id_qk, k > 0, lead);
-                umma_commit(&sm.s_full[w], lead);
+                for (int k = 0; k < HD / 16; k++) umma_ss(tm + sb * TK, qa + 16 * k, ka + 16 * k, id_qk, k > 0, lead);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int k = 0; k < HD / 16; k++) umma_ss(tm + sb * TK, qa + BUF + 16 * k, ka + 16 * k, id_qk, 1, lead);
+                }
+                umma_commit(&sm.s_full[sb], lead);
             };
             auto pv = [&](int w, int j) {
                 const uint64_t va = dv + (j & 1) * BUF;
+                if constexpr (F32) {
 #pragma unroll
-                for (int k = 0; k < TK / 16; k++)
-                    umma_ts(tm + 2 * TK + w * HD, tm + w * TK + 8 * k + (k >= HC / 16 ? HC / 2 : 0), va + 2 * SBO / 16 * k, id_pv, j > 0 || k > 0, lead);
+                    for (int part = 0; part < 2; part++)
+#pragma unroll
+                        for (int k = 0; k < TK / 16; k++)
+                            umma_ts(tm + 2 * TK + part * HD, tm + (j & 1) * TK + 16 * k + 8 * part, va + 2 * SBO / 16 * k, id_pv, k > 0, lead);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < TK / 16; k++)
+                        umma_ts(tm + 2 * TK + w * HD, tm + w * TK + 8 * k + (k >= HC / 16 ? HC / 2 : 0), va + 2 * SBO / 16 * k, id_pv, j > 0 || k > 0, lead);
+                }
             };
             bool ok = nt == 0 || (mbar_wait(&sm.q_full, 0, &sm.abort) && mbar_wait(&sm.k_full[0], 0, &sm.abort));
             if (ok && nt > 0) {
@@ -712,8 +824,26 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
                 for (int w = 0; w < nw; w++) qk(w, 0);
                 umma_commit(&sm.k_empty[0], lead);
             }
+            if constexpr (F32) {
 #pragma unroll 1
-            for (int j = 0; ok && j < nt; j++) {
+                for (int j = 0; ok && j < nt; j++) {
+                    if (j + 1 < nt) {
+                        ok = mbar_wait(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, &sm.abort);
+                        if (!ok) break;
+                        tc_after();
+                        qk(0, j + 1);
+                        umma_commit(&sm.k_empty[(j + 1) & 1], lead);
+                    }
+                    ok = mbar_wait(&sm.p_full[0], j & 1, &sm.abort) && mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, &sm.abort);
+                    if (!ok) break;
+                    tc_after();
+                    pv(0, j);
+                    umma_commit(&sm.o_full[0], lead);
+                    umma_commit(&sm.v_empty[j & 1], lead);
+                }
+            }
+#pragma unroll 1
+            for (int j = 0; !F32 && ok && j < nt; j++) {
 #pragma unroll 1
                 for (int w = 0; ok && w < nw; w++) {
                     ok = mbar_wait(&sm.p_full[w], j & 1, &sm.abort) && mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, &sm.abort);
@@ -741,7 +871,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv8_prefill(const __grid_constan
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == 24) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == SW + 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 bool smem_opt_in(const void *fn, size_t bytes) {
@@ -763,8 +893,10 @@ template <int HD, int FMT, typename QT, bool SHAPED> int launch_shape(const Kv8A
     constexpr size_t bytes = sizeof(Smem<HD>);
     static_assert(bytes <= 227 * 1024, "shared memory");
     if (!smem_opt_in((const void *)fn, bytes)) return set_error(TLMG_EIO, "kv8_attend: shared memory opt-in failed");
-    const int64_t tiles = ((int64_t)a.b.max_q * a.G + 2 * TQ - 1) / (2 * TQ);
-    fn<<<dim3((unsigned)(tiles * a.c.KV), a.b.n_seq), THREADS, bytes, st>>>(a);
+    using RL = Role<sizeof(QT) == 4>;
+    constexpr int rows = RL::TILES * TQ;
+    const int64_t tiles = ((int64_t)a.b.max_q * a.G + rows - 1) / rows;
+    fn<<<dim3((unsigned)(tiles * a.c.KV), a.b.n_seq), RL::THREADS, bytes, st>>>(a);
     count_launch();
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? TLMG_OK : cuda_fail(e, "kv8_attend launch");
@@ -773,6 +905,7 @@ template <int HD, int FMT, typename QT> int launch(const Kv8Attn &a, cudaStream_
     return a.softcap > 0.0f || a.slopes || a.doc || a.c.pos ? launch_shape<HD, FMT, QT, true>(a, st) : launch_shape<HD, FMT, QT, false>(a, st);
 }
 template <int HD, int FMT> int launch_q(const Kv8Attn &a, int q_dt, cudaStream_t st) {
+    if (q_dt == TLMG_DT_F32) return launch<HD, FMT, float>(a, st);
     return q_dt == TLMG_DT_F16 ? launch<HD, FMT, __half>(a, st) : launch<HD, FMT, __nv_bfloat16>(a, st);
 }
 template <int HD> int launch_fmt(const Kv8Attn &a, int fmt, int q_dt, cudaStream_t st) {
@@ -782,7 +915,8 @@ template <int HD> int launch_fmt(const Kv8Attn &a, int fmt, int q_dt, cudaStream
 }  // namespace
 
 bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt) {
-    return q_dt != TLMG_DT_F32 && c.hd <= 128 && (int64_t)b.max_q * (H / c.KV) >= TQ;
+    (void)q_dt;
+    return c.hd <= 128 && (int64_t)b.max_q * (H / c.KV) >= TQ;
 }
 
 int kv8_prefill(const Kv8Attn &a, int fmt, int q_dt, cudaStream_t st) {
