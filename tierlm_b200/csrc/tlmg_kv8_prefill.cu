@@ -64,6 +64,7 @@ template <bool F32> struct Role {
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int META = 4;           // buffers of per-key scales
+constexpr int LIST = 2048;        // key tiles (262,144 rows) up to which tiles of other documents are left out
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ uint32_t saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -79,7 +80,8 @@ template <int HD> struct Smem {
     float qs[2][TQ], part[2][2][TQ], sums[2][2][TQ];     // [tile][half][row]: the halves' maxima; in the end their sums
     uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], x_full[2], o_full[2], meta_full[META], drain;
     uint32_t tmem;
-    int abort, pmin, pmax;
+    int abort, pmin, pmax, dmin, dmax, n_list;
+    uint16_t list[LIST];      // the key tiles that hold a key of the queries' documents
 };
 
 __device__ __forceinline__ void mbar_init(uint64_t *b, uint32_t n) {
@@ -282,6 +284,8 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
         sm.abort = 0;
         sm.pmin = INT32_MAX;
         sm.pmax = INT32_MIN;
+        sm.dmin = INT32_MAX;
+        sm.dmax = INT32_MIN;
         mbar_init(&sm.q_full, two ? 4 * TQ : 2 * TQ);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sm.k_full[i], CV / 2);
@@ -308,13 +312,52 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
         const int p = a.b.q_pos ? a.b.q_pos[q.q0 + i] : q.L - q.n + i;
         atomicMin(&sm.pmin, p);
         atomicMax(&sm.pmax, p);
+        if constexpr (SHAPED)
+            if (a.doc) {
+                const int d = p >= 0 && p < a.doc_stride ? a.doc[(size_t)s * a.doc_stride + p] : -1;
+                atomicMin(&sm.dmin, d);
+                atomicMax(&sm.dmax, d);
+            }
     }
     __syncthreads();
     const int pmin = sm.pmin, pmax = sm.pmax;
     const Kv8Range<TK> rg = kv8_range<TK>(a, q, s, pmin, pmax);
     const uint32_t tmem = sm.tmem;
     const int32_t *docs = a.doc ? a.doc + (size_t)s * a.doc_stride : nullptr;
-    const int n = rg.n;
+    int n = rg.n;
+    bool listed = false;
+    if constexpr (SHAPED) {
+        listed = docs && !a.c.pos && n <= LIST;
+        if (listed) {
+            // a tile takes part if one of its keys' documents lies between the queries' smallest and largest
+            const int lo = sm.dmin, hi = sm.dmax;
+            for (int v = warp; v < n; v += THREADS / 32) {
+                bool any = false;
+                for (int t = rg.t0(v) + lane; t < rg.t0(v) + TK && t < q.L; t += 32) {
+                    const int d = t < a.doc_stride ? docs[t] : -1;
+                    any = any || (d >= lo && d <= hi);
+                }
+                any = __any_sync(0xFFFFFFFFu, any);
+                if (lane == 0) sm.list[v] = any;
+            }
+            __syncthreads();
+            if (warp == 0) {   // the flags become the tiles' numbers, in place and in order
+                int at = 0;
+                for (int v0 = 0; v0 < n; v0 += 32) {
+                    const bool in = v0 + lane < n && sm.list[v0 + lane];
+                    const uint32_t b = __ballot_sync(0xFFFFFFFFu, in);
+                    __syncwarp();
+                    if (in) sm.list[at + __popc(b & ((1u << lane) - 1u))] = (uint16_t)(v0 + lane);
+                    __syncwarp();
+                    at += __popc(b);
+                }
+                if (lane == 0) sm.n_list = at;
+            }
+            __syncthreads();
+            n = sm.n_list;
+        }
+    }
+    auto tile_at = [&](int j) { return rg.t0(SHAPED && listed ? (int)sm.list[j] : j); };
 
     if (warp < SW) {
         // ---- softmax of one query tile ----
@@ -407,7 +450,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
             }
 #pragma unroll 1
             for (int j = 0; ok && j < n; j++) {
-                const int t0 = rg.t0(j), mb = j & (META - 1);
+                const int t0 = tile_at(j), mb = j & (META - 1);
                 const int sb = F32 ? j & 1 : w;                     // buffer of S
                 const uint32_t ts = tmem + lanes + sb * TK;
                 ok = mbar_wait_warp(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait_warp(&sm.s_full[sb], F32 ? (j >> 1) & 1 : j & 1, &sm.abort);
@@ -702,14 +745,14 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
         int32_t te = -1, te_next = -1;
         auto entry = [&](int j) {
             if (j >= n || !is_v) return -1;
-            const int t = rg.t0(j) + h;
+            const int t = tile_at(j) + h;
             return t < q.L ? __ldg(table + (t >> a.c.lp)) : -1;
         };
         float mk = 0.0f, mv = 0.0f;
         int mp = 0, md = -1;
         auto rows_of = [&](int j, int32_t e) {   // row numbers of tile j; its scales into registers
             if (!is_v) return;   // (V's threads: what they wait for covers the last use of a buffer of scales)
-            const int t = rg.t0(j) + h;
+            const int t = tile_at(j) + h;
             const bool have = t < q.L && a.c.ok(e);
             const uint32_t rid = have ? a.c.row(e, kvh, t) : 0xFFFFFFFFu;
             sm.row[j & 1][h] = rid;
