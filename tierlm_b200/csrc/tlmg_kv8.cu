@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_append(const Kv8View c, c
     const XT *x = (is_v ? xv : xk) + (q.q0 + (int64_t)(ta - t_new)) * x_stride + (int64_t)kv * c.hd;
     const int per = c.hd >> 2, lper = 31 - __clz(per), n4 = (t1 - ta) << lper;
     float a = 0.0f;
+#pragma unroll 8
     for (int i = lane; i < n4; i += 32) a = amax4(a, kv8_ld4(x + (int64_t)(i >> lper) * x_stride + 4 * (i & (per - 1))));
     float d = scale_of<FMT>(warp_max(a));
     float old = 0.0f;
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_append(const Kv8View c, c
     }
     if (lane == 0) *scale = d;
     uint32_t *w = reinterpret_cast<uint32_t *>(codes + (size_t)(ta - t0) * c.hd);
+#pragma unroll 4
     for (int i = lane; i < n4; i += 32)
         w[i] = codes4<FMT>(kv8_ld4(x + (int64_t)(i >> lper) * x_stride + 4 * (i & (per - 1))), d, inv);
     if (c.pos && !is_v)
@@ -190,7 +192,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 constexpr int SEL_THREADS = 1024;
 constexpr int SEL_BINS = 2048;
 constexpr int SEL_CLUSTER = 8;
-constexpr int SEL_ALONE = 8192;   // rows up to which one CTA is as fast as a cluster
+constexpr int SEL_KEEP = 4;       // keys a thread holds
+constexpr int SEL_ALONE = 4096;   // rows up to which one CTA is as fast as a cluster
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -241,31 +244,24 @@ __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_
     // this CTA's part of the rows between, a multiple of the warp
     const int mid = L - recent - sink, part = ((mid + CS - 1) / CS + 31) / 32 * 32;
     const int lo = sink + min(mid, (int)rank * part), hi = sink + min(mid, ((int)rank + 1) * part);
+    uint32_t key[SEL_KEEP];                    // the part's first keys stay in registers
+#pragma unroll
+    for (int u = 0; u < SEL_KEEP; u++) {
+        const int t = lo + u * SEL_THREADS + tid;
+        key[u] = t < hi ? weight_key(w[t]) : 0u;
+    }
     uint32_t prefix = 0, left = (uint32_t)m;   // key bits found so far; rows still to take below them
     for (int pass = 0; pass < 3; pass++) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
         uint32_t *h = hist[pass & 1];          // the other one may still be read by the cluster
         for (int i = tid; i < bins; i += SEL_THREADS) h[i] = 0;
         __syncthreads();
-        for (int t0 = lo; t0 < hi; t0 += 4 * SEL_THREADS) {
-            uint32_t key[4];
+        auto count = [&](uint32_t key, bool in) {
+            if (in && (pass == 0 || (key >> (shift + (pass == 2 ? 10 : 11))) == prefix)) atomicAdd(&h[(key >> shift) & (uint32_t)(bins - 1)], 1u);
+        };
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int t = t0 + u * SEL_THREADS + tid;
-                key[u] = t < hi ? weight_key(w[t]) : 0u;
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const bool in = t0 + u * SEL_THREADS + tid < hi && (pass == 0 || (key[u] >> (shift + (pass == 2 ? 10 : 11))) == prefix);
-                const uint32_t bin = (key[u] >> shift) & (uint32_t)(bins - 1);
-                // equal digits of a warp are counted once: accumulated weights hold many equal values
-                const uint32_t act = __ballot_sync(0xFFFFFFFFu, in);
-                if (in) {
-                    const uint32_t peers = __match_any_sync(act, bin);
-                    if (lane == __ffs(peers) - 1) atomicAdd(&h[bin], (uint32_t)__popc(peers));
-                }
-            }
-        }
+        for (int u = 0; u < SEL_KEEP; u++) count(key[u], lo + u * SEL_THREADS + tid < hi);
+        for (int t = lo + SEL_KEEP * SEL_THREADS + tid; t < hi; t += SEL_THREADS) count(weight_key(w[t]), true);
         sync_all<CS>();
         // counts from the top: thread i covers the bins / 1024 bins there
         const int per = bins / SEL_THREADS, b0 = bins - 1 - per * tid;
@@ -299,10 +295,16 @@ __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_
     uint32_t n_out = 0, n_eq = 0;
     if constexpr (CS > 1) {   // rows larger and equal in the parts before this one
         uint32_t g = 0, e = 0;
-        for (int t = lo + tid; t < hi; t += SEL_THREADS) {
-            const uint32_t key = weight_key(w[t]);
-            g += key > prefix;
-            e += key == prefix;
+#pragma unroll
+        for (int u = 0; u < SEL_KEEP; u++) {
+            const bool in = lo + u * SEL_THREADS + tid < hi;
+            g += in && key[u] > prefix;
+            e += in && key[u] == prefix;
+        }
+        for (int t = lo + SEL_KEEP * SEL_THREADS + tid; t < hi; t += SEL_THREADS) {
+            const uint32_t k = weight_key(w[t]);
+            g += k > prefix;
+            e += k == prefix;
         }
         g = __reduce_add_sync(0xFFFFFFFFu, g);
         e = __reduce_add_sync(0xFFFFFFFFu, e);
@@ -322,8 +324,8 @@ __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_
     }
     for (int t0 = lo; t0 < hi; t0 += SEL_THREADS) {
         const int t = t0 + tid;
-        const uint32_t key = t < hi ? weight_key(w[t]) : 0u;
-        const bool gt = t < hi && key > prefix, eq = t < hi && key == prefix;
+        const uint32_t k = t < hi ? weight_key(w[t]) : 0u;
+        const bool gt = t < hi && k > prefix, eq = t < hi && k == prefix;
         const uint32_t bg = __ballot_sync(0xFFFFFFFFu, gt), be = __ballot_sync(0xFFFFFFFFu, eq);
         if (lane == 0) {
             wsum[0][warp] = __popc(bg);
@@ -392,20 +394,50 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_compact(const Kv8View c, 
     };
     float a = 0.0f;
     bool any = false;
-    rounds([&](int, uint4 w, float v) {
+    auto top = [&](uint4 w, float v) {
         any = true;
         a = amax4(amax4(amax4(amax4(a, values4<FS>(w.x, v)), values4<FS>(w.y, v)), values4<FS>(w.z, v)), values4<FS>(w.w, v));
-    });
-    any = __any_sync(0xFFFFFFFFu, any);
-    const float q = scale_of<FD>(warp_max(a)), inv = __frcp_rn(q);
-    if (dok && any) {
-        if (lane == 0) (is_v ? d.vs : d.ks)[dr >> d.lb] = q;
-        uint8_t *to = (is_v ? d.v : d.k) + (size_t)dr * d.hd + at;
-        rounds([&](int j, uint4 w, float v) {
-            *reinterpret_cast<uint4 *>(to + (size_t)j * d.hd) =
-                make_uint4(codes4<FD>(values4<FS>(w.x, v), q, inv), codes4<FD>(values4<FS>(w.y, v), q, inv),
-                           codes4<FD>(values4<FS>(w.z, v), q, inv), codes4<FD>(values4<FS>(w.w, v), q, inv));
-        });
+    };
+    uint8_t *to = (is_v ? d.v : d.k) + (size_t)dr * d.hd + at;
+    float q = 0.0f, inv = 0.0f;
+    auto put = [&](int j, uint4 w, float v) {
+        *reinterpret_cast<uint4 *>(to + (size_t)j * d.hd) =
+            make_uint4(codes4<FD>(values4<FS>(w.x, v), q, inv), codes4<FD>(values4<FS>(w.y, v), q, inv),
+                       codes4<FD>(values4<FS>(w.z, v), q, inv), codes4<FD>(values4<FS>(w.w, v), q, inv));
+    };
+    auto scale = [&] {
+        any = __any_sync(0xFFFFFFFFu, any);
+        q = scale_of<FD>(warp_max(a));
+        inv = __frcp_rn(q);
+        any = any && dok;
+        if (any && lane == 0) (is_v ? d.vs : d.ks)[dr >> d.lb] = q;
+    };
+    if (nj <= 8 * rpi) {   // the block's codes fit the warp's registers: all its loads at once, and once
+        uint32_t r = 0;
+        const bool ok = source(lane, r);
+        const float v = ok ? sc[r >> c.lb] : 0.0f;
+        uint4 w[8];
+        float vv[8];
+        bool have[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int j = i * rpi + sub;
+            const uint32_t rr = __shfl_sync(0xFFFFFFFFu, r, j & 31);
+            vv[i] = __shfl_sync(0xFFFFFFFFu, v, j & 31);
+            have[i] = __shfl_sync(0xFFFFFFFFu, (int)ok, j & 31) && j < nj;
+            if (have[i]) w[i] = *reinterpret_cast<const uint4 *>(pool + (size_t)rr * c.hd + at);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (have[i]) top(w[i], vv[i]);
+        scale();
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (have[i] && any) put(i * rpi + sub, w[i], vv[i]);
+    } else {
+        rounds([&](int, uint4 w, float v) { top(w, v); });
+        scale();
+        if (any) rounds(put);
     }
     if (!is_v)
         for (int j = lane; j < nj; j += 32) {

@@ -122,11 +122,18 @@ __device__ __forceinline__ Kv8Range<TILE> key_range(const Kv8Attn &a, const Kv8S
     return kv8_range<TILE>(a, q, s, pmin, pmax);
 }
 
+// CTAs of an SM, by registers: two f32 row tiles take 255; 16-bit queries over e4m3 rows spill at the 168 of three CTAs
+// (64 ragged sequences: 121 us with three, 101 with two; int8 rows 99 and 106).
+constexpr int split_ctas(int hd, bool f32, int rm, int fmt) {
+    return hd > 128 ? 1 : f32 ? (rm == 2 ? 2 : 3) : fmt == TLMG_KV8_E4M3 && hd == 128 ? 2 : 3;
+}
+
 template <int HD, int FMT, typename QT, int RM>
-__global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const __grid_constant__ Kv8Attn a) {
+__global__ void __launch_bounds__(32 * NW, split_ctas(HD, sizeof(QT) == 4, RM, FMT)) k_kv8_split(const __grid_constant__ Kv8Attn a) {
     constexpr bool F32 = sizeof(QT) == 4;
     constexpr int ROWS = 8 * RM;                             // query rows of the CTA (RM of a thread)
     constexpr int QR = F32 || RM == 2 ? 4 : 2;               // registers of a query fragment: rows 8 .. 15 may be zeros
+    constexpr int MT = F32 ? RM : 1;                         // MMA row tiles (8 f32 rows or 16 others)
     constexpr int NT = HD / 8, KC = HD / 64, NST = Plan<HD>::NST;
     using P = Plan<HD>;
     extern __shared__ __align__(16) uint8_t sm[];
@@ -243,7 +250,7 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
     load_te(NST - 1);
 
     // this thread's query rows: f16 fragments, the power of two taken out, masks
-    uint32_t qa[4 * KC][QR];
+    uint32_t qa[MT][4 * KC][QR];
     float qs[RM], slope[RM];
     int qp[RM], qd[RM];
     {
@@ -269,7 +276,7 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
             // the row's largest element to 2^9 .. 2^10
             const int e = min(max(exp_above(m) - 10, -100), 100);
             up[r] = live ? pow2i(-e) : 0.0f;
-            qs[r] = pow2i(e) * a.scale * kv8_f16_unit<FMT>() * (a.softcap > 0.0f ? a.inv_cap : LOG2E);
+            qs[r] = pow2i(e) * a.scale * kv8_cvt_unit<FMT>() * (a.softcap > 0.0f ? a.inv_cap : LOG2E);
         }
 #pragma unroll
         for (int c = 0; c < 4 * KC; c++) {
@@ -281,16 +288,19 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
                 x[r][c].w *= up[r];
             }
             if constexpr (F32) {
-                split_f16(x[0][c].x, x[0][c].y, qa[c][0], qa[c][1]);
-                split_f16(x[0][c].z, x[0][c].w, qa[c][2], qa[c][3]);
+#pragma unroll
+                for (int r = 0; r < RM; r++) {
+                    split_f16(x[r][c].x, x[r][c].y, qa[r][c][0], qa[r][c][1]);
+                    split_f16(x[r][c].z, x[r][c].w, qa[r][c][2], qa[r][c][3]);
+                }
             } else if constexpr (RM == 2) {
-                qa[c][0] = pack_f16(x[0][c].x, x[0][c].y);
-                qa[c][1] = pack_f16(x[1][c].x, x[1][c].y);
-                qa[c][2] = pack_f16(x[0][c].z, x[0][c].w);
-                qa[c][3] = pack_f16(x[1][c].z, x[1][c].w);
+                qa[0][c][0] = pack_f16(x[0][c].x, x[0][c].y);
+                qa[0][c][1] = pack_f16(x[1][c].x, x[1][c].y);
+                qa[0][c][2] = pack_f16(x[0][c].z, x[0][c].w);
+                qa[0][c][3] = pack_f16(x[1][c].z, x[1][c].w);
             } else {
-                qa[c][0] = pack_f16(x[0][c].x, x[0][c].y);
-                qa[c][1] = pack_f16(x[0][c].z, x[0][c].w);
+                qa[0][c][0] = pack_f16(x[0][c].x, x[0][c].y);
+                qa[0][c][1] = pack_f16(x[0][c].z, x[0][c].w);
             }
         }
     }
@@ -315,7 +325,7 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
         __syncwarp();
         const uint8_t *st = ring + (i % NST) * P::STAGE;
         const int t0 = rg.t0(v0 + warp + NW * i);
-        float sc[4][4];
+        float sc[MT][4][4];
 #pragma unroll
         for (int c = 0; c < KC; c++)
 #pragma unroll
@@ -324,9 +334,12 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
                 const uint32_t x[4] = { kv8_bias<FMT>(w.x), kv8_bias<FMT>(w.y), kv8_bias<FMT>(w.z), kv8_bias<FMT>(w.w) };
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t b0 = kv8_half2<FMT, 0>(x[j]), b1 = kv8_half2<FMT, 1>(x[j]);
-                    if (c == 0 && j == 0) mma_f16_0(sc[nt], qa[0], b0, b1);
-                    else mma_f16(sc[nt], qa[4 * c + j], b0, b1);
+                    const uint32_t b0 = kv8_cvt2<FMT, 0, false>(x[j]), b1 = kv8_cvt2<FMT, 1, false>(x[j]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        if (c == 0 && j == 0) mma_f16_0(sc[mt][nt], qa[mt][0], b0, b1);
+                        else mma_f16(sc[mt][nt], qa[mt][4 * c + j], b0, b1);
+                    }
                 }
             }
         // scores in log2 units (with a cap: over it, until the tanh), masked ones -inf
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
             for (int r = 0; r < RM; r++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const float dot = F32 ? __fmaf_rn(sc[nt][2 + u], LO, sc[nt][u]) : sc[nt][2 * r + u];
+                    const float dot = F32 ? __fmaf_rn(sc[F32 ? r : 0][nt][2 + u], LO, sc[F32 ? r : 0][nt][u]) : sc[0][nt][F32 ? 0 : 2 * r + u];
                     z[r][2 * nt + u] = dot * ((u ? ks2.y : ks2.x) * qs[r]);
                 }
         }
@@ -401,7 +414,7 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
             }
         }
         float alpha[RM], back[RM];
-        uint32_t pa[2][QR];
+        uint32_t pa[MT][2][QR];
 #pragma unroll
         for (int r = 0; r < RM; r++) {
             float m = fmaxf(fmaxf(fmaxf(z[r][0], z[r][1]), fmaxf(z[r][2], z[r][3])), fmaxf(fmaxf(z[r][4], z[r][5]), fmaxf(z[r][6], z[r][7])));
@@ -426,23 +439,26 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
             const int e = exp_above(top);
             // p vs 2^(15 - e) < 2^15
             const float up = pow2i(min(15 - e, 100));
-            back[r] = pow2i(max(e - 15, -100)) * kv8_f16_unit<FMT>();
+            back[r] = pow2i(max(e - 15, -100)) * kv8_cvt_unit<FMT>();
 #pragma unroll
             for (int j = 0; j < 8; j++) z[r][j] *= up;
         }
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
             if constexpr (F32) {
-                split_f16(z[0][4 * kk], z[0][4 * kk + 1], pa[kk][0], pa[kk][1]);
-                split_f16(z[0][4 * kk + 2], z[0][4 * kk + 3], pa[kk][2], pa[kk][3]);
+#pragma unroll
+                for (int r = 0; r < RM; r++) {
+                    split_f16(z[r][4 * kk], z[r][4 * kk + 1], pa[r][kk][0], pa[r][kk][1]);
+                    split_f16(z[r][4 * kk + 2], z[r][4 * kk + 3], pa[r][kk][2], pa[r][kk][3]);
+                }
             } else if constexpr (RM == 2) {
-                pa[kk][0] = pack_f16(z[0][4 * kk], z[0][4 * kk + 1]);
-                pa[kk][1] = pack_f16(z[RM - 1][4 * kk], z[RM - 1][4 * kk + 1]);
-                pa[kk][2] = pack_f16(z[0][4 * kk + 2], z[0][4 * kk + 3]);
-                pa[kk][3] = pack_f16(z[RM - 1][4 * kk + 2], z[RM - 1][4 * kk + 3]);
+                pa[0][kk][0] = pack_f16(z[0][4 * kk], z[0][4 * kk + 1]);
+                pa[0][kk][1] = pack_f16(z[RM - 1][4 * kk], z[RM - 1][4 * kk + 1]);
+                pa[0][kk][2] = pack_f16(z[0][4 * kk + 2], z[0][4 * kk + 3]);
+                pa[0][kk][3] = pack_f16(z[RM - 1][4 * kk + 2], z[RM - 1][4 * kk + 3]);
             } else {
-                pa[kk][0] = pack_f16(z[0][4 * kk], z[0][4 * kk + 1]);
-                pa[kk][1] = pack_f16(z[0][4 * kk + 2], z[0][4 * kk + 3]);
+                pa[0][kk][0] = pack_f16(z[0][4 * kk], z[0][4 * kk + 1]);
+                pa[0][kk][1] = pack_f16(z[0][4 * kk + 2], z[0][4 * kk + 3]);
             }
         }
         bool same = alpha[0] == 1.0f;
@@ -453,6 +469,7 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
 #pragma unroll
                 for (int r = 0; r < 2 * RM; r++) o[j][r] *= alpha[r >> 1];
         }
+        asm volatile("" ::: "memory");   // V's words are not fetched before here: their registers are the probabilities'
         const uint8_t *vt = st + TILE * HD;
 #pragma unroll
         for (int c = 0; c < P::VP; c++) {
@@ -484,22 +501,28 @@ __global__ void __launch_bounds__(32 * NW, HD <= 128 ? 3 : 1) k_kv8_split(const 
                 }
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    float acc[4];
+                    float acc[MT][4];
 #pragma unroll
                     for (int kk = 0; kk < 2; kk++) {
                         const uint32_t *u = y < 2 ? ev : od;
-                        const uint32_t b0 = (y & 1) ? kv8_half2<FMT, 1>(u[2 * kk]) : kv8_half2<FMT, 0>(u[2 * kk]);
-                        const uint32_t b1 = (y & 1) ? kv8_half2<FMT, 1>(u[2 * kk + 1]) : kv8_half2<FMT, 0>(u[2 * kk + 1]);
-                        if (kk == 0) mma_f16_0(acc, pa[kk], b0, b1);
-                        else mma_f16(acc, pa[kk], b0, b1);
+                        const uint32_t b0 = (y & 1) ? kv8_cvt2<FMT, 1, true>(u[2 * kk]) : kv8_cvt2<FMT, 0, true>(u[2 * kk]);
+                        const uint32_t b1 = (y & 1) ? kv8_cvt2<FMT, 1, true>(u[2 * kk + 1]) : kv8_cvt2<FMT, 0, true>(u[2 * kk + 1]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            if (kk == 0) mma_f16_0(acc[mt], pa[mt][kk], b0, b1);
+                            else mma_f16(acc[mt], pa[mt][kk], b0, b1);
+                        }
                     }
                     float (&oj)[2 * RM] = o[16 * c + 4 * x + y];
                     if constexpr (F32) {
-                        oj[0] = __fmaf_rn(__fmaf_rn(acc[2], LO, acc[0]), back[0], oj[0]);
-                        oj[1] = __fmaf_rn(__fmaf_rn(acc[3], LO, acc[1]), back[0], oj[1]);
+#pragma unroll
+                        for (int r = 0; r < RM; r++) {
+                            oj[2 * r] = __fmaf_rn(__fmaf_rn(acc[r][2], LO, acc[r][0]), back[r], oj[2 * r]);
+                            oj[2 * r + 1] = __fmaf_rn(__fmaf_rn(acc[r][3], LO, acc[r][1]), back[r], oj[2 * r + 1]);
+                        }
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 2 * RM; r++) oj[r] = __fmaf_rn(acc[r], back[r >> 1], oj[r]);
+                        for (int r = 0; r < 2 * RM; r++) oj[r] = __fmaf_rn(acc[0][r], back[r >> 1], oj[r]);
                     }
                 }
             }
@@ -702,8 +725,8 @@ Split split_plan(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_scor
     const int G = H / c.KV;
     p.wide = !weights && kv8_prefill_serves(c, b, H, q_dt);
     if (p.wide) return p;
-    // 16 query rows a CTA only where there are more than 8 (and 16-bit queries, whose fragments leave the room)
-    p.rm = q_dt != TLMG_DT_F32 && (int64_t)b.max_q * G > 8 ? 2 : 1;
+    // 16 query rows a CTA where there are more than 8 (not for f32 ones of 256 dims: no registers)
+    p.rm = (int64_t)b.max_q * G > 8 && (q_dt != TLMG_DT_F32 || c.hd <= 128) ? 2 : 1;
     const int rows = 8 * p.rm;
     p.rtiles = ((int64_t)b.max_q * G + rows - 1) / rows;
     // rows that a query tile can see at most (the prefix is only known to the device)
@@ -711,7 +734,7 @@ Split split_plan(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_scor
     if (s.window > 0 && s.causal && !c.pos && !s.prefix && !b.q_pos)
         vis = std::min<int64_t>(vis, (int64_t)s.window + (rows + G - 1) / G + TILE);
     // Spans: one round of the CTAs that the SMs hold for one sequence; four for a batch, whose lengths differ.
-    const int64_t slots = (int64_t)sm_count() * (c.hd <= 128 ? 3 : 1) * (b.n_seq > 1 ? 4 : 1);
+    const int64_t slots = (int64_t)sm_count() * split_ctas(c.hd, q_dt == TLMG_DT_F32, p.rm, c.fmt) * (b.n_seq > 1 ? 4 : 1);
     const int64_t tiles = std::max<int64_t>(1, (vis + TILE - 1) / TILE), base = p.rtiles * c.KV * b.n_seq;
     const int64_t want = std::max<int64_t>(1, slots / base);
     p.tiles = (int)std::max<int64_t>(NW, (tiles + want - 1) / want);
@@ -759,7 +782,7 @@ int launch_split_rows(const Kv8Attn &a, const Split &p, cudaStream_t st) {
     return e == cudaSuccess ? TLMG_OK : cuda_fail(e, "kv8_attend launch");
 }
 template <int HD, int FMT, typename QT> int launch_split(const Kv8Attn &a, const Split &p, cudaStream_t st) {
-    if constexpr (sizeof(QT) == 2)
+    if constexpr (sizeof(QT) == 2 || HD <= 128)
         if (p.rm == 2) return launch_split_rows<HD, FMT, QT, 2>(a, p, st);
     return launch_split_rows<HD, FMT, QT, 1>(a, p, st);
 }
