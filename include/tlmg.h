@@ -40,6 +40,9 @@ enum {
     TLMG_DT_F32 = 0, TLMG_DT_F16 = 1, TLMG_DT_BF16 = 2, TLMG_DT_Q8_0 = 8, TLMG_DT_Q4_K = 12,
     TLMG_DT_Q5_K = 13, TLMG_DT_Q6_K = 14, TLMG_DT_Q8_K = 15, TLMG_DT_MXFP4 = 39
 };
+/* kv_dt of tlmg_step_open beside F32 and BF16: the 8-bit KV cache (last
+ * section), 16 rows per scale. */
+enum { TLMG_DT_KV8_INT8 = 0x101, TLMG_DT_KV8_E4M3 = 0x102 };
 
 /* ---- library --------------------------------------------------------- */
 /* Thread-local message of the last failure (replaces tlm_errmsg,
@@ -344,7 +347,8 @@ int tlmg_ep_combine(tlmg_ctx *ctx, int n_tok, const float *back, const int32_t *
  * the RoPE inverse frequencies inv_freq[head_dim / 2] and attention scale
  * exactly as the reference's model holds them (tlm_model_open, plain or
  * YaRN-transformed), KV pages for max_ctx positions per layer (kv_dt F32
- * or BF16) and the attention mode (TLMG_ATTN_EXACT or _SPLIT). */
+ * or BF16; TLMG_DT_KV8_INT8 or _E4M3: 8-bit rows, a fourth of the f32 pages'
+ * memory, with _SPLIT) and the attention mode (TLMG_ATTN_EXACT or _SPLIT). */
 int tlmg_step_open(tlmg_ctx *ctx, int n_heads, int n_kv_heads, int head_dim, int vocab,
                    const float *inv_freq, float attn_scale, int max_ctx, int kv_dt, int attn_mode);
 /* Attention weights of one layer (host or device memory, copied):

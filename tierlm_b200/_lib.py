@@ -18,6 +18,8 @@ TLMG_ERANGE, TLMG_ENOTFOUND, TLMG_EUNSUP, TLMG_EBUSY = -5, -6, -7, -8
 
 # dtype codes (= tlm_dtype)
 F32, F16, BF16, Q8_0, Q4_K, Q5_K, Q6_K, Q8_K, MXFP4 = 0, 1, 2, 8, 12, 13, 14, 15, 39
+# kv_dt of the decoder step's 8-bit KV cache
+KV8_INT8, KV8_E4M3 = 0x101, 0x102
 DTYPE_NAMES = {F32: "f32", F16: "f16", BF16: "bf16", Q8_0: "q8_0", Q4_K: "q4_k", Q5_K: "q5_k",
                Q6_K: "q6_k", Q8_K: "q8_k", MXFP4: "mxfp4"}
 

@@ -1620,7 +1620,9 @@ int tlmg_step_open(tlmg_ctx *c, int n_heads, int n_kv_heads, int head_dim, int v
     if (c->step) return set_error(TLMG_EBUSY, "step_open: already open");
     const int H = n_heads, KV = n_kv_heads, hd = head_dim, L = c->g.n_layers;
     if (H <= 0 || KV <= 0 || H % KV || H / KV > 16 || (hd != 64 && hd != 128 && hd != 256) || vocab <= 0 ||
-        max_ctx <= 0 || max_ctx > 65536 || (kv_dt != DT_F32 && kv_dt != DT_BF16) ||
+        max_ctx <= 0 || max_ctx > 65536 ||
+        (kv_dt != DT_F32 && kv_dt != DT_BF16 &&
+         ((kv_dt != TLMG_DT_KV8_INT8 && kv_dt != TLMG_DT_KV8_E4M3) || attn_mode != TLMG_ATTN_SPLIT)) ||
         (attn_mode != TLMG_ATTN_EXACT && attn_mode != TLMG_ATTN_SPLIT))
         return set_error(TLMG_EINVAL, "step_open: heads %d/%d x %d, vocab %d, max_ctx %d, kv dtype %d, mode %d", H, KV,
                          hd, vocab, max_ctx, kv_dt, attn_mode);
@@ -1631,7 +1633,8 @@ int tlmg_step_open(tlmg_ctx *c, int n_heads, int n_kv_heads, int head_dim, int v
     m->hd = hd;
     m->vocab = vocab;
     m->max_ctx = max_ctx;
-    m->page = 1;
+    const bool is8 = kv_dt == TLMG_DT_KV8_INT8 || kv_dt == TLMG_DT_KV8_E4M3;
+    m->page = is8 ? 32 : 1;   // 8-bit pages hold the attention's tiles of 32 rows whole
     while (m->page < max_ctx) m->page <<= 1;
     m->kv_dt = kv_dt;
     m->attn_mode = attn_mode;
@@ -1639,9 +1642,22 @@ int tlmg_step_open(tlmg_ctx *c, int n_heads, int n_kv_heads, int head_dim, int v
     m->inv_freq.assign(inv_freq, inv_freq + hd / 2);
     m->A.resize(L);
     const int D = c->g.d_model, nq = (H + 2 * KV) * hd;
-    const size_t es = kv_dt == DT_F32 ? 4 : 2, pool = (size_t)L * KV * m->page * hd * es;
+    const size_t es = is8 ? 1 : kv_dt == DT_F32 ? 4 : 2, pool = (size_t)L * KV * m->page * hd * es;
+    constexpr int KV8_BLOCK = 16;
+    tlmg_kv8 kv8 = { (void *)256, (void *)256, (float *)256, (float *)256, nullptr, kv_dt & 0xFF,
+                     L, KV, m->page, KV8_BLOCK, hd };
     size_t work = 0;
-    for (int T = 1; T <= max_ctx; T++) work = std::max(work, attention_work_bytes(attn_mode, kv_dt, T, H, KV, hd));
+    if (is8) {   // (a size only: no pointer of these is followed)
+        const tlmg_kv8_batch b = { (int32_t *)256, (int32_t *)256, (int32_t *)256, nullptr, 1, 1, 1, 1, max_ctx };
+        const tlmg_kv8_score sc = { 0.0f, 0.0f, nullptr, nullptr, nullptr, 0, 1, 0 };
+        work = tlmg_kv8_attend_work_bytes(&kv8, &b, &sc, H, TLMG_DT_F32, 0);
+        if (!work) {
+            delete m;
+            return TLMG_EINVAL;   // (the call's message stands)
+        }
+    } else {
+        for (int T = 1; T <= max_ctx; T++) work = std::max(work, attention_work_bytes(attn_mode, kv_dt, T, H, KV, hd));
+    }
     m->awork_bytes = work;
     const size_t aq = std::max(tlmg_qact_bytes(DT_Q8_K, H * hd), tlmg_qact_bytes(DT_Q8_0, H * hd)) + 4 * (size_t)H * hd;
     const size_t xq = tlmg_qact_bytes(DT_Q8_K, D) + tlmg_qact_bytes(DT_Q8_0, D) + 64;
@@ -1650,7 +1666,9 @@ int tlmg_step_open(tlmg_ctx *c, int n_heads, int n_kv_heads, int head_dim, int v
         !(m->att = (float *)dalloc(c, 4 * (size_t)H * hd)) || !(m->aq = (uint8_t *)dalloc(c, aq)) ||
         !(m->xb = (float *)dalloc(c, 4 * (size_t)D)) || !(m->xq = (uint8_t *)dalloc(c, xq)) ||
         !(m->rope = (float *)dalloc(c, 4 * (size_t)max_ctx * hd)) || !(m->logits = (float *)dalloc(c, 4 * (size_t)vocab)) ||
-        !(m->dargs = (int32_t *)dalloc(c, 16))) {
+        !(m->dargs = (int32_t *)dalloc(c, 16)) ||
+        (is8 && (!(kv8.k_scale = (float *)dalloc(c, pool / hd / KV8_BLOCK * 4)) ||
+                 !(kv8.v_scale = (float *)dalloc(c, pool / hd / KV8_BLOCK * 4)) || !(m->q_start = (int32_t *)dalloc(c, 8))))) {
         delete m;
         return set_error(TLMG_ENOMEM, "step_open: KV pages and scratch (%zu bytes of pages)", 2 * pool);
     }
@@ -1671,6 +1689,18 @@ int tlmg_step_open(tlmg_ctx *c, int n_heads, int n_kv_heads, int head_dim, int v
         cudaMemset(m->kpool, 0, pool) != cudaSuccess || cudaMemset(m->vpool, 0, pool) != cudaSuccess) {
         delete m;
         return set_error(TLMG_EIO, "step_open: table upload");
+    }
+    if (is8) {
+        const int32_t start[2] = { 0, 1 };
+        if (cudaMemcpy(m->q_start, start, sizeof(start), cudaMemcpyHostToDevice) != cudaSuccess ||
+            cudaMemset(kv8.k_scale, 0, pool / hd / KV8_BLOCK * 4) != cudaSuccess ||
+            cudaMemset(kv8.v_scale, 0, pool / hd / KV8_BLOCK * 4) != cudaSuccess) {
+            delete m;
+            return set_error(TLMG_EIO, "step_open: 8-bit pages");
+        }
+        kv8.k = m->kpool;
+        kv8.v = m->vpool;
+        m->kv8 = kv8;
     }
     c->step = m;
     return TLMG_OK;
@@ -1838,10 +1868,13 @@ static int step_body(tlmg_ctx *c, int token, int pos, bool head, const int32_t *
             }
         }
         if ((rc = step_heads(m, l, pos, dargs, g.norm_eps, st))) return rc;
-        if ((rc = decode_attention_impl(m.attn_mode, m.kv_dt, m.qkv, m.kpool, m.vpool, L, m.table + l, m.page,
-                                        dargs ? m.max_ctx : pos + 1, dargs ? dargs + 2 : nullptr, H, KV, hd, m.awork,
-                                        m.awork_bytes, m.att, st)))
+        if (m.is_kv8()) {
+            if ((rc = step_attend_kv8(m, l, st))) return rc;
+        } else if ((rc = decode_attention_impl(m.attn_mode, m.kv_dt, m.qkv, m.kpool, m.vpool, L, m.table + l, m.page,
+                                               dargs ? m.max_ctx : pos + 1, dargs ? dargs + 2 : nullptr, H, KV, hd,
+                                               m.awork, m.awork_bytes, m.att, st))) {
             return rc;
+        }
         ActCache aa{ m.att, H * hd, m.aq, m.aq + aoff80 };
         if ((rc = aa.get(A.dt[3], st, &act)) ||
             (rc = launch_matvec(A.dt[3], A.w[3], A.rb[3], act, dh, H * hd, 0, D, st, dh)))   // h += o . att
@@ -1964,6 +1997,8 @@ static int decode_step(tlmg_ctx *c, int token, int pos, float *logits) {
             }
             tev = m.tev.data();
         }
+        // (8-bit pages take the row count from device memory in every step)
+        if (m.is_kv8() && (rc = step_set_args(m.dargs, token, pos, st))) return rc;
         set_pdl(true);
         rc = step_body(c, token, pos, head != 0, nullptr, tev);
         set_pdl(false);

@@ -103,7 +103,8 @@ __device__ __forceinline__ void kv_store(__nv_bfloat16 *p, float v) { *p = __flo
 // RMSNorm with the layer's q_norm / k_norm weights when present (rmsnorm in
 // place, src/lib/tlm_model.c:744-747), then rope() (:720-727): pairs (j,
 // j + hd/2), a' = a cs - b sn, b' = b cs + a sn. k-head blocks then store
-// k and v of position pos into the layer's page (pages [KV][page][hd]).
+// k and v of position pos into the layer's page (pages [KV][page][hd]; no
+// page: both stay in qkv).
 template <typename KT>
 __global__ void k_heads(float *__restrict__ qkv, int H, int KV, int hd, const float *__restrict__ q_norm,
                         const float *__restrict__ k_norm, float eps, const float *__restrict__ rope_all,
@@ -131,7 +132,7 @@ __global__ void k_heads(float *__restrict__ qkv, int H, int KV, int hd, const fl
     const float o = i < half ? __fsub_rn(__fmul_rn(v[i], cs[j]), __fmul_rn(v[i + half], sn[j]))
                              : __fadd_rn(__fmul_rn(v[i], cs[j]), __fmul_rn(v[j], sn[j]));
     x[i] = o;
-    if (!is_q) {
+    if (!is_q && kpage) {
         const int h = b - H;
         const size_t off = ((size_t)h * page + pos) * hd + i;
         kv_store(kpage + off, o);
@@ -143,7 +144,10 @@ int step_heads(const StepModel &m, int l, int pos, const int32_t *dargs, float e
     const StepLayer &A = m.A[l];
     const float *rope = m.rope;
     const size_t per = (size_t)m.KV * m.page * m.hd;   // one layer's page
-    if (m.kv_dt == DT_F32) {
+    if (m.is_kv8()) {
+        launch_k(k_heads<float>, m.H + m.KV, m.hd, 0, st, m.qkv, m.H, m.KV, m.hd, A.q_norm, A.k_norm, eps, rope,
+                 (float *)nullptr, (float *)nullptr, m.page, pos, dargs);
+    } else if (m.kv_dt == DT_F32) {
         float *kp = static_cast<float *>(m.kpool) + (size_t)l * per, *vp = static_cast<float *>(m.vpool) + (size_t)l * per;
         launch_k(k_heads<float>, m.H + m.KV, m.hd, 0, st, m.qkv, m.H, m.KV, m.hd, A.q_norm, A.k_norm, eps, rope, kp,
                  vp, m.page, pos, dargs);
@@ -156,6 +160,19 @@ int step_heads(const StepModel &m, int l, int pos, const int32_t *dargs, float e
     count_launch();
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? TLMG_OK : cuda_fail(e, "attention heads launch");
+}
+
+int step_attend_kv8(const StepModel &m, int l, cudaStream_t st) {
+    // max_kv = max_ctx in every step: eager and replayed steps split the rows, and so round, alike
+    const tlmg_kv8_batch b = { m.table + l, m.q_start, m.dargs + 2, nullptr, 1, 1, 1, 1, m.max_ctx };
+    tlmg_kv8_score s = {};
+    s.causal = 1;
+    const float *k = m.qkv + (size_t)m.H * m.hd, *v = k + (size_t)m.KV * m.hd;
+    int rc = tlmg_kv8_append(&m.kv8, &b, TLMG_DT_F32, k, v, 0, st);
+    if (!rc)
+        rc = tlmg_kv8_attend(&m.kv8, &b, &s, m.H, TLMG_DT_F32, m.qkv, 0, m.att, nullptr, nullptr, 0, m.awork,
+                             m.awork_bytes, st);
+    return rc;
 }
 
 }  // namespace tlmg

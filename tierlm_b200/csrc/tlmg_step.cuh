@@ -6,6 +6,8 @@
 #include <vector>
 #include <cuda_runtime.h>
 
+#include "../../include/tlmg.h"
+
 namespace tlmg {
 
 // Attention weights of one layer, copied into device memory. When q, k and
@@ -37,6 +39,11 @@ struct StepModel {
     // KV pages: one page of `page` positions per layer, [L][KV][page][hd]
     void *kpool = nullptr, *vpool = nullptr;
     int32_t *table = nullptr;           // [L]: table[l] = l
+    // 8-bit pages (kv_dt TLMG_DT_KV8_*): every layer's page in one cache, and
+    // the one-token batch's q_start = { 0, 1 }
+    tlmg_kv8 kv8 = {};
+    int32_t *q_start = nullptr;
+    bool is_kv8() const { return kv8.k != nullptr; }
     float *awork = nullptr;
     size_t awork_bytes = 0;
     // per-step scratch
@@ -88,7 +95,11 @@ int step_embed(int dt, const uint8_t *base, size_t rb, int token, const int32_t 
                cudaStream_t st);
 // qk-norm (when given), RoPE of the q and k heads in qkv, then k and v of
 // the position into layer l's page (device buffers of m; the position's
-// RoPE row of m.rope).
+// RoPE row of m.rope). 8-bit pages are left to step_attend_kv8.
 int step_heads(const StepModel &m, int l, int pos, const int32_t *dargs, float eps, cudaStream_t st);
+
+// 8-bit pages: appends the position's K and V rows (in m.qkv) to layer l and
+// attends into m.att. The row count is read from m.dargs[2].
+int step_attend_kv8(const StepModel &m, int l, cudaStream_t st);
 
 }  // namespace tlmg

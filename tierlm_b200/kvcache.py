@@ -286,3 +286,78 @@ class Kv8Cache:
                                          weights.shape[2], _f32(weights_out, "weights_out"),
                                          0 if weights_out is None else weights_out.shape[2], st))
         return rows, lens
+
+
+def _main() -> None:
+    """`python -m tierlm_b200.kvcache --prompt N --tokens T --keep R`: one layer's
+    serving loop on random rows. A prompt goes in by chunks (append, then
+    attention of the chunk), tokens are decoded one by one while the weights
+    that every row receives are accumulated, the sequence is cut to R rows by
+    those weights, and decoding goes on in the rows that are left. Prints the
+    device time of each part (CUDA events, second of two passes) and how far
+    the outputs after the cut are from those of the whole cache."""
+    import argparse
+    ap = argparse.ArgumentParser()
+    ap.add_argument("--prompt", type=int, default=8192)
+    ap.add_argument("--chunk", type=int, default=2048)
+    ap.add_argument("--tokens", type=int, default=32)
+    ap.add_argument("--keep", type=int, default=2048)
+    ap.add_argument("--fmt", choices=["int8", "e4m3"], default="int8")
+    ap.add_argument("--heads", type=int, default=32)
+    ap.add_argument("--kv-heads", type=int, default=4)
+    ap.add_argument("--head-dim", type=int, default=128)
+    ap.add_argument("--page", type=int, default=64)
+    ap.add_argument("--softcap", type=float, default=0.0)
+    a = ap.parse_args()
+    dev = torch.device("cuda:0")
+    check(load().tlmg_init(0))
+    H, KV, hd, N, T = a.heads, a.kv_heads, a.head_dim, a.prompt, a.tokens
+    if a.keep < 36 or N <= 0 or T <= 0 or a.chunk <= 0:
+        raise SystemExit("kvcache: prompt, tokens and chunk of at least 1, keep of at least 36 rows")
+    whole, cut = -(-(N + 2 * T) // a.page), -(-(a.keep + T) // a.page)
+    g = torch.Generator(device=dev).manual_seed(0)
+    rnd = lambda n, h: torch.randn((n, h, hd), generator=g, device=dev).to(torch.bfloat16)  # noqa: E731
+    q, k, v = rnd(N + 2 * T, H), rnd(N + 2 * T, KV), rnd(N + 2 * T, KV)
+    cache = Kv8Cache(whole + cut, KV, a.page, hd, fmt=INT8 if a.fmt == "int8" else E4M3, positions=True, device=dev)
+    order = torch.randperm(whole + cut, generator=g, device=dev).to(torch.int32)
+    table, cut_table = order[None, :whole].contiguous(), order[None, whole:].contiguous()
+    score = Score(softcap=a.softcap)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    one = i32(0, 1)
+
+    def feed(i: int, n: int, tab: torch.Tensor, rows: int, **kw):
+        """Tokens i .. i + n - 1 into a sequence that then has `rows` rows."""
+        at = torch.arange(i, i + n, dtype=torch.int32, device=dev)
+        b = Kv8Batch(tab, one if n == 1 else i32(0, n), i32(rows), n, rows, q_pos=at)
+        cache.append(k[i:i + n], v[i:i + n], b)
+        return cache.attend(q[i:i + n], b, score, **kw), b
+
+    def timed(what: str, fn, show: bool):
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        r = fn()
+        e1.record()
+        torch.cuda.synchronize()
+        if show:
+            print(f"{what}: {e0.elapsed_time(e1):.3f} ms")
+        return r
+
+    for show in (False, True):
+        weights = torch.zeros((1, KV, N + 2 * T), device=dev)
+        timed(f"prompt of {N} in chunks of {a.chunk}",
+              lambda: [feed(i, min(a.chunk, N - i), table, min(i + a.chunk, N)) for i in range(0, N, a.chunk)], show)
+        b = timed(f"{T} tokens, weights accumulated",
+                  lambda: [feed(i, 1, table, i + 1, weights=weights)[1] for i in range(N, N + T)], show)[-1]
+        rows, lens = timed(f"cut of {N + T} rows to {a.keep}",
+                           lambda: cache.evict(weights, b, cut_table, a.keep, sink=4, recent=32), show)
+        left = int(lens[0])
+        short = timed(f"{T} tokens in {left} rows",
+                      lambda: [feed(N + T + i, 1, cut_table, left + i + 1)[0] for i in range(T)], show)
+        full = timed(f"{T} tokens in {N + T} rows",
+                     lambda: [feed(N + T + i, 1, table, N + T + i + 1)[0] for i in range(T)], show)
+    s, f = torch.cat(short).float(), torch.cat(full).float()
+    print(f"kept {left} of {N + T} rows a head; |out - whole| / |whole| = {float((s - f).norm() / f.norm()):.3f}")
+
+
+if __name__ == "__main__":
+    _main()

@@ -223,8 +223,9 @@ class MoeContext:
     # ---- the whole decoder step (tlm_model_step on the GPU)
     def step_open(self, n_heads: int, n_kv_heads: int, head_dim: int, vocab: int, inv_freq,
                   attn_scale: float = 1.0, max_ctx: int = 1024, kv_dtype: int = 0, attn_mode: int = 0) -> None:
-        """KV pages for max_ctx positions (kv_dtype F32 = 0 or BF16 = 2),
-        attention mode 0 = exact, 1 = split; inv_freq f32[head_dim / 2]."""
+        """KV pages for max_ctx positions (kv_dtype F32 = 0, BF16 = 2, or with
+        attn_mode 1 the 8-bit rows _lib.KV8_INT8 / KV8_E4M3), attention mode
+        0 = exact, 1 = split; inv_freq f32[head_dim / 2]."""
         inv = np.ascontiguousarray(inv_freq, np.float32)
         check(self._lib.tlmg_step_open(self._h, n_heads, n_kv_heads, head_dim, vocab, _ptr(inv), float(attn_scale),
                                        max_ctx, kv_dtype, attn_mode))
