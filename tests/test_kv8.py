@@ -543,6 +543,36 @@ def test_prefill_positions_and_poison():
     assert torch.isnan(out[150:]).all() and (out[:150] == good[:150]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("pool", ["ascending", "jumbled_tiles", "none"])
+@pytest.mark.parametrize("name", ["causal", "window", "sinks", "doc", "doc_window", "both_ways"])
+def test_prefill_whole_tiles(name, pool, dtype):
+    """Key tiles that every query sees, that none sees and that some see, by positions with gaps and by documents."""
+    lens, news, H, KV, hd = [700, 420], [260, 150], 4, 2, 64
+    host, table, q_start, q, rng = make(34, lens, news, H, KV, hd, K.INT8, 16, 16, pos=pool != "none", dtype=dtype)
+    q_pos = None
+    if pool != "none":
+        q_pos = np.zeros(q_start[-1], np.int32)
+        for s, L in enumerate(lens):
+            for h in range(KV):                        # every head has kept other rows
+                p = np.sort(rng.permutation(2 * L)[:L]).astype(np.int32)
+                p[L - news[s]:] = 2 * L + np.arange(news[s])
+                if pool == "jumbled_tiles":            # whole tiles of 128 rows, the queries' own among them, in another order
+                    p = p[np.concatenate([np.arange(128, 256), np.arange(L - L % 128, L), np.arange(128),
+                                          np.arange(256, L - L % 128)])]
+                for t in range(L):
+                    host.pos[table[s, t // 16], h, t % 16] = p[t]
+            q_pos[q_start[s]:q_start[s + 1]] = 2 * L + np.arange(news[s])
+    span = 2 * max(lens) + 300
+    doc = np.zeros((2, span), np.int32)
+    doc[:, span // 3:], doc[:, span // 2:] = 1, 2
+    doc[0, :] = np.where(np.arange(span) < 600, doc[0, :], 2)
+    mods = {"causal": {}, "window": dict(window=300), "sinks": dict(window=140, prefix=np.array([130, 3], np.int32)), "doc": dict(doc=doc),
+            "doc_window": dict(doc=doc, window=200), "both_ways": dict(causal=False)}[name]
+    check_attend(host, table, q_start, lens, q, H, q_pos=q_pos, **mods)
+
+
 def mods_of(name, rng, lens, H):
     n = len(lens)
     doc = np.full((n, max(lens)), -1, np.int32)

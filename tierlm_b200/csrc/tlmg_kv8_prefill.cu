@@ -64,7 +64,9 @@ template <bool F32> struct Role {
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int META = 4;           // buffers of per-key scales
-constexpr int LIST = 2048;        // key tiles (262,144 rows) up to which tiles of other documents are left out
+// Key tiles (262,144 rows) up to which those that no query of the CTA sees are left out by a list, where a position pool or
+// documents mask: 8,192 tokens of 32 heads on 4 with a pool took 3,350 us with every tile read.
+constexpr int LIST = 2048;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ uint32_t saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -75,13 +77,14 @@ template <int HD> struct Smem {
     alignas(128) uint8_t v[2][TK * HD * 2];
     alignas(16) float ks[META][TK], vs[META][TK], lv[META][TK], rv[META][TK];   // scales; of V also log2 and 1 / scale
     alignas(16) int pos[META][TK], doc[META][TK];
-    alignas(4) uint8_t tame[META][4];
+    // per quarter of a tile: no scale is extreme; with a table to mask by: every row of the CTA sees every key
+    alignas(4) uint8_t tame[META][4], seen[META][4];
     uint32_t row[2][TK];
     float qs[2][TQ], part[2][2][TQ], sums[2][2][TQ];     // [tile][half][row]: the halves' maxima; in the end their sums
     uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], x_full[2], o_full[2], meta_full[META], drain;
     uint32_t tmem;
     int abort, pmin, pmax, dmin, dmax, n_list;
-    uint16_t list[LIST];      // the key tiles that hold a key of the queries' documents
+    uint16_t list[LIST];      // the key tiles that hold a key which a query may see
 };
 
 __device__ __forceinline__ void mbar_init(uint64_t *b, uint32_t n) {
@@ -327,15 +330,32 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
     int n = rg.n;
     bool listed = false;
     if constexpr (SHAPED) {
-        listed = docs && !a.c.pos && n <= LIST;
+        listed = n <= LIST && (docs || (a.c.pos && (a.causal || a.window)));
         if (listed) {
-            // a tile takes part if one of its keys' documents lies between the queries' smallest and largest
-            const int lo = sm.dmin, hi = sm.dmax;
+            // a tile takes part if one of its keys lies where the rows' positions allow, and its document between the
+            // queries' smallest and largest (a bad page's rows stand at 0, as below)
+            const int lo = sm.dmin, hi = sm.dmax, pre = a.prefix ? a.prefix[s] : 0;
+            const int32_t *table = a.b.page_table + (size_t)s * a.b.table_stride;
             for (int v = warp; v < n; v += THREADS / 32) {
                 bool any = false;
-                for (int t = rg.t0(v) + lane; t < rg.t0(v) + TK && t < q.L; t += 32) {
-                    const int d = t < a.doc_stride ? docs[t] : -1;
-                    any = any || (d >= lo && d <= hi);
+                int kp[TK / 32];
+#pragma unroll
+                for (int i = 0; i < TK / 32; i++) {
+                    const int t = rg.t0(v) + 32 * i + lane;
+                    kp[i] = t;
+                    if (a.c.pos) {
+                        const int32_t e = t < q.L ? __ldg(table + (t >> a.c.lp)) : -1;
+                        kp[i] = a.c.ok(e) ? __ldg(a.c.pos + a.c.row(e, kvh, t)) : 0;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < TK / 32; i++) {
+                    bool see = kp[i] < pre || ((!a.causal || kp[i] <= pmax) && (!a.window || (int64_t)pmin - kp[i] < a.window));
+                    if (docs) {
+                        const int d = kp[i] >= 0 && kp[i] < a.doc_stride ? __ldg(docs + kp[i]) : -1;
+                        see = see && d >= lo && d <= hi;
+                    }
+                    any = any || (see && rg.t0(v) + 32 * i + lane < q.L);
                 }
                 any = __any_sync(0xFFFFFFFFu, any);
                 if (lane == 0) sm.list[v] = any;
@@ -458,7 +478,8 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                 tc_after();
                 const float *ks = sm.ks[mb], *vs = sm.vs[mb], *lv = sm.lv[mb];
                 // every key of the tile is seen by every row of the CTA
-                const bool open = !lists && t0 + TK <= q.L && (!a.causal || t0 + TK - 1 <= pmin) && (!a.window || pmax - t0 < a.window);
+                const bool open = lists ? *reinterpret_cast<const uint32_t *>(sm.seen[mb]) == 0x01010101u
+                                        : t0 + TK <= q.L && (!a.causal || t0 + TK - 1 <= pmin) && (!a.window || pmax - t0 < a.window);
                 // one scale for 8 keys, none of them extreme: the scales come in per group
                 const bool grp = a.c.lb >= 3 && *reinterpret_cast<const uint32_t *>(sm.tame[mb]) == 0x01010101u;
                 const bool rawS = open && grp && !(SHAPED && (a.softcap > 0.0f || a.slopes));
@@ -774,8 +795,17 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
             sm.rv[mb][h] = F32 ? __frcp_rn(mv) : __fdividef(1.0f, mv);
             const bool tame = __all_sync(0xFFFFFFFFu, mv > 0x1p-60f && mv < 0x1p60f);
             if (lane == 0) sm.tame[mb][warp - SW - 4] = tame;
-            sm.pos[mb][h] = mp;
-            sm.doc[mb][h] = md;
+            if constexpr (SHAPED) {
+                if (a.c.pos || docs) {
+                    const int t = tile_at(j) + h, p = a.c.pos ? mp : t;
+                    bool see = t < q.L && (!a.causal || p <= pmin) && (!a.window || (int64_t)pmax - p < a.window);
+                    see = see && (!docs || (sm.dmin == md && sm.dmax == md));
+                    see = __all_sync(0xFFFFFFFFu, see);
+                    if (lane == 0) sm.seen[mb][warp - SW - 4] = see;
+                    sm.pos[mb][h] = mp;
+                    sm.doc[mb][h] = md;
+                }
+            }
             mbar_arrive(&sm.meta_full[mb]);
         };
         auto load = [&](int j, int i0, uint4 (&x)[NP]) {   // pieces i0 .. i0 + NP - 1 of the thread

@@ -290,7 +290,7 @@ class Kv8Cache:
 
 def _main() -> None:
     """`python -m tierlm_b200.kvcache --prompt N --tokens T --keep R`: one layer's
-    serving loop on random rows. A prompt goes in by chunks (append, then
+    serving loop on random rows, a tenth of them near what the tokens ask for. A prompt goes in by chunks (append, then
     attention of the chunk), tokens are decoded one by one while the weights
     that every row receives are accumulated, the sequence is cut to R rows by
     those weights, and decoding goes on in the rows that are left. Prints the
@@ -318,6 +318,9 @@ def _main() -> None:
     g = torch.Generator(device=dev).manual_seed(0)
     rnd = lambda n, h: torch.randn((n, h, hd), generator=g, device=dev).to(torch.bfloat16)  # noqa: E731
     q, k, v = rnd(N + 2 * T, H), rnd(N + 2 * T, KV), rnd(N + 2 * T, KV)
+    u = rnd(1, 1).sign() * (8.0 / hd ** 0.5) ** 0.5     # adds 8 to a score where both have it
+    q += u
+    k += u * (torch.rand((N + 2 * T, 1, 1), generator=g, device=dev) < 0.1)
     cache = Kv8Cache(whole + cut, KV, a.page, hd, fmt=INT8 if a.fmt == "int8" else E4M3, positions=True, device=dev)
     order = torch.randperm(whole + cut, generator=g, device=dev).to(torch.int32)
     table, cut_table = order[None, :whole].contiguous(), order[None, whole:].contiguous()
