@@ -573,6 +573,21 @@ def test_prefill_whole_tiles(name, pool, dtype):
     check_attend(host, table, q_start, lens, q, H, q_pos=q_pos, **mods)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("max_q,max_kv", [(600, 310), (40000, 200000), (40000, 60000)])
+def test_prefill_loose_bounds(max_q, max_kv, dtype):
+    """max_q and max_kv far above the lengths: the same results whether all, some or one of the KV heads share a turn."""
+    lens, news, H, KV, hd = [300, 5, 260], [280, 5, 3], 6, 3, 128
+    host, table, q_start, q, _ = make(35, lens, news, H, KV, hd, K.E4M3, 16, 16, dtype=dtype)
+    want = host.gpu().attend(q.cuda(), batch(table, q_start, lens), lse=True)
+    got = host.gpu().attend(q.cuda(), batch(table, q_start, lens, max_q=max_q, max_kv=max_kv), lse=True)
+    ref, rlse, _, ds, mags, _ = reference(host, q.float().numpy(), table, q_start, lens, H)
+    for out, lse in (want, got):
+        assert_close(out.float().cpu().numpy(), ref, out_bound(ref, mags, ds, dtype))
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
 def mods_of(name, rng, lens, H):
     n = len(lens)
     doc = np.full((n, max(lens)), -1, np.int32)

@@ -683,19 +683,6 @@ __global__ void __launch_bounds__(WG_THREADS) k_kv8_weights(const __grid_constan
     a.weights[((int64_t)s * a.c.KV + kvh) * a.w_stride + t] += sum;
 }
 
-int sm_count() {
-    static thread_local int dev = -1, n = 0;
-    int d = 0;
-    cudaGetDevice(&d);
-    if (d != dev) {
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d) != cudaSuccess || n <= 0) {
-            cudaGetLastError();
-            n = 148;
-        }
-        dev = d;
-    }
-    return n;
-}
 
 bool smem_opt_in(const void *fn, size_t bytes) {
     static thread_local std::vector<std::pair<const void *, int>> done;
@@ -723,8 +710,11 @@ struct Split {
 Split split_plan(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_score &s, int H, int q_dt, bool weights) {
     Split p{};
     const int G = H / c.KV;
-    p.wide = !weights && kv8_prefill_serves(c, b, H, q_dt);
-    if (p.wide) return p;
+    p.wide = !weights && kv8_prefill_serves(c, b, H);
+    if (p.wide) {
+        p.total = kv8_prefill_work_bytes(c, b, H, q_dt) + 16;
+        return p;
+    }
     // 16 query rows a CTA where there are more than 8 (not for f32 ones of 256 dims: no registers)
     p.rm = (int64_t)b.max_q * G > 8 && (q_dt != TLMG_DT_F32 || c.hd <= 128) ? 2 : 1;
     const int rows = 8 * p.rm;
@@ -847,6 +837,7 @@ extern "C" int tlmg_kv8_attend(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const
                          "kv8_attend: work holds %zu bytes at %p, needs %zu, 16-byte aligned", work_bytes, work, p.total);
     Kv8Attn a{};
     a.c = kv8_view(c);
+    a.kv8 = *c;
     a.b = *b;
     a.H = H;
     a.G = H / c->KV;
@@ -881,6 +872,6 @@ extern "C" int tlmg_kv8_attend(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const
         a.lse2 = a.scores + rows * p.s_stride;
     }
     cudaStream_t cs = pick_stream(stream);
-    if (p.wide) return kv8_prefill(a, c->fmt, q_dt, cs);
+    if (p.wide) return kv8_prefill(a, q_dt, work, cs);
     return c->fmt == TLMG_KV8_INT8 ? launch_split_hd<TLMG_KV8_INT8>(a, p, q_dt, cs) : launch_split_hd<TLMG_KV8_E4M3>(a, p, q_dt, cs);
 }

@@ -25,6 +25,12 @@ struct Kv8Attn {
     int n_split, tiles;
     float *po, *pm, *pl, *scores, *lse2;
     int64_t s_stride;
+    // many query rows: the cache as the caller gave it; tile images of the sequences from s0 and the nkv KV heads from kv0,
+    // n_img tiles for each pair, and what an image's code is worth
+    tlmg_kv8 kv8;
+    uint8_t *img, *heads;
+    int s0, kv0, nkv, n_img;
+    float unit;
 };
 
 // tanh(x) = x (c0 + c1 x^2 + .. + c5 x^10) for |x| < TANH_X within 2e-7: fitted (reweighted least squares towards the
@@ -53,6 +59,7 @@ __device__ __forceinline__ float kv8_ex2(float x) {   // 2^x, results below 2^-1
 template <int TILE> struct Kv8Range {
     int nA, loB, n;   // tiles of the first part, first row of the second, tiles in all
     __device__ __forceinline__ int t0(int v) const { return v < nA ? v * TILE : loB + (v - nA) * TILE; }
+    __device__ __forceinline__ bool has(int t) const { return t < nA * TILE || (t >= loB && t < loB + (n - nA) * TILE); }
 };
 template <int TILE>
 __device__ __forceinline__ Kv8Range<TILE> kv8_range(const Kv8Attn &a, const Kv8Seq &q, int s, int pmin, int pmax) {
@@ -75,8 +82,23 @@ __device__ __forceinline__ Kv8Range<TILE> kv8_range(const Kv8Attn &a, const Kv8S
     return r;
 }
 
-// The form for many query rows (tlmg_kv8_prefill.cu): whether it serves a call, and the call.
-bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt);
-int kv8_prefill(const Kv8Attn &a, int fmt, int q_dt, cudaStream_t st);
+inline int sm_count() {
+    thread_local int dev = -1, n = 0;
+    int d = 0;
+    cudaGetDevice(&d);
+    if (d != dev) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            n = 148;
+        }
+        dev = d;
+    }
+    return n;
+}
+
+// The form for many query rows (tlmg_kv8_prefill.cu): whether it serves a call, its workspace, and the call.
+bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H);
+size_t kv8_prefill_work_bytes(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt);
+int kv8_prefill(const Kv8Attn &a, int q_dt, void *work, cudaStream_t st);
 
 }  // namespace tlmg

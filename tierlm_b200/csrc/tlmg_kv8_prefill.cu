@@ -53,13 +53,17 @@ constexpr int CK = 16;            // columns of a round of the softmax loops: fe
 constexpr int HC = TK / 2;        // keys of a softmax thread: two threads share a query row
 constexpr int CV = 256;           // converting threads
 // What differs between 16-bit queries (two query tiles in turn) and f32 ones (one tile of which every operand but K and V
-// has a high and a low part). Registers a thread: 16-bit 72 at launch (896 x 72 = 64,512), then 512 x 80 + 256 x 56 +
-// 128 x 72 = 64,512; f32 96 at launch (640 x 96 = 61,440), then 256 x 144 + 256 x 56 + 128 x 72 = 60,416.
-template <bool F32> struct Role {
+// has a high and a low part), with converting warps or with tile images. Registers a thread: 16-bit 72 at launch (896 x 72 =
+// 64,512), then 512 x 80 + 256 x 56 + 128 x 72 = 64,512; f32 96 at launch (640 x 96 = 61,440), then 256 x 144 + 256 x 56 +
+// 128 x 72 = 60,416. Images: 16-bit 96 at launch (640 x 96 = 61,440), then 512 x 104 + 128 x 64 = 61,440; f32 168 at
+// launch (384 x 168 = 64,512), then 256 x 200 + 128 x 96 = 63,488.
+template <bool F32, bool IMG> struct Role {
     static constexpr int TILES = F32 ? 1 : 2;                 // query tiles of a CTA
-    static constexpr int SW = 8 * TILES;                      // softmax warps; then 8 that convert and 4 for the MMAs
-    static constexpr int THREADS = 32 * (SW + 12);
-    static constexpr int REGS_SOFTMAX = F32 ? 144 : 80, REGS_CONVERT = 56, REGS_MMA = 72;
+    static constexpr int SW = 8 * TILES;                      // softmax warps; then those that convert and 4 for the MMAs
+    static constexpr int MW = SW + (IMG ? 0 : 8);             // the MMAs' first warp
+    static constexpr int THREADS = 32 * (MW + 4);
+    static constexpr int REGS_SOFTMAX = IMG ? (F32 ? 200 : 104) : F32 ? 144 : 80, REGS_CONVERT = 56,
+                         REGS_MMA = IMG ? (F32 ? 96 : 64) : 72;
 };
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -71,12 +75,23 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ uint32_t saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// What the softmax needs of a tile's keys: scales (of V also log2 and 1 / scale), positions and documents.
+struct Meta {
+    float ks[TK], vs[TK], lv[TK], rv[TK];
+    int pos[TK], doc[TK];
+};
+// A tile as an image in global memory: K and V as the tensor core reads them, then Meta; and what decides whether it is read.
+template <int HD> constexpr size_t IMAGE = 2 * (size_t)TK * HD * 2 + sizeof(Meta);
+struct alignas(16) Kv8Head {
+    int pmin, pmax, dmin, dmax;   // of its rows: positions and documents
+    int tame, pad[3];
+};
+
 template <int HD> struct Smem {
     alignas(128) uint8_t q[2][TQ * HD * 2];
     alignas(128) uint8_t k[2][TK * HD * 2];
     alignas(128) uint8_t v[2][TK * HD * 2];
-    alignas(16) float ks[META][TK], vs[META][TK], lv[META][TK], rv[META][TK];   // scales; of V also log2 and 1 / scale
-    alignas(16) int pos[META][TK], doc[META][TK];
+    alignas(128) Meta m[META];
     // per quarter of a tile: no scale is extreme; with a table to mask by: every row of the CTA sees every key
     alignas(4) uint8_t tame[META][4], seen[META][4];
     uint32_t row[2][TK];
@@ -203,6 +218,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void mbar_expect(uint64_t *b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(saddr(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *b) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(saddr(dst)), "l"(src), "r"(bytes),
+                 "r"(saddr(b))
+                 : "memory");
+}
+
 // packed pairs of f32 (one issue slot for two)
 typedef unsigned long long f2;
 __device__ __forceinline__ f2 pk(float x, float y) {
@@ -250,21 +274,111 @@ __device__ __forceinline__ float cap_exp(float y, float capl) {
 
 constexpr float TOP = 14.0f;   // log2 of the largest p * v_scale right after a row's reference moved
 
+// Smallest and largest position of a sequence's tokens (by all threads of the CTA).
+__device__ __forceinline__ void token_span(const Kv8Attn &a, const Kv8Seq &q, int *mm, int &pmin, int &pmax) {
+    pmin = q.L - q.n, pmax = q.L - 1;
+    if (!a.b.q_pos) return;
+    if (threadIdx.x == 0) mm[0] = INT32_MAX, mm[1] = INT32_MIN;
+    __syncthreads();
+    int lo = INT32_MAX, hi = INT32_MIN;
+    for (int i = threadIdx.x; i < q.n; i += blockDim.x) {
+        const int p = a.b.q_pos[q.q0 + i];
+        lo = min(lo, p), hi = max(hi, p);
+    }
+    lo = __reduce_min_sync(0xFFFFFFFFu, lo), hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+    if ((threadIdx.x & 31) == 0) atomicMin(&mm[0], lo), atomicMax(&mm[1], hi);
+    __syncthreads();
+    pmin = mm[0], pmax = mm[1];
+}
+// Whether a row between these positions may be seen by a token between those.
+__device__ __forceinline__ bool may_see(const Kv8Attn &a, int pre, int kmin, int kmax, int pmin, int pmax) {
+    return kmin < pre || ((!a.causal || kmin <= pmax) && (!a.window || (int64_t)pmin - kmax < a.window));
+}
+
+// Tile images: every key tile that a token of its sequence may see, converted once for all of the query tiles. One CTA a
+// tile and KV head.
+template <int HD, int FMT>
+__global__ void __launch_bounds__(256) k_kv8_images(const __grid_constant__ Kv8Attn a) {
+    constexpr int SBO = HD * 16, PC = HD / 16, NP = TK * PC / 128;
+    __shared__ int mm[2], span[4][4], ok4[4];
+    __shared__ uint32_t row[TK];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = a.s0 + blockIdx.z, kvh = a.kv0 + blockIdx.y, t0 = blockIdx.x * TK;
+    Kv8Seq q;
+    if (!kv8_seq(a.b, a.c.lp, s, q) || t0 >= q.L || q.n == 0) return;
+    int pmin, pmax;
+    token_span(a, q, mm, pmin, pmax);
+    const Kv8Range<TK> rg = kv8_range<TK>(a, q, s, pmin, pmax);
+    if (!rg.has(t0)) return;
+    const size_t at = ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * a.n_img + blockIdx.x;
+    uint8_t *img = a.img + at * IMAGE<HD>;
+    Kv8Head *head = reinterpret_cast<Kv8Head *>(a.heads) + at;
+    const int32_t *table = a.b.page_table + (size_t)s * a.b.table_stride;
+    if (tid < TK) {
+        const int t = t0 + tid;
+        const int32_t e = t < q.L ? __ldg(table + (t >> a.c.lp)) : -1;
+        const bool have = a.c.ok(e);
+        const uint32_t rid = have ? a.c.row(e, kvh, t) : 0xFFFFFFFFu;
+        row[tid] = rid;
+        const float none = t < q.L ? __uint_as_float(0x7FC00000u) : 1.0f;   // a bad page: NaN for whoever sees it
+        const float ks = have ? __ldg(a.c.ks + (rid >> a.c.lb)) : none, vs = have ? __ldg(a.c.vs + (rid >> a.c.lb)) : none;
+        const int p = a.c.pos ? (have ? __ldg(a.c.pos + rid) : 0) : t;
+        const int d = a.doc && p >= 0 && p < a.doc_stride ? __ldg(a.doc + (size_t)s * a.doc_stride + p) : -1;
+        Meta *m = reinterpret_cast<Meta *>(img + 4 * TK * HD);
+        m->ks[tid] = ks, m->vs[tid] = vs, m->lv[tid] = fmaxf(log2f(vs), -60.0f), m->rv[tid] = __frcp_rn(vs);
+        m->pos[tid] = p, m->doc[tid] = d;
+        const bool in = t < q.L, tame = __all_sync(0xFFFFFFFFu, vs > 0x1p-60f && vs < 0x1p60f);
+        const int x0 = __reduce_min_sync(0xFFFFFFFFu, in ? p : INT32_MAX), x1 = __reduce_max_sync(0xFFFFFFFFu, in ? p : INT32_MIN),
+                  x2 = __reduce_min_sync(0xFFFFFFFFu, in ? d : INT32_MAX), x3 = __reduce_max_sync(0xFFFFFFFFu, in ? d : INT32_MIN);
+        if (lane == 0) span[warp][0] = x0, span[warp][1] = x1, span[warp][2] = x2, span[warp][3] = x3, ok4[warp] = tame;
+    }
+    __syncthreads();
+    Kv8Head hd;
+    hd.pmin = min(min(span[0][0], span[1][0]), min(span[2][0], span[3][0]));
+    hd.pmax = max(max(span[0][1], span[1][1]), max(span[2][1], span[3][1]));
+    hd.dmin = min(min(span[0][2], span[1][2]), min(span[2][2], span[3][2]));
+    hd.dmax = max(max(span[0][3], span[1][3]), max(span[2][3], span[3][3]));
+    hd.tame = ok4[0] && ok4[1] && ok4[2] && ok4[3];
+    hd.pad[0] = hd.pad[1] = hd.pad[2] = 0;
+    if (tid == 0) *head = hd;
+    // hidden by the position pool from every token: no list takes it (a sequence too long for lists reads all tiles)
+    if (a.c.pos && rg.n <= LIST && !may_see(a, a.prefix ? a.prefix[s] : 0, hd.pmin, hd.pmax, pmin, pmax)) return;
+    const int h = tid & 127, prow = (h & 7) + 8 * (h / (8 * PC)), piece = (h >> 3) % PC;
+    constexpr int RSTEP = 8 * (128 / (8 * PC));
+    const uint8_t *pool = tid >= 128 ? a.c.v : a.c.k;
+    uint8_t *dst = img + (tid >= 128 ? 2 * TK * HD : 0) + (prow >> 3) * SBO + piece * 256 + (prow & 7) * 16;
+    uint4 x[NP];
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        const uint32_t rid = row[prow + RSTEP * i];
+        x[i] = rid != 0xFFFFFFFFu ? __ldg(reinterpret_cast<const uint4 *>(pool + (size_t)rid * HD + 16 * piece)) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NP; i++, dst += RSTEP / 8 * SBO) {
+        const uint32_t b0 = kv8_bias<FMT>(x[i].x), b1 = kv8_bias<FMT>(x[i].y), b2 = kv8_bias<FMT>(x[i].z), b3 = kv8_bias<FMT>(x[i].w);
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(kv8_half2<FMT, 0>(b0), kv8_half2<FMT, 1>(b0), kv8_half2<FMT, 0>(b1), kv8_half2<FMT, 1>(b1));
+        *reinterpret_cast<uint4 *>(dst + 128) = make_uint4(kv8_half2<FMT, 0>(b2), kv8_half2<FMT, 1>(b2), kv8_half2<FMT, 0>(b3), kv8_half2<FMT, 1>(b3));
+    }
+}
+
+// IMG: K and V come as tile images (whose codes' unit is a.unit) by bulk copies; else by 8 converting warps.
 // SHAPED: softcap, slopes, documents or a position pool; without them the code is half the size, and the instruction
 // cache is what these roles share most tightly.
-template <int HD, int FMT, typename QT, bool SHAPED>
-__global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefill(const __grid_constant__ Kv8Attn a) {
+template <int HD, int FMT, typename QT, bool SHAPED, bool IMG>
+__global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_prefill(const __grid_constant__ Kv8Attn a) {
     extern __shared__ __align__(128) uint8_t raw[];
     Smem<HD> &sm = *reinterpret_cast<Smem<HD> *>(raw);
     constexpr bool F32 = sizeof(QT) == 4;
-    using RL = Role<F32>;
-    constexpr int THREADS = RL::THREADS, SW = RL::SW, RPC = RL::TILES * TQ;   // query rows of the CTA
+    using RL = Role<F32, IMG>;
+    constexpr int THREADS = RL::THREADS, SW = RL::SW, MW = RL::MW, RPC = RL::TILES * TQ;   // query rows of the CTA
     constexpr int SBO = HD * 16;              // bytes between 8-row groups of an operand
     constexpr int PC = HD / 16;               // 16-byte pieces of a code row
     constexpr int NP = TK * PC / CV;          // pieces of half a tile per converting thread
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int s = blockIdx.y, kvh = blockIdx.x % a.c.KV;
-    const int tiles = gridDim.x / a.c.KV, rt = tiles - 1 - blockIdx.x / a.c.KV;   // the last tokens see the most keys: first
+    const int nkv = IMG ? a.nkv : a.c.KV, s = (IMG ? a.s0 : 0) + blockIdx.y, kvh = (IMG ? a.kv0 : 0) + blockIdx.x % nkv;
+    const int tiles = gridDim.x / nkv, rt = tiles - 1 - blockIdx.x / nkv;   // the last tokens see the most keys: first
+    const float unit = IMG ? a.unit : kv8_f16_unit<FMT>();
+    const size_t slot = IMG ? ((size_t)blockIdx.y * nkv + blockIdx.x % nkv) * a.n_img : 0;
+    const Kv8Head *heads = reinterpret_cast<const Kv8Head *>(a.heads) + slot;
     QT *out = static_cast<QT *>(a.out);
     Kv8Seq q;
     if (!kv8_seq(a.b, a.c.lp, s, q)) {
@@ -291,8 +405,8 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
         sm.dmax = INT32_MIN;
         mbar_init(&sm.q_full, two ? 4 * TQ : 2 * TQ);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sm.k_full[i], CV / 2);
-            mbar_init(&sm.v_full[i], CV / 2);
+            mbar_init(&sm.k_full[i], IMG ? 1 : CV / 2);
+            mbar_init(&sm.v_full[i], IMG ? 1 : CV / 2);
             mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_empty[i], 1);
             mbar_init(&sm.s_full[i], 1);
@@ -300,11 +414,11 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
             mbar_init(&sm.x_full[i], 2 * TQ);
             mbar_init(&sm.o_full[i], 1);
         }
-        for (int i = 0; i < META; i++) mbar_init(&sm.meta_full[i], 128);
+        for (int i = 0; i < META; i++) mbar_init(&sm.meta_full[i], IMG ? 1 : 128);
         mbar_init(&sm.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == SW + 8) {
+    if (warp == MW) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -336,7 +450,13 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
             // queries' smallest and largest (a bad page's rows stand at 0, as below)
             const int lo = sm.dmin, hi = sm.dmax, pre = a.prefix ? a.prefix[s] : 0;
             const int32_t *table = a.b.page_table + (size_t)s * a.b.table_stride;
-            for (int v = warp; v < n; v += THREADS / 32) {
+            if constexpr (IMG) {
+                for (int v = tid; v < n; v += THREADS) {
+                    const int4 x = __ldg(reinterpret_cast<const int4 *>(heads + rg.t0(v) / TK));
+                    sm.list[v] = may_see(a, pre, x.x, x.y, pmin, pmax) && (!docs || (x.w >= lo && x.z <= hi));
+                }
+            }
+            for (int v = warp; !IMG && v < n; v += THREADS / 32) {
                 bool any = false;
                 int kp[TK / 32];
 #pragma unroll
@@ -425,7 +545,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                     m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
                     const int e = min(max((int)((__float_as_uint(m) >> 23) & 255u) - 136, -100), 100);
                     const float up = R0 + w * TQ + row < n_rows ? __int_as_float((127 - e) << 23) : 0.0f;
-                    if (cq == 0) sm.qs[w][row] = __int_as_float((127 + e) << 23) * a.scale * kv8_f16_unit<FMT>();
+                    if (cq == 0) sm.qs[w][row] = __int_as_float((127 + e) << 23) * a.scale * unit;
                     uint8_t *dst = sm.q[w] + (row >> 3) * SBO + (row & 7) * 16 + cq * 128;
 #pragma unroll
                     for (int i = 0; i < HD / 32; i++) {
@@ -476,7 +596,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                 ok = mbar_wait_warp(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait_warp(&sm.s_full[sb], F32 ? (j >> 1) & 1 : j & 1, &sm.abort);
                 if (!ok) break;
                 tc_after();
-                const float *ks = sm.ks[mb], *vs = sm.vs[mb], *lv = sm.lv[mb];
+                const float *ks = sm.m[mb].ks, *vs = sm.m[mb].vs, *lv = sm.m[mb].lv;
                 // every key of the tile is seen by every row of the CTA
                 const bool open = lists ? *reinterpret_cast<const uint32_t *>(sm.seen[mb]) == 0x01010101u
                                         : t0 + TK <= q.L && (!a.causal || t0 + TK - 1 <= pmin) && (!a.window || pmax - t0 < a.window);
@@ -541,7 +661,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                         if (ali) {
                             if (by_pos) {
 #pragma unroll
-                                for (int i = 0; i < CK; i++) z[i] = __fmaf_rn(-slope, fabsf((float)(qp - sm.pos[mb][c + i])), z[i]);
+                                for (int i = 0; i < CK; i++) z[i] = __fmaf_rn(-slope, fabsf((float)(qp - sm.m[mb].pos[c + i])), z[i]);
                             } else {
                                 const float far = (float)(qp - t0 - c);
 #pragma unroll
@@ -553,7 +673,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                             if (by_pos) {
 #pragma unroll
                                 for (int i = 0; i < CK; i++) {
-                                    const int kp = sm.pos[mb][c + i];
+                                    const int kp = sm.m[mb].pos[c + i];
                                     const bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
                                     z[i] = see && t0 + c + i < q.L ? z[i] : -INFINITY;
                                 }
@@ -564,7 +684,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                             if (by_doc) {
 #pragma unroll
                                 for (int i = 0; i < CK; i += 4) {
-                                    const int4 d = *reinterpret_cast<const int4 *>(&sm.doc[mb][c + i]);
+                                    const int4 d = *reinterpret_cast<const int4 *>(&sm.m[mb].doc[c + i]);
                                     z[i] = d.x == qd ? z[i] : -INFINITY;
                                     z[i + 1] = d.y == qd ? z[i + 1] : -INFINITY;
                                     z[i + 2] = d.z == qd ? z[i + 2] : -INFINITY;
@@ -592,12 +712,12 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                         tmem_ld4(ts + c, x);
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const int col = c + i, t = t0 + col, kp = SHAPED && a.c.pos ? sm.pos[mb][col] : t;
+                            const int col = c + i, t = t0 + col, kp = SHAPED && a.c.pos ? sm.m[mb].pos[col] : t;
                             float z = __uint_as_float(x[i]) * (ks[col] * mul);
                             if (SHAPED && a.softcap > 0.0f) z = cap_exp(z, capl);
                             if (SHAPED && a.slopes) z = __fmaf_rn(-slope, fabsf((float)(qp - kp)), z);
                             bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
-                            see = see && t < q.L && (!(SHAPED && docs) || sm.doc[mb][col] == qd);
+                            see = see && t < q.L && (!(SHAPED && docs) || sm.m[mb].doc[col] == qd);
                             z = see ? z : -INFINITY;
                             m0 = fmaxf(m0, z + lv[col]);
                             x[i] = __float_as_uint(z);
@@ -651,7 +771,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                             }
                             float u0, u1;
                             upk(add2(add2(pk(y[0], y[1]), pk(y[2], y[3])), add2(pk(y[4], y[5]), pk(y[6], y[7]))), u0, u1);
-                            lsum = __fmaf_rn(u0 + u1, sm.rv[mb][c + g], lsum);
+                            lsum = __fmaf_rn(u0 + u1, sm.m[mb].rv[c + g], lsum);
                         }
                         if constexpr (F32) {   // high parts and remainders of 16 keys over their 16 scores
                             tmem_st8(ts + c, p);
@@ -718,7 +838,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                 l = lsum + sm.sums[w][half ^ 1][r];
             }
             tc_after();
-            const float inv = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? 0.0f : __fdividef(kv8_f16_unit<FMT>(), l);
+            const float inv = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? 0.0f : __fdividef(unit, l);
             if constexpr (F32) {
                 if (ok && n > 0) add_o();
                 if (live)
@@ -749,7 +869,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
             if (live && half == 0 && a.lse)
                 a.lse[orow] = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? -INFINITY : (log2f(l) - (wref == -INFINITY ? 0.0f : TOP - wref)) * LN2;
         }
-    } else if (warp < SW + 8) {
+    } else if (!IMG && warp < MW) {
         // ---- codes to f16 ----
         regs_down<RL::REGS_CONVERT>();
         const int c = tid - 32 * SW;
@@ -789,10 +909,10 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
         auto put_meta = [&](int j) {
             if (!is_v) return;
             const int mb = j & (META - 1);
-            sm.ks[mb][h] = mk;
-            sm.vs[mb][h] = mv;
-            sm.lv[mb][h] = fmaxf(F32 ? log2f(mv) : __log2f(mv), -60.0f);
-            sm.rv[mb][h] = F32 ? __frcp_rn(mv) : __fdividef(1.0f, mv);
+            sm.m[mb].ks[h] = mk;
+            sm.m[mb].vs[h] = mv;
+            sm.m[mb].lv[h] = fmaxf(log2f(mv), -60.0f);
+            sm.m[mb].rv[h] = __frcp_rn(mv);
             const bool tame = __all_sync(0xFFFFFFFFu, mv > 0x1p-60f && mv < 0x1p60f);
             if (lane == 0) sm.tame[mb][warp - SW - 4] = tame;
             if constexpr (SHAPED) {
@@ -802,8 +922,8 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
                     see = see && (!docs || (sm.dmin == md && sm.dmax == md));
                     see = __all_sync(0xFFFFFFFFu, see);
                     if (lane == 0) sm.seen[mb][warp - SW - 4] = see;
-                    sm.pos[mb][h] = mp;
-                    sm.doc[mb][h] = md;
+                    sm.m[mb].pos[h] = mp;
+                    sm.m[mb].doc[h] = md;
                 }
             }
             mbar_arrive(&sm.meta_full[mb]);
@@ -858,7 +978,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
     } else {
         // ---- MMAs ----
         regs_down<RL::REGS_MMA>();
-        if (warp == SW + 8) {
+        if (warp == MW) {
             constexpr uint32_t id_qk = idesc(TK, false), id_pv = idesc(HD, true);
             const uint32_t lead = lane == 0, tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
             const int nt = __shfl_sync(0xFFFFFFFFu, n, 0), nw = __shfl_sync(0xFFFFFFFFu, two ? 2 : 1, 0);
@@ -938,13 +1058,56 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4>::THREADS, 1) k_kv8_prefi
             // nothing may be in flight when the TMEM goes
             umma_commit(&sm.drain, lead);
             mbar_wait(&sm.drain, 0, nullptr);
+        } else if (IMG && warp == MW + 1 && lane == 0) {
+            // ---- tile images to shared memory ----
+            const uint8_t *img = a.img + slot * IMAGE<HD>;
+            constexpr uint32_t HALF = TK * HD * 2;
+            const uint32_t meta_bytes = SHAPED ? sizeof(Meta) : 4 * TK * 4;
+            auto meta = [&](int j) {
+                const int t0 = tile_at(j), v = t0 / TK, mb = j & (META - 1);
+                const Kv8Head x = heads[v];
+                *reinterpret_cast<uint32_t *>(sm.tame[mb]) = x.tame ? 0x01010101u : 0u;
+                if (SHAPED && (docs || a.c.pos)) {
+                    const bool see = t0 + TK <= q.L && (!a.causal || x.pmax <= pmin) && (!a.window || (int64_t)pmax - x.pmin < a.window) &&
+                                     (!docs || (sm.dmin == x.dmin && sm.dmax == x.dmin && x.dmax == x.dmin));
+                    *reinterpret_cast<uint32_t *>(sm.seen[mb]) = see ? 0x01010101u : 0u;
+                }
+                mbar_expect(&sm.meta_full[mb], meta_bytes);
+                bulk_load(&sm.m[mb], img + (size_t)v * IMAGE<HD> + 2 * HALF, meta_bytes, &sm.meta_full[mb]);
+            };
+            if (n > 0) meta(0);
+            if (n > 1) meta(1);
+            bool ok = true;
+            int j = 0;
+#pragma unroll 1
+            for (; j < n; j++) {
+                const int b = j & 1;
+                const uint8_t *src = img + (size_t)(tile_at(j) / TK) * IMAGE<HD>;
+                if (j >= 2) ok = mbar_wait(&sm.k_empty[b], ((j >> 1) - 1) & 1, &sm.abort);
+                if (!ok) break;
+                mbar_expect(&sm.k_full[b], HALF);
+                bulk_load(sm.k[b], src, HALF, &sm.k_full[b]);
+                if (j >= 2) ok = mbar_wait(&sm.v_empty[b], ((j >> 1) - 1) & 1, &sm.abort);
+                if (!ok) break;
+                mbar_expect(&sm.v_full[b], HALF);
+                bulk_load(sm.v[b], src + HALF, HALF, &sm.v_full[b]);
+                // PV of tile j - 2 is done: its scales' buffer is free
+                if (j + 2 < n) meta(j + 2);
+            }
+            if (!ok) {   // nothing may be in flight when the shared memory goes
+                for (int i = max(j - 2, 0); i <= j; i++) {
+                    mbar_wait(&sm.k_full[i & 1], (i >> 1) & 1, nullptr);
+                    if (i < j) mbar_wait(&sm.v_full[i & 1], (i >> 1) & 1, nullptr);
+                }
+                for (int i = max(j - 2, 0); i < min(j + 2, n); i++) mbar_wait(&sm.meta_full[i & (META - 1)], (i / META) & 1, nullptr);
+            }
         }
     }
     __syncwarp();
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == SW + 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == MW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 bool smem_opt_in(const void *fn, size_t bytes) {
@@ -961,39 +1124,85 @@ bool smem_opt_in(const void *fn, size_t bytes) {
     return true;
 }
 
-template <int HD, int FMT, typename QT, bool SHAPED> int launch_shape(const Kv8Attn &a, cudaStream_t st) {
-    auto fn = k_kv8_prefill<HD, FMT, QT, SHAPED>;
+// Key tiles of a sequence, and (sequence, KV head) pairs whose images one launch holds; 0 pairs: converting warps. Images
+// pay where enough query tiles share them (IMG_TILES below); above IMG_BYTES the pairs go in turns, each of which has to
+// fill the SMs twice.
+constexpr int IMG_TILES = 4;
+constexpr size_t IMG_BYTES = (size_t)256 << 20;
+struct Images {
+    int n_img, n_seq, n_kv;   // sequences and KV heads of a launch
+    size_t bytes;
+};
+Images images(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt) {
+    Images r{};
+    const int64_t rows = q_dt == TLMG_DT_F32 ? TQ : 2 * TQ, tiles = ((int64_t)b.max_q * (H / c.KV) + rows - 1) / rows;
+    if (tiles < IMG_TILES) return r;
+    r.n_img = (b.max_kv + TK - 1) / TK;
+    const size_t one = (size_t)r.n_img * ((c.hd == 64 ? IMAGE<64> : IMAGE<128>) + sizeof(Kv8Head));
+    const int64_t fit = std::max<int64_t>(1, (int64_t)(IMG_BYTES / std::max<size_t>(one, 1)));
+    if (fit >= c.KV) r.n_kv = c.KV, r.n_seq = (int)std::min<int64_t>(b.n_seq, fit / c.KV);
+    else r.n_kv = (int)fit, r.n_seq = 1;
+    const bool all = r.n_kv == c.KV && r.n_seq == b.n_seq;
+    if (!all && r.n_kv * r.n_seq * tiles < 2 * sm_count()) return Images{};
+    r.bytes = (size_t)r.n_kv * r.n_seq * one;
+    return r;
+}
+
+template <int HD, int FMT, typename QT, bool SHAPED, bool IMG> int launch_shape(const Kv8Attn &a, dim3 grid, cudaStream_t st) {
+    auto fn = k_kv8_prefill<HD, FMT, QT, SHAPED, IMG>;
     constexpr size_t bytes = sizeof(Smem<HD>);
     static_assert(bytes <= 227 * 1024, "shared memory");
     if (!smem_opt_in((const void *)fn, bytes)) return set_error(TLMG_EIO, "kv8_attend: shared memory opt-in failed");
-    using RL = Role<sizeof(QT) == 4>;
-    constexpr int rows = RL::TILES * TQ;
-    const int64_t tiles = ((int64_t)a.b.max_q * a.G + rows - 1) / rows;
-    fn<<<dim3((unsigned)(tiles * a.c.KV), a.b.n_seq), RL::THREADS, bytes, st>>>(a);
+    fn<<<grid, Role<sizeof(QT) == 4, IMG>::THREADS, bytes, st>>>(a);
     count_launch();
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? TLMG_OK : cuda_fail(e, "kv8_attend launch");
 }
-template <int HD, int FMT, typename QT> int launch(const Kv8Attn &a, cudaStream_t st) {
-    return a.softcap > 0.0f || a.slopes || a.doc || a.c.pos ? launch_shape<HD, FMT, QT, true>(a, st) : launch_shape<HD, FMT, QT, false>(a, st);
+template <int HD, int FMT, typename QT> int launch(const Kv8Attn &a0, void *work, cudaStream_t st) {
+    Kv8Attn a = a0;
+    const bool shaped = a.softcap > 0.0f || a.slopes || a.doc || a.c.pos;
+    constexpr int rows = Role<sizeof(QT) == 4, true>::TILES * TQ;
+    const unsigned tiles = (unsigned)(((int64_t)a.b.max_q * a.G + rows - 1) / rows);
+    const Images im = images(a.kv8, a.b, a.H, sizeof(QT) == 4 ? TLMG_DT_F32 : TLMG_DT_F16);
+    if (!im.n_kv) {
+        const dim3 grid(tiles * a.c.KV, a.b.n_seq);
+        return shaped ? launch_shape<HD, FMT, QT, true, false>(a, grid, st) : launch_shape<HD, FMT, QT, false, false>(a, grid, st);
+    }
+    a.unit = kv8_f16_unit<FMT>();
+    a.n_img = im.n_img;
+    a.img = static_cast<uint8_t *>(work);
+    a.heads = a.img + (size_t)im.n_kv * im.n_seq * im.n_img * IMAGE<HD>;
+    for (a.s0 = 0; a.s0 < a.b.n_seq; a.s0 += im.n_seq)
+        for (a.kv0 = 0; a.kv0 < a.c.KV; a.kv0 += im.n_kv) {
+            const int ns = std::min(im.n_seq, a.b.n_seq - a.s0);
+            a.nkv = std::min(im.n_kv, a.c.KV - a.kv0);
+            k_kv8_images<HD, FMT><<<dim3(im.n_img, a.nkv, ns), 256, 0, st>>>(a);
+            count_launch();
+            const dim3 grid(tiles * a.nkv, ns);
+            const int rc = shaped ? launch_shape<HD, TLMG_KV8_INT8, QT, true, true>(a, grid, st)
+                                  : launch_shape<HD, TLMG_KV8_INT8, QT, false, true>(a, grid, st);
+            if (rc) return rc;
+        }
+    return TLMG_OK;
 }
-template <int HD, int FMT> int launch_q(const Kv8Attn &a, int q_dt, cudaStream_t st) {
-    if (q_dt == TLMG_DT_F32) return launch<HD, FMT, float>(a, st);
-    return q_dt == TLMG_DT_F16 ? launch<HD, FMT, __half>(a, st) : launch<HD, FMT, __nv_bfloat16>(a, st);
+template <int HD, int FMT> int launch_q(const Kv8Attn &a, int q_dt, void *work, cudaStream_t st) {
+    if (q_dt == TLMG_DT_F32) return launch<HD, FMT, float>(a, work, st);
+    return q_dt == TLMG_DT_F16 ? launch<HD, FMT, __half>(a, work, st) : launch<HD, FMT, __nv_bfloat16>(a, work, st);
 }
-template <int HD> int launch_fmt(const Kv8Attn &a, int fmt, int q_dt, cudaStream_t st) {
-    return fmt == TLMG_KV8_INT8 ? launch_q<HD, TLMG_KV8_INT8>(a, q_dt, st) : launch_q<HD, TLMG_KV8_E4M3>(a, q_dt, st);
+template <int HD> int launch_fmt(const Kv8Attn &a, int q_dt, void *work, cudaStream_t st) {
+    return a.kv8.fmt == TLMG_KV8_INT8 ? launch_q<HD, TLMG_KV8_INT8>(a, q_dt, work, st) : launch_q<HD, TLMG_KV8_E4M3>(a, q_dt, work, st);
 }
 
 }  // namespace
 
-bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt) {
-    (void)q_dt;
+bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H) {
     return c.hd <= 128 && (int64_t)b.max_q * (H / c.KV) >= TQ;
 }
 
-int kv8_prefill(const Kv8Attn &a, int fmt, int q_dt, cudaStream_t st) {
-    return a.c.hd == 64 ? launch_fmt<64>(a, fmt, q_dt, st) : launch_fmt<128>(a, fmt, q_dt, st);
+size_t kv8_prefill_work_bytes(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt) { return images(c, b, H, q_dt).bytes; }
+
+int kv8_prefill(const Kv8Attn &a, int q_dt, void *work, cudaStream_t st) {
+    return a.c.hd == 64 ? launch_fmt<64>(a, q_dt, work, st) : launch_fmt<128>(a, q_dt, work, st);
 }
 
 }  // namespace tlmg
