@@ -273,6 +273,7 @@ __device__ __forceinline__ float cap_exp(float y, float capl) {
 }
 
 constexpr float TOP = 14.0f;   // log2 of the largest p * v_scale right after a row's reference moved
+constexpr float GROW = 1.9f;   // how far it may grow before the reference moves again: 2^15.9 is an f16 (65,504 its largest)
 
 // Smallest and largest position of a sequence's tokens (by all threads of the CTA).
 __device__ __forceinline__ void token_span(const Kv8Attn &a, const Kv8Seq &q, int *mm, int &pmin, int &pmax) {
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                 ok = mbar_wait_warp(&sm.x_full[w], j & 1, &sm.abort);
                 if (!ok) break;
                 m0 = fmaxf(m0, sm.part[w][half ^ 1][r]);
-                const bool grow = m0 > wref + 1.0f;
+                const bool grow = m0 > wref + GROW;
                 float fnew = 1.0f;
                 if (__any_sync(0xFFFFFFFFu, grow)) {
                     const float f = grow && wref != -INFINITY ? ex2(wref - m0) : 1.0f;
@@ -979,6 +980,8 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
         // ---- MMAs ----
         regs_down<RL::REGS_MMA>();
         if (warp == MW) {
+            // One warp for both query tiles: with a warp each the tiles' phases drift together, and the tensor core and the
+            // softmax warps wait for each other in turn (18k chunk without cap 902 us, in turn 739).
             constexpr uint32_t id_qk = idesc(TK, false), id_pv = idesc(HD, true);
             const uint32_t lead = lane == 0, tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
             const int nt = __shfl_sync(0xFFFFFFFFu, n, 0), nw = __shfl_sync(0xFFFFFFFFu, two ? 2 : 1, 0);
@@ -1037,17 +1040,17 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
             }
 #pragma unroll 1
             for (int j = 0; !F32 && ok && j < nt; j++) {
+                // V of this tile and K of the next are there long before the weights: those waits come first, once
+                ok = mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, &sm.abort) &&
+                     (j + 1 == nt || mbar_wait(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, &sm.abort));
 #pragma unroll 1
                 for (int w = 0; ok && w < nw; w++) {
-                    ok = mbar_wait(&sm.p_full[w], j & 1, &sm.abort) && mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, &sm.abort);
+                    ok = mbar_wait(&sm.p_full[w], j & 1, &sm.abort);
                     if (!ok) break;
                     tc_after();
                     pv(w, j);
                     if (w == nw - 1) umma_commit(&sm.v_empty[j & 1], lead);
                     if (j + 1 < nt) {
-                        ok = mbar_wait(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, &sm.abort);
-                        if (!ok) break;
-                        tc_after();
                         qk(w, j + 1);
                         if (w == nw - 1) umma_commit(&sm.k_empty[(j + 1) & 1], lead);
                     } else {
