@@ -49,7 +49,6 @@ namespace {
 
 constexpr int TK = 128;           // keys of a tile
 constexpr int TQ = 128;           // query rows of a tile
-constexpr int CK = 16;            // columns of a round of the softmax loops: few registers, four warps a scheduler
 constexpr int HC = TK / 2;        // keys of a softmax thread: two threads share a query row
 constexpr int CV = 256;           // converting threads
 // What differs between 16-bit queries (two query tiles in turn) and f32 ones (one tile of which every operand but K and V
@@ -96,7 +95,7 @@ template <int HD> struct Smem {
     alignas(4) uint8_t tame[META][4], seen[META][4];
     uint32_t row[2][TK];
     float qs[2][TQ], part[2][2][TQ], sums[2][2][TQ];     // [tile][half][row]: the halves' maxima; in the end their sums
-    uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], x_full[2], o_full[2], meta_full[META], drain;
+    uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], p_half[2], x_full[2], o_full[2], meta_full[META], drain;
     uint32_t tmem;
     int abort, pmin, pmax, dmin, dmax, n_list;
     uint16_t list[LIST];      // the key tiles that hold a key which a query may see
@@ -216,6 +215,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
                  "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ldc(uint32_t a, uint32_t (&v)[32]) { tmem_ld32(a, v); }
+__device__ __forceinline__ void tmem_stc(uint32_t a, const uint32_t (&v)[8]) { tmem_st8(a, v); }
+__device__ __forceinline__ void tmem_stc(uint32_t a, const uint32_t (&v)[16]) { tmem_st16(a, v); }
+__device__ __forceinline__ void tmem_stc(uint32_t a, const uint32_t (&v)[32]) { tmem_st32(a, v); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void mbar_expect(uint64_t *b, uint32_t bytes) {
@@ -412,6 +415,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
             mbar_init(&sm.v_empty[i], 1);
             mbar_init(&sm.s_full[i], 1);
             mbar_init(&sm.p_full[i], 2 * TQ);
+            mbar_init(&sm.p_half[i], 2 * TQ);
             mbar_init(&sm.x_full[i], 2 * TQ);
             mbar_init(&sm.o_full[i], 1);
         }
@@ -589,6 +593,8 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
 #pragma unroll
                 for (int i = 0; i < HD / 2; i++) o[i] = 0.0f;
             }
+            // columns of a round of these loops: as many as the registers take (18k chunk without cap: 16 columns 702 us, 32 676)
+            constexpr int CK = IMG && !F32 ? 32 : 16;
 #pragma unroll 1
             for (int j = 0; ok && j < n; j++) {
                 const int t0 = tile_at(j), mb = j & (META - 1);
@@ -638,7 +644,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                         for (int g = 0; g < CK; g += 8) {
                             const float k = ks[c + g] * mul;
 #pragma unroll
-                            for (int i = 0; i < 8; i++) z[g + i] = __uint_as_float(xa[g + i]) * k;
+                            for (int i = 0; i < 8; i += 2) upk(mul2(pku(xa[g + i], xa[g + i + 1]), pk(k, k)), z[g + i], z[g + i + 1]);
                         }
                         if (cap) {
                             float big = 0.0f;
@@ -695,14 +701,12 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                         }
 #pragma unroll
                         for (int g = 0; g < CK; g += 8) {
-                            float y = z[g], y1 = z[g + 1];
-#pragma unroll
-                            for (int i = 2; i < 8; i += 2) y = fmaxf(y, z[g + i]), y1 = fmaxf(y1, z[g + i + 1]);
-                            m0 = fmaxf(m0, fmaxf(y, y1) + lv[c + g]);
+                            const float y = fmaxf(fmaxf(z[g], z[g + 1]), z[g + 2]), y1 = fmaxf(fmaxf(z[g + 3], z[g + 4]), z[g + 5]);
+                            m0 = fmaxf(m0, fmaxf(fmaxf(fmaxf(y, y1), z[g + 6]), z[g + 7]) + lv[c + g]);
                         }
 #pragma unroll
                         for (int i = 0; i < CK; i++) xa[i] = __float_as_uint(z[i]);
-                        tmem_st16(ts + c, xa);
+                        tmem_stc(ts + c, xa);
                     }
                     tmem_wait_st();
                 } else {
@@ -746,7 +750,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                             tmem_ldc(to + c, xa);
 #pragma unroll
                             for (int i = 0; i < CK; i++) xa[i] = __float_as_uint(__uint_as_float(xa[i]) * f);
-                            tmem_st16(to + c, xa);
+                            tmem_stc(to + c, xa);
                         }
                         tmem_wait_st();
                     }
@@ -775,12 +779,17 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                             lsum = __fmaf_rn(u0 + u1, sm.m[mb].rv[c + g], lsum);
                         }
                         if constexpr (F32) {   // high parts and remainders of 16 keys over their 16 scores
-                            tmem_st8(ts + c, p);
+                            tmem_stc(ts + c, p);
 #pragma unroll
                             for (int i = 0; i < CK / 2; i++) p[i] = xa[i];
-                            tmem_st8(ts + c + 8, p);
+                            tmem_stc(ts + c + 8, p);
                         } else {
-                            tmem_st8(ts + (c + k0) / 2, p);   // columns whose scores are read already
+                            tmem_stc(ts + (c + k0) / 2, p);   // columns whose scores are read already
+                            if (c == k0 + HC / 2 - CK) {        // the first half of these weights: their product can start
+                                tmem_wait_st();
+                                tc_before();
+                                mbar_arrive(&sm.p_half[w]);
+                            }
                         }
                     }
                 } else if constexpr (F32) {
@@ -796,10 +805,10 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                             p[i / 2] = pack_f16(u0, u1);
                             xa[i / 2] = rest_f16(u0, u1, p[i / 2], 0x1p11f);
                         }
-                        tmem_st8(ts + c, p);
+                        tmem_stc(ts + c, p);
 #pragma unroll
                         for (int i = 0; i < CK / 2; i++) p[i] = xa[i];
-                        tmem_st8(ts + c + 8, p);
+                        tmem_stc(ts + c + 8, p);
                     }
                 } else {
 #pragma unroll 1
@@ -817,6 +826,9 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                         p[1] = pack_f16(__uint_as_float(x[2]), __uint_as_float(x[3]));
                         tmem_st2(ts + (c + k0) / 2, p);
                     }
+                    tmem_wait_st();
+                    tc_before();
+                    mbar_arrive(&sm.p_half[w]);
                 }
                 tmem_wait_st();
                 if constexpr (F32) {   // the last tile's product: the next one starts over it
@@ -1000,7 +1012,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                 }
                 umma_commit(&sm.s_full[sb], lead);
             };
-            auto pv = [&](int w, int j) {
+            auto pv = [&](int w, int j, int part) {
                 const uint64_t va = dv + (j & 1) * BUF;
                 if constexpr (F32) {
 #pragma unroll
@@ -1010,8 +1022,10 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                             umma_ts(tm + 2 * TK + part * HD, tm + (j & 1) * TK + 16 * k + 8 * part, va + 2 * SBO / 16 * k, id_pv, k > 0, lead);
                 } else {
 #pragma unroll
-                    for (int k = 0; k < TK / 16; k++)
-                        umma_ts(tm + 2 * TK + w * HD, tm + w * TK + 8 * k + (k >= HC / 16 ? HC / 2 : 0), va + 2 * SBO / 16 * k, id_pv, j > 0 || k > 0, lead);
+                    for (int i = 0; i < TK / 32; i++) {
+                        const int k = (i & 1) + (i & 2) * 2, kk = k + 2 * part;
+                        umma_ts(tm + 2 * TK + w * HD, tm + w * TK + 8 * kk + (k >= HC / 16 ? HC / 2 : 0), va + 2 * SBO / 16 * kk, id_pv, j > 0 || part > 0 || i > 0, lead);
+                    }
                 }
             };
             bool ok = nt == 0 || (mbar_wait(&sm.q_full, 0, &sm.abort) && mbar_wait(&sm.k_full[0], 0, &sm.abort));
@@ -1033,7 +1047,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                     ok = mbar_wait(&sm.p_full[0], j & 1, &sm.abort) && mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, &sm.abort);
                     if (!ok) break;
                     tc_after();
-                    pv(0, j);
+                    pv(0, j, 0);
                     umma_commit(&sm.o_full[0], lead);
                     umma_commit(&sm.v_empty[j & 1], lead);
                 }
@@ -1045,10 +1059,14 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                      (j + 1 == nt || mbar_wait(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, &sm.abort));
 #pragma unroll 1
                 for (int w = 0; ok && w < nw; w++) {
+                    ok = mbar_wait(&sm.p_half[w], j & 1, &sm.abort);
+                    if (!ok) break;
+                    tc_after();
+                    pv(w, j, 0);
                     ok = mbar_wait(&sm.p_full[w], j & 1, &sm.abort);
                     if (!ok) break;
                     tc_after();
-                    pv(w, j);
+                    pv(w, j, 1);
                     if (w == nw - 1) umma_commit(&sm.v_empty[j & 1], lead);
                     if (j + 1 < nt) {
                         qk(w, j + 1);
