@@ -588,6 +588,21 @@ def test_prefill_loose_bounds(max_q, max_kv, dtype):
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("news", [[40, 33], [200, 7]])
+@pytest.mark.parametrize("name", ["plain", "window", "sinks", "doc", "cap", "both_ways"])
+def test_prefill_pieces(name, news, dtype):
+    """Few query tiles over many rows: the keys go in pieces that are joined, some of them without a visible key."""
+    lens, H, KV, hd = [2600, 1100], 12, 2, 64
+    host, table, q_start, q, rng = make(36, lens, news, H, KV, hd, K.INT8, 64, 16, dtype=dtype)
+    doc = np.zeros((2, max(lens)), np.int32)
+    doc[:, 900:], doc[0, 2480:] = 1, 2
+    mods = {"plain": {}, "window": dict(window=700), "sinks": dict(window=150, prefix=np.array([600, 20], np.int32)), "doc": dict(doc=doc),
+            "cap": dict(softcap=3.0), "both_ways": dict(causal=False)}[name]
+    check_attend(host, table, q_start, lens, q, H, **mods)
+
+
 def mods_of(name, rng, lens, H):
     n = len(lens)
     doc = np.full((n, max(lens)), -1, np.int32)

@@ -712,7 +712,7 @@ Split split_plan(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_scor
     const int G = H / c.KV;
     p.wide = !weights && kv8_prefill_serves(c, b, H);
     if (p.wide) {
-        p.total = kv8_prefill_work_bytes(c, b, H, q_dt) + 16;
+        p.total = kv8_prefill_work_bytes(c, b, s, H, q_dt) + 16;
         return p;
     }
     // 16 query rows a CTA where there are more than 8 (not for f32 ones of 256 dims: no registers)

@@ -31,6 +31,8 @@ struct Kv8Attn {
     uint8_t *img, *heads;
     int s0, kv0, nkv, n_img;
     float unit;
+    // its items: query tiles of a sequence and head; the items from n_full on go in pieces
+    int q_tiles, n_full, pieces;
 };
 
 // tanh(x) = x (c0 + c1 x^2 + .. + c5 x^10) for |x| < TANH_X within 2e-7: fitted (reweighted least squares towards the
@@ -98,7 +100,7 @@ inline int sm_count() {
 
 // The form for many query rows (tlmg_kv8_prefill.cu): whether it serves a call, its workspace, and the call.
 bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H);
-size_t kv8_prefill_work_bytes(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt);
+size_t kv8_prefill_work_bytes(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_score &s, int H, int q_dt);
 int kv8_prefill(const Kv8Attn &a, int q_dt, void *work, cudaStream_t st);
 
 }  // namespace tlmg

@@ -278,6 +278,53 @@ __device__ __forceinline__ float cap_exp(float y, float capl) {
 constexpr float TOP = 14.0f;   // log2 of the largest p * v_scale right after a row's reference moved
 constexpr float GROW = 1.9f;   // how far it may grow before the reference moves again: 2^15.9 is an f16 (65,504 its largest)
 
+// The CTAs' work: one item a query tile and KV head, last tokens first since they see the most keys; the items from a.n_full
+// on are cut along the keys.
+struct Kv8Item {
+    int s, kvh, rt, piece, pieces;
+};
+__device__ __forceinline__ Kv8Item kv8_item(const Kv8Attn &a, int b) {
+    Kv8Item r;
+    r.pieces = b < a.n_full ? 1 : a.pieces;
+    r.piece = b < a.n_full ? 0 : (b - a.n_full) % a.pieces;
+    const int i = b < a.n_full ? b : a.n_full + (b - a.n_full) / a.pieces, per = a.q_tiles * a.nkv, x = i % per;
+    r.s = a.s0 + i / per;
+    r.kvh = a.kv0 + x % a.nkv;
+    r.rt = a.q_tiles - 1 - x / a.nkv;
+    return r;
+}
+
+// Joins the pieces: out = sum_p o_p 2^(w_p - W) / sum_p l_p 2^(w_p - W), W the largest reference; one warp a query row.
+template <int HD, typename QT>
+__global__ void __launch_bounds__(256) k_kv8_pieces(const __grid_constant__ Kv8Attn a) {
+    constexpr int RPC = Role<sizeof(QT) == 4, true>::TILES * TQ;
+    const int lane = threadIdx.x & 31, t = blockIdx.x / (RPC / 8), r = blockIdx.x % (RPC / 8) * 8 + (threadIdx.x >> 5);
+    const Kv8Item it = kv8_item(a, a.n_full + t * a.pieces);
+    Kv8Seq q;
+    const int R = it.rt * RPC + r;
+    if (!kv8_seq(a.b, a.c.lp, it.s, q) || R >= q.n * a.G) return;     // (a bad sequence's rows are NaN already)
+    const int64_t row = (q.q0 + (int64_t)(R / a.G)) * a.H + it.kvh * a.G + R % a.G;
+    const size_t p0 = (size_t)t * a.pieces * RPC + r;
+    float W = -INFINITY, L = 0.0f;
+    for (int p = 0; p < a.pieces; p++) W = fmaxf(W, a.pm[p0 + (size_t)p * RPC]);
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = 0; p < a.pieces; p++) {
+        const size_t at = p0 + (size_t)p * RPC;
+        const float w = a.pm[at], l = a.pl[at];
+        if (w == -INFINITY && l == 0.0f) continue;                 // no visible keys
+        const float f = w == -INFINITY ? 1.0f : ex2(w - W);        // -inf with a sum: a NaN, which stays
+        L = __fmaf_rn(l, f, L);
+        if (lane < HD / 4) {
+            const float4 u = *reinterpret_cast<const float4 *>(a.po + at * HD + 4 * lane);
+            v = make_float4(__fmaf_rn(u.x, f, v.x), __fmaf_rn(u.y, f, v.y), __fmaf_rn(u.z, f, v.z), __fmaf_rn(u.w, f, v.w));
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+    if (lane < HD / 4)
+        kv8_st4(static_cast<QT *>(a.out) + row * HD + 4 * lane, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    if (lane == 0 && a.lse) a.lse[row] = L == 0.0f ? -INFINITY : (log2f(L) - (W == -INFINITY ? 0.0f : TOP - W)) * LN2;
+}
+
 // Smallest and largest position of a sequence's tokens (by all threads of the CTA).
 __device__ __forceinline__ void token_span(const Kv8Attn &a, const Kv8Seq &q, int *mm, int &pmin, int &pmax) {
     pmin = q.L - q.n, pmax = q.L - 1;
@@ -378,10 +425,10 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
     constexpr int PC = HD / 16;               // 16-byte pieces of a code row
     constexpr int NP = TK * PC / CV;          // pieces of half a tile per converting thread
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int nkv = IMG ? a.nkv : a.c.KV, s = (IMG ? a.s0 : 0) + blockIdx.y, kvh = (IMG ? a.kv0 : 0) + blockIdx.x % nkv;
-    const int tiles = gridDim.x / nkv, rt = tiles - 1 - blockIdx.x / nkv;   // the last tokens see the most keys: first
+    const Kv8Item it = kv8_item(a, blockIdx.x);
+    const int s = it.s, kvh = it.kvh, tiles = a.q_tiles, rt = it.rt;
     const float unit = IMG ? a.unit : kv8_f16_unit<FMT>();
-    const size_t slot = IMG ? ((size_t)blockIdx.y * nkv + blockIdx.x % nkv) * a.n_img : 0;
+    const size_t slot = IMG ? ((size_t)(s - a.s0) * a.nkv + kvh - a.kv0) * a.n_img : 0;
     const Kv8Head *heads = reinterpret_cast<const Kv8Head *>(a.heads) + slot;
     QT *out = static_cast<QT *>(a.out);
     Kv8Seq q;
@@ -502,7 +549,10 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
             n = sm.n_list;
         }
     }
-    auto tile_at = [&](int j) { return rg.t0(SHAPED && listed ? (int)sm.list[j] : j); };
+    // a piece takes its share of the tiles
+    const int first = (int)((int64_t)n * it.piece / it.pieces);
+    n = (int)((int64_t)n * (it.piece + 1) / it.pieces) - first;
+    auto tile_at = [&](int j) { return rg.t0(SHAPED && listed ? (int)sm.list[first + j] : first + j); };
 
     if (warp < SW) {
         // ---- softmax of one query tile ----
@@ -851,13 +901,16 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                 l = lsum + sm.sums[w][half ^ 1][r];
             }
             tc_after();
-            const float inv = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? 0.0f : __fdividef(unit, l);
+            const bool part = it.pieces > 1;     // the sums go to the workspace, for the join
+            const float inv = !ok ? __uint_as_float(0x7FC00000u) : part ? unit : l == 0.0f ? 0.0f : __fdividef(unit, l);
+            const size_t prow = part ? ((size_t)(blockIdx.x - a.n_full) * RPC + w * TQ + r) : 0;
             if constexpr (F32) {
                 if (ok && n > 0) add_o();
+                float *dst = part ? a.po + prow * HD : reinterpret_cast<float *>(out) + orow * HD;
                 if (live)
 #pragma unroll
                     for (int i = 0; i < HD / 2; i += 4)
-                        kv8_st4(out + orow * HD + half * (HD / 2) + i, make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
+                        kv8_st4(dst + half * (HD / 2) + i, make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
             }
 #pragma unroll 1
             for (int c = half * (HD / 2); !F32 && c < (half + 1) * (HD / 2); c += 32) {
@@ -868,7 +921,12 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
 #pragma unroll
                     for (int i = 0; i < 32; i++) x[i] = 0;
                 }
-                if (live)
+                if (live && part) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        kv8_st4(a.po + prow * HD + c + i, make_float4(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv,
+                                                                      __uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv));
+                } else if (live) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
                         uint4 o;
@@ -878,8 +936,12 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                                                                             __uint_as_float(x[i + 6]) * inv, __uint_as_float(x[i + 7]) * inv));
                         *reinterpret_cast<uint4 *>(out + orow * HD + c + i) = o;
                     }
+                }
             }
-            if (live && half == 0 && a.lse)
+            if (live && half == 0 && part) {
+                a.pm[prow] = wref;
+                a.pl[prow] = ok ? l : __uint_as_float(0x7FC00000u);
+            } else if (live && half == 0 && a.lse)
                 a.lse[orow] = !ok ? __uint_as_float(0x7FC00000u) : l == 0.0f ? -INFINITY : (log2f(l) - (wref == -INFINITY ? 0.0f : TOP - wref)) * LN2;
         }
     } else if (!IMG && warp < MW) {
@@ -1169,7 +1231,33 @@ Images images(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt) {
     return r;
 }
 
-template <int HD, int FMT, typename QT, bool SHAPED, bool IMG> int launch_shape(const Kv8Attn &a, dim3 grid, cudaStream_t st) {
+// Items on the SMs: whole rounds of them as they are, the rest (all of them where they leave SMs idle) cut along the keys
+// into pieces of PIECE tiles or more. In units of a tile's time (2.4 us) a CTA's start and end cost about 5, the join 3 and
+// what a piece writes and the join reads 1 / 50. Beyond ROUNDS rounds the last one is too small a part. Without and with
+// pieces: 18k chunk (256 items, 108 of them in 4 pieces) 1,073 and 1,028 us, 65,536 rows 2,344 and 2,071, 32 tokens of 32
+// heads on 4 over 131,072 rows (4 items in 37) 159 with.
+constexpr int ROUNDS = 8, PIECE = 4;
+struct Tail {
+    int n_full, pieces, n_tail;
+};
+Tail tail_plan(const tlmg_kv8 &c, const tlmg_kv8_batch &b, bool causal, int window, int64_t items, int rows) {
+    const int64_t sms = sm_count(), full = items / sms * sms, left = items - full;
+    Tail r{ (int)items, 1, 0 };
+    if (full > ROUNDS * sms || left == 0) return r;
+    // key tiles of such an item: its tokens are among the first ones where whole rounds came before
+    int64_t keys = b.max_kv;
+    if (causal) keys = std::max<int64_t>(b.max_kv - b.max_q, 0) + (full ? b.max_q * left / items : b.max_q / 2);
+    if (window > 0 && causal && !c.pos) keys = std::min<int64_t>(keys, (int64_t)window + rows);
+    const int64_t kt = std::max<int64_t>(1, keys / TK);
+    int64_t best = kt + 5;
+    for (int64_t s = 2; s <= kt / PIECE && left * s <= 4 * sms; s++) {
+        const int64_t cost = (left * s + sms - 1) / sms * ((kt + s - 1) / s + 5) + 3 + left * s / 50;
+        if (cost < best) best = cost, r = { (int)full, (int)s, (int)left };
+    }
+    return r;
+}
+
+template <int HD, int FMT, typename QT, bool SHAPED, bool IMG> int launch_shape(const Kv8Attn &a, unsigned grid, cudaStream_t st) {
     auto fn = k_kv8_prefill<HD, FMT, QT, SHAPED, IMG>;
     constexpr size_t bytes = sizeof(Smem<HD>);
     static_assert(bytes <= 227 * 1024, "shared memory");
@@ -1179,32 +1267,70 @@ template <int HD, int FMT, typename QT, bool SHAPED, bool IMG> int launch_shape(
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? TLMG_OK : cuda_fail(e, "kv8_attend launch");
 }
+// What a call does, from its sizes alone: workspace = images, then the pieces' outputs, references and sums.
+struct Wide {
+    Images im;
+    Tail tail;
+    int q_tiles;
+    size_t part, bytes;   // rows of partial results
+};
+Wide wide_plan(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt, bool causal, int window) {
+    Wide p;
+    p.im = images(c, b, H, q_dt);
+    const int rows = q_dt == TLMG_DT_F32 ? TQ : 2 * TQ;
+    p.q_tiles = (int)(((int64_t)b.max_q * (H / c.KV) + rows - 1) / rows);
+    const int64_t items = (int64_t)p.q_tiles * c.KV * b.n_seq;
+    p.tail = Tail{ (int)std::min<int64_t>(items, INT32_MAX), 1, 0 };
+    if (!p.im.n_kv || (p.im.n_kv == c.KV && p.im.n_seq == b.n_seq)) p.tail = tail_plan(c, b, causal, window, items, rows);
+    p.part = (size_t)p.tail.n_tail * p.tail.pieces * rows;
+    p.bytes = p.im.bytes + p.part * (c.hd + 2) * 4;
+    return p;
+}
+
 template <int HD, int FMT, typename QT> int launch(const Kv8Attn &a0, void *work, cudaStream_t st) {
     Kv8Attn a = a0;
     const bool shaped = a.softcap > 0.0f || a.slopes || a.doc || a.c.pos;
-    constexpr int rows = Role<sizeof(QT) == 4, true>::TILES * TQ;
-    const unsigned tiles = (unsigned)(((int64_t)a.b.max_q * a.G + rows - 1) / rows);
-    const Images im = images(a.kv8, a.b, a.H, sizeof(QT) == 4 ? TLMG_DT_F32 : TLMG_DT_F16);
+    const Wide p = wide_plan(a.kv8, a.b, a.H, sizeof(QT) == 4 ? TLMG_DT_F32 : TLMG_DT_F16, a.causal, a.window);
+    const Images &im = p.im;
+    if ((int64_t)p.q_tiles * a.c.KV * a.b.n_seq > INT32_MAX)
+        return set_error(TLMG_ERANGE, "kv8_attend: %d sequences of %d KV heads and %d tokens are too many for a call", a.b.n_seq, a.c.KV, a.b.max_q);
+    a.q_tiles = p.q_tiles;
+    a.pieces = p.tail.pieces;
+    a.po = reinterpret_cast<float *>(static_cast<uint8_t *>(work) + im.bytes);
+    a.pm = a.po + p.part * HD;
+    a.pl = a.pm + p.part;
+    a.s0 = a.kv0 = 0;
+    int rc = TLMG_OK;
     if (!im.n_kv) {
-        const dim3 grid(tiles * a.c.KV, a.b.n_seq);
-        return shaped ? launch_shape<HD, FMT, QT, true, false>(a, grid, st) : launch_shape<HD, FMT, QT, false, false>(a, grid, st);
+        a.nkv = a.c.KV;
+        a.n_full = p.tail.n_full;
+        const unsigned grid = (unsigned)(a.n_full + p.tail.n_tail * a.pieces);
+        rc = shaped ? launch_shape<HD, FMT, QT, true, false>(a, grid, st) : launch_shape<HD, FMT, QT, false, false>(a, grid, st);
+    } else {
+        a.unit = kv8_f16_unit<FMT>();
+        a.n_img = im.n_img;
+        a.img = static_cast<uint8_t *>(work);
+        a.heads = a.img + (size_t)im.n_kv * im.n_seq * im.n_img * IMAGE<HD>;
+        for (a.s0 = 0; !rc && a.s0 < a.b.n_seq; a.s0 += im.n_seq)
+            for (a.kv0 = 0; !rc && a.kv0 < a.c.KV; a.kv0 += im.n_kv) {
+                const int ns = std::min(im.n_seq, a.b.n_seq - a.s0);
+                a.nkv = std::min(im.n_kv, a.c.KV - a.kv0);
+                k_kv8_images<HD, FMT><<<dim3(im.n_img, a.nkv, ns), 256, 0, st>>>(a);
+                count_launch();
+                a.n_full = p.tail.n_tail ? p.tail.n_full : a.q_tiles * a.nkv * ns;
+                const unsigned grid = (unsigned)(a.n_full + p.tail.n_tail * a.pieces);
+                rc = shaped ? launch_shape<HD, TLMG_KV8_INT8, QT, true, true>(a, grid, st)
+                            : launch_shape<HD, TLMG_KV8_INT8, QT, false, true>(a, grid, st);
+            }
+        a.s0 = a.kv0 = 0;
     }
-    a.unit = kv8_f16_unit<FMT>();
-    a.n_img = im.n_img;
-    a.img = static_cast<uint8_t *>(work);
-    a.heads = a.img + (size_t)im.n_kv * im.n_seq * im.n_img * IMAGE<HD>;
-    for (a.s0 = 0; a.s0 < a.b.n_seq; a.s0 += im.n_seq)
-        for (a.kv0 = 0; a.kv0 < a.c.KV; a.kv0 += im.n_kv) {
-            const int ns = std::min(im.n_seq, a.b.n_seq - a.s0);
-            a.nkv = std::min(im.n_kv, a.c.KV - a.kv0);
-            k_kv8_images<HD, FMT><<<dim3(im.n_img, a.nkv, ns), 256, 0, st>>>(a);
-            count_launch();
-            const dim3 grid(tiles * a.nkv, ns);
-            const int rc = shaped ? launch_shape<HD, TLMG_KV8_INT8, QT, true, true>(a, grid, st)
-                                  : launch_shape<HD, TLMG_KV8_INT8, QT, false, true>(a, grid, st);
-            if (rc) return rc;
-        }
-    return TLMG_OK;
+    if (rc || !p.tail.n_tail) return rc;
+    constexpr int rows = Role<sizeof(QT) == 4, true>::TILES * TQ;
+    a.nkv = a.c.KV;
+    k_kv8_pieces<HD, QT><<<p.tail.n_tail * (rows / 8), 256, 0, st>>>(a);
+    count_launch();
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? TLMG_OK : cuda_fail(e, "kv8_attend launch");
 }
 template <int HD, int FMT> int launch_q(const Kv8Attn &a, int q_dt, void *work, cudaStream_t st) {
     if (q_dt == TLMG_DT_F32) return launch<HD, FMT, float>(a, work, st);
@@ -1220,7 +1346,9 @@ bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H) {
     return c.hd <= 128 && (int64_t)b.max_q * (H / c.KV) >= TQ;
 }
 
-size_t kv8_prefill_work_bytes(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H, int q_dt) { return images(c, b, H, q_dt).bytes; }
+size_t kv8_prefill_work_bytes(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_score &s, int H, int q_dt) {
+    return wide_plan(c, b, H, q_dt, s.causal, s.window).bytes;
+}
 
 int kv8_prefill(const Kv8Attn &a, int q_dt, void *work, cudaStream_t st) {
     return a.c.hd == 64 ? launch_fmt<64>(a, q_dt, work, st) : launch_fmt<128>(a, q_dt, work, st);
