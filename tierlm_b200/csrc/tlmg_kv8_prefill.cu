@@ -1208,10 +1208,10 @@ bool smem_opt_in(const void *fn, size_t bytes) {
 }
 
 // Key tiles of a sequence, and (sequence, KV head) pairs whose images one launch holds; 0 pairs: converting warps. Images
-// pay where enough query tiles share them (IMG_TILES below); above IMG_BYTES the pairs go in turns, each of which has to
-// fill the SMs twice.
-constexpr int IMG_TILES = 4;
-constexpr size_t IMG_BYTES = (size_t)256 << 20;
+// pay from IMG_TILES query tiles on (131,072 rows, 1 / 2 / 4 / 8 tiles a head: 190 / 245 / 368 / 637 us with them, 153 /
+// 244 / 430 / 841 without). Above IMG_BYTES the pairs go in turns, each of which has to fill the SMs twice.
+constexpr int IMG_TILES = 3;
+constexpr size_t IMG_BYTES = (size_t)512 << 20;
 struct Images {
     int n_img, n_seq, n_kv;   // sequences and KV heads of a launch
     size_t bytes;
@@ -1343,7 +1343,12 @@ template <int HD> int launch_fmt(const Kv8Attn &a, int q_dt, void *work, cudaStr
 }  // namespace
 
 bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H) {
-    return c.hd <= 128 && (int64_t)b.max_q * (H / c.KV) >= TQ;
+    // 32 heads on 4 of 128, a call as Python makes it: 16 tokens over 701 / 2,048 / 8,192 / 131,072 rows take 36 / 43 / 49 /
+    // 135 us here and 20 / 25 / 40 / 318 us in the kernel for few rows; 32 tokens over 2,048 / 8,192 rows 51 / 57 and 32 / 64,
+    // 64 tokens over 2,048 rows 51 and 45. The two meet where rows x keys x dims of all heads come to WIDE_WORK.
+    constexpr int64_t WIDE_WORK = (int64_t)3 << 28;
+    const int64_t rows = (int64_t)b.max_q * (H / c.KV);
+    return c.hd <= 128 && rows >= TQ && (double)rows * c.KV * b.n_seq * b.max_kv * c.hd >= (double)WIDE_WORK;
 }
 
 size_t kv8_prefill_work_bytes(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_score &s, int H, int q_dt) {
