@@ -493,7 +493,15 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
     const Kv8Range<TK> rg = kv8_range<TK>(a, q, s, pmin, pmax);
     const uint32_t tmem = sm.tmem;
     const int32_t *docs = a.doc ? a.doc + (size_t)s * a.doc_stride : nullptr;
-    int n = rg.n;
+    // A piece takes its share of the tiles: of those listed where a tile's header says who sees it, else of all of them (a
+    // list of all for each of 37 pieces cost a third of 32 tokens over 131,072 rows).
+    int n = rg.n, first = 0;
+    auto share = [&] {
+        first = (int)((int64_t)n * it.piece / it.pieces);
+        n = (int)((int64_t)n * (it.piece + 1) / it.pieces) - first;
+    };
+    if (!IMG) share();
+    const int v_0 = first;
     bool listed = false;
     if constexpr (SHAPED) {
         listed = n <= LIST && (docs || (a.c.pos && (a.causal || a.window)));
@@ -509,11 +517,12 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                 }
             }
             for (int v = warp; !IMG && v < n; v += THREADS / 32) {
+                const int tv = rg.t0(v_0 + v);
                 bool any = false;
                 int kp[TK / 32];
 #pragma unroll
                 for (int i = 0; i < TK / 32; i++) {
-                    const int t = rg.t0(v) + 32 * i + lane;
+                    const int t = tv + 32 * i + lane;
                     kp[i] = t;
                     if (a.c.pos) {
                         const int32_t e = t < q.L ? __ldg(table + (t >> a.c.lp)) : -1;
@@ -527,7 +536,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                         const int d = kp[i] >= 0 && kp[i] < a.doc_stride ? __ldg(docs + kp[i]) : -1;
                         see = see && d >= lo && d <= hi;
                     }
-                    any = any || (see && rg.t0(v) + 32 * i + lane < q.L);
+                    any = any || (see && tv + 32 * i + lane < q.L);
                 }
                 any = __any_sync(0xFFFFFFFFu, any);
                 if (lane == 0) sm.list[v] = any;
@@ -547,12 +556,11 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
             }
             __syncthreads();
             n = sm.n_list;
+            first = 0;
         }
     }
-    // a piece takes its share of the tiles
-    const int first = (int)((int64_t)n * it.piece / it.pieces);
-    n = (int)((int64_t)n * (it.piece + 1) / it.pieces) - first;
-    auto tile_at = [&](int j) { return rg.t0(SHAPED && listed ? (int)sm.list[first + j] : first + j); };
+    if (IMG) share();
+    auto tile_at = [&](int j) { return rg.t0(SHAPED && listed ? v_0 + sm.list[first + j] : first + j); };
 
     if (warp < SW) {
         // ---- softmax of one query tile ----
