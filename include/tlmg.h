@@ -595,7 +595,9 @@ typedef struct {
 /* A batch of sequences with new tokens. Sequence s has kv_len[s] rows, the
  * last n = q_start[s + 1] - q_start[s] of them new; its tokens are rows
  * q_start[s] .. of the token-major buffers (total_q tokens in all). max_q and
- * max_kv bound n and kv_len on the host (they size the launch). A sequence
+ * max_kv (at most 2^30) bound n and kv_len on the host: they size the launch
+ * and choose how the work is divided, so results may round otherwise under
+ * other bounds. A sequence
  * whose device-side lengths break 0 <= n <= max_q, n <= kv_len <= max_kv,
  * kv_len <= table_stride * page or the bounds of total_q is not followed:
  * appends skip it, attention returns NaN for its tokens. A page-table entry
@@ -654,7 +656,9 @@ typedef struct {
  * entry: the sums are the same in every run.
  *
  * work: scratch of tlmg_kv8_attend_work_bytes(...), 16-byte aligned; calls
- * that may overlap need scratch of their own. */
+ * that may overlap need scratch of their own. Prompts keep the key tiles in
+ * it as f16: 2.1 bytes a code that they may see, 512 MB at most (or, where that
+ * is more, one KV head of one sequence), and at most 80 MB of partial sums. */
 size_t tlmg_kv8_attend_work_bytes(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const tlmg_kv8_score *s, int H, int q_dt,
                                   int with_weights);
 int tlmg_kv8_attend(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const tlmg_kv8_score *s, int H, int q_dt, const void *q,

