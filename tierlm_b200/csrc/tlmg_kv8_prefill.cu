@@ -457,6 +457,13 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
     if (R0 >= n_rows) return;
     const bool two = !F32 && R0 + TQ < n_rows;
     const int i0 = token_of(R0), i1 = min(q.n, token_of(R0 + RPC - 1) + 1);
+    // the query rows set out for L2 while the CTA finds its tiles
+    constexpr int LINES = HD * (int)sizeof(QT) / 128;
+    for (int i = tid; i < min(RPC, n_rows - R0) * LINES; i += THREADS) {
+        const int R = R0 + i / LINES, tk = token_of(R);
+        const QT *x = static_cast<const QT *>(a.q) + (q.q0 + (int64_t)tk) * a.q_stride + (kvh * a.G + R - tk * a.G) * HD;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(x + i % LINES * (128 / (int)sizeof(QT))));
+    }
     if (tid == 0) {
         sm.abort = 0;
         sm.pmin = INT32_MAX;
@@ -921,13 +928,20 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
             const bool part = it.pieces > 1;     // the sums go to the workspace, for the join
             const float inv = !ok ? __uint_as_float(0x7FC00000u) : part ? unit : l == 0.0f ? 0.0f : __fdividef(unit, l);
             const size_t prow = part ? ((size_t)(blockIdx.x - a.n_full) * RPC + w * TQ + r) : 0;
+            // The warp's 32 half rows go through its share of the queries' buffer (their products are done), 16-byte chunks
+            // crossed so that neither side meets a bank twice, and out in whole lines: one row a lane, as they lie in TMEM,
+            // took 4,500 clocks a CTA.
+            constexpr int CH = HD / 2 * (int)sizeof(QT) / 16;
+            auto cross = [](int row) { return CH == 4 ? (row >> 1) & 3 : row & 7; };
+            uint8_t *stage = sm.q[F32 ? 0 : w] + (warp & 7) * (32 * CH * 16);
+            auto put = [&](int ch, uint4 v) { *reinterpret_cast<uint4 *>(stage + lane * CH * 16 + ((ch ^ cross(lane)) * 16)) = v; };
             if constexpr (F32) {
                 if (ok && n > 0) add_o();
-                float *dst = part ? a.po + prow * HD : reinterpret_cast<float *>(out) + orow * HD;
-                if (live)
 #pragma unroll
-                    for (int i = 0; i < HD / 2; i += 4)
-                        kv8_st4(dst + half * (HD / 2) + i, make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
+                for (int i = 0; i < HD / 2; i += 4) {
+                    const float4 v = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                    put(i / 4, *reinterpret_cast<const uint4 *>(&v));
+                }
             }
 #pragma unroll 1
             for (int c = half * (HD / 2); !F32 && c < (half + 1) * (HD / 2); c += 32) {
@@ -938,12 +952,13 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
 #pragma unroll
                     for (int i = 0; i < 32; i++) x[i] = 0;
                 }
-                if (live && part) {
+                if (part) {
+                    if (live)
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        kv8_st4(a.po + prow * HD + c + i, make_float4(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv,
-                                                                      __uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv));
-                } else if (live) {
+                        for (int i = 0; i < 32; i += 4)
+                            kv8_st4(a.po + prow * HD + c + i, make_float4(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv,
+                                                                          __uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv));
+                } else {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
                         uint4 o;
@@ -951,8 +966,20 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                                                                         __uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv));
                         kv8_st4(reinterpret_cast<QT *>(&o) + 4, make_float4(__uint_as_float(x[i + 4]) * inv, __uint_as_float(x[i + 5]) * inv,
                                                                             __uint_as_float(x[i + 6]) * inv, __uint_as_float(x[i + 7]) * inv));
-                        *reinterpret_cast<uint4 *>(out + orow * HD + c + i) = o;
+                        put((c - half * (HD / 2) + i) / 8, o);
                     }
+                }
+            }
+            if (F32 || !part) {
+                __syncwarp();
+                QT *to_rows = F32 && part ? reinterpret_cast<QT *>(a.po) : out;
+                const long long my = !live ? -1 : F32 && part ? (long long)prow : (long long)orow;
+#pragma unroll 4
+                for (int i = 0; i < CH; i++) {
+                    const int row = (32 * i + lane) / CH, ch = (32 * i + lane) % CH;
+                    const long long at = __shfl_sync(0xFFFFFFFFu, my, row);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stage + row * CH * 16 + ((ch ^ cross(row)) * 16));
+                    if (at >= 0) *reinterpret_cast<uint4 *>(to_rows + at * HD + half * (HD / 2) + ch * (16 / (int)sizeof(QT))) = v;
                 }
             }
             if (live && half == 0 && part) {
