@@ -654,6 +654,22 @@ def test_prefill_pieces(name, news, dtype):
     check_attend(host, table, q_start, lens, q, H, max_kv=bound, **mods)
 
 
+@pytest.mark.gpu
+def test_long_prompt():
+    """A prompt of more query tiles than a grid's second dimension takes: its last tokens as a call of their own gives them.
+    Both are within (2^-8 + 2^-10) max |v| of the exact result."""
+    L, H, KV, hd, last = 16500, 32, 2, 64, 40
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v, q = (torch.randn((L, h, hd), generator=g, device="cuda").to(torch.bfloat16) for h in (KV, KV, H))
+    cache = K.Kv8Cache(-(-L // 64), KV, 64, hd)
+    table = np.arange(-(-L // 64), dtype=np.int32)[None]
+    whole = batch(table, [0, L], [L])
+    cache.append(k, v, whole)
+    out = cache.attend(q, whole)[L - last:].float()
+    want = cache.attend(q[L - last:].contiguous(), batch(table, [0, last], [L])).float()
+    assert float((out - want).abs().max()) <= 2 * (2.0 ** -8 + 2.0 ** -10) * float(v.float().abs().max())
+
+
 def mods_of(name, rng, lens, H):
     n = len(lens)
     doc = np.full((n, max(lens)), -1, np.int32)

@@ -806,7 +806,8 @@ int check_attend(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const tlmg_kv8_scor
         s->window < 0 || (s->doc && s->doc_stride <= 0))
         return set_error(TLMG_EINVAL, "kv8_attend: scale %g, softcap %g, window %d, document stride %d", (double)s->scale,
                          (double)s->softcap, s->window, s->doc_stride);
-    if ((int64_t)b->total_q * H > INT32_MAX || ((int64_t)b->max_q * (H / c->KV) + 7) / 8 * c->KV > 65535)
+    const int64_t rows = (int64_t)b->max_q * (H / c->KV);   // (the kernel for few rows has query tiles in its grid's y)
+    if ((int64_t)b->total_q * H > INT32_MAX || (kv8_prefill_serves(*c, *b, H) ? rows >= 1 << 28 : (rows + 7) / 8 * c->KV > 65535))
         return set_error(TLMG_ERANGE, "kv8_attend: %d tokens x %d heads, at most %d tokens a sequence", b->total_q, H, b->max_q);
     return TLMG_OK;
 }

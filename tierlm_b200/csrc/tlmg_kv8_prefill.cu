@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
         }
         return;
     }
-    // R / G for the rows of a call (fewer than 2^20): the division's own code would be a good part of the start
+    // R / G for the rows of a call (fewer than 2^28, G at most 16): the division's own code would be a good part of the start
     auto token_of = [&](int R) { return (int)__umulhi((uint32_t)R, a.inv_g) + (a.G == 1 ? R : 0); };
     const int n_rows = q.n * a.G, R0 = rt * RPC;
     if (R0 >= n_rows) return;
