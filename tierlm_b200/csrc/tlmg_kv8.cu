@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_compact(const Kv8View c, 
         any = any && dok;
         if (any && lane == 0) (is_v ? d.vs : d.ks)[dr >> d.lb] = q;
     };
-    if (nj <= 8 * rpi) {   // the block's codes fit the warp's registers: all its loads at once, and once
+    if (nj <= min(32, 8 * rpi)) {   // a row a lane, and the codes fit the warp's registers: all the block's loads at once, and once
         uint32_t r = 0;
         const bool ok = source(lane, r);
         const float v = ok ? sc[r >> c.lb] : 0.0f;
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_compact(const Kv8View c, 
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int j = i * rpi + sub;
-            const uint32_t rr = __shfl_sync(0xFFFFFFFFu, r, j & 31);
+            const uint32_t rr = __shfl_sync(0xFFFFFFFFu, r, j & 31);   // (from j = 32 on: no row, below)
             vv[i] = __shfl_sync(0xFFFFFFFFu, v, j & 31);
             have[i] = __shfl_sync(0xFFFFFFFFu, (int)ok, j & 31) && j < nj;
             if (have[i]) w[i] = *reinterpret_cast<const uint4 *>(pool + (size_t)rr * c.hd + at);
