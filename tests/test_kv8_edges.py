@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_kv8 import Host, assert_cache, batch, make, quantise, select_reference, tables, up
+from test_kv8 import WIDE, Host, assert_cache, batch, check_attend, make, quantise, select_reference, tables, up
 
 from tierlm_b200 import kvcache as K
 
@@ -50,3 +50,24 @@ def test_evict_large_blocks(hd, dblock, keep, src_fmt, dst_fmt):
                 dst.pos[e, h, o + at] = pr[rr[at], h]
     assert_cache(dst_gpu, dst)
     assert (w_out.cpu().numpy() == want_w).all()
+
+
+# ---- attention ----------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_wide_rising_scores(hd, dtype):
+    """Scores that rise from key tile to key tile, now in the one and now in the other half of a tile: every tile moves the
+    reference that the two threads of a query row agree on."""
+    rng = np.random.default_rng(51)
+    L, n, H, KV, page = 1700, 90, 4, 2, 64
+    table, n_pages = tables(rng, [L], page)
+    host = Host(n_pages, KV, page, hd, K.INT8, 16)
+    u = rng.standard_normal(hd) / np.sqrt(hd)
+    t = np.arange(L)
+    rise = 3.0 * (t // 128) + np.where((t // 64 + t // 128) % 2 == 0, 2.0, 0.0)
+    k = (rng.standard_normal((L, KV, hd)) * 0.3 + (rise[:, None] * u)[:, None]).astype(np.float32)
+    host.append(k, rng.standard_normal((L, KV, hd)).astype(np.float32), table, [0, L], [L])
+    q = torch.from_numpy(((rng.standard_normal((n, H, hd)) * 0.3 + u * rng.uniform(0.5, 2, (n, H, 1)) * np.sqrt(hd))).astype(np.float32)).to(dtype)
+    for causal in (True, False):
+        check_attend(host, table, [0, n], [L], q, H, max_kv=WIDE, causal=causal)

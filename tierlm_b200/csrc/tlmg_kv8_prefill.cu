@@ -103,7 +103,7 @@ template <int HD> struct Smem {
     // per quarter of a tile: no scale is extreme; with a table to mask by: every row of the CTA sees every key
     alignas(4) uint8_t tame[META][4], seen[META][4];
     uint32_t row[2][TK];
-    float qs[2][TQ], part[2][2][TQ], sums[2][2][TQ];     // [tile][half][row]: the halves' maxima; in the end their sums
+    float qs[2][TQ], part[2][2][TQ], sums[2][2][TQ];     // [tile (f32 queries' maxima: key tile & 1)][half][row]: the halves' maxima; in the end their sums
     uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], p_half[2], x_full[2], o_full[2], meta_full[META], drain;
     uint32_t tmem;
     int abort, pmin, pmax, dmin, dmax, n_list;
@@ -805,12 +805,16 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                     }
                     tmem_wait_st();
                 }
-                // the other half's maximum: both threads of a row go by the same reference
-                sm.part[w][half][r] = m0;
+                // The other half's maximum: both threads of a row go by the same reference. 16-bit queries: this tile's
+                // scores came after the last tile's weights of all threads, so the entries of that tile have been read.
+                // f32 ones: S of this tile may have come before; two buffers in turn, and x_full of the tile between
+                // says that they have.
+                const int pb = F32 ? j & 1 : w;
+                sm.part[pb][half][r] = m0;
                 mbar_arrive(&sm.x_full[w]);
                 ok = mbar_wait_warp(&sm.x_full[w], j & 1, &sm.abort);
                 if (!ok) break;
-                m0 = fmaxf(m0, sm.part[w][half ^ 1][r]);
+                m0 = fmaxf(m0, sm.part[pb][half ^ 1][r]);
                 const bool grow = m0 > wref + GROW;
                 float fnew = 1.0f;
                 if (__any_sync(0xFFFFFFFFu, grow)) {
