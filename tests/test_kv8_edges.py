@@ -71,3 +71,57 @@ def test_wide_rising_scores(hd, dtype):
     q = torch.from_numpy(((rng.standard_normal((n, H, hd)) * 0.3 + u * rng.uniform(0.5, 2, (n, H, 1)) * np.sqrt(hd))).astype(np.float32)).to(dtype)
     for causal in (True, False):
         check_attend(host, table, [0, n], [L], q, H, max_kv=WIDE, causal=causal)
+
+
+def on_device(cache, table_row, L, q, H, scale=0.0, visible=None):
+    """64-bit attention of q [n][H][hd] over rows 0 .. L - 1 of one sequence, on the GPU: out, sum p |v|, sum |q k| scale at
+    its largest; visible [n] rows (None: all L)."""
+    row0 = torch.zeros(1, dtype=torch.int32, device="cuda")
+    k, v = cache.read(table_row[None].contiguous(), row0, torch.tensor([0, L], dtype=torch.int32, device="cuda"), L)
+    n, hd, KV = q.shape[0], q.shape[2], k.shape[1]
+    scale = scale or hd ** -0.5
+    out, mag = (torch.empty((n, H, hd), dtype=torch.float64, device="cuda") for _ in range(2))
+    top = torch.empty((n, H), dtype=torch.float64, device="cuda")
+    for h in range(H):
+        kk, vv = k[:, h * KV // H].double(), v[:, h * KV // H].double()
+        z = scale * (q[:, h].double() @ kk.T)
+        if visible is not None:
+            z = z.masked_fill(torch.arange(L, device="cuda")[None] >= visible[:, None], -torch.inf)
+        p = torch.softmax(z, -1)
+        out[:, h], mag[:, h] = p @ vv, p @ vv.abs()
+        top[:, h] = scale * (q[:, h].double().abs() @ kk.abs().T).amax(-1)
+    return out, mag, top
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,n_seq,T", [(64, 1, 2368), (128, 1, 2368), (64, 74, 32)])
+def test_long_rows(hd, n_seq, T, dtype):
+    """131,072 rows of positive values under even weights, in as many items as the SMs take whole (their key tiles stay one
+    sum), on images (1 sequence) and with converting warps (74 over the same pages). Each output: the bounds of test_kv8.py
+    and 2^-13 sum p |v| for the tensor core's sums, which truncate by 2^-23 of it at most, 1,024 times a run of 128 key tiles.
+    f16's mean relative error over all of these outputs: 2^-13 from the runs and 2^-14 for the mean of the roundings, uniform in 2^-12
+    at most over columns of different size. (One run over all rows: 8e-4.)"""
+    L, H, KV, page = 131072, 16, 1, 128
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    cache = K.Kv8Cache(L // page, KV, page, hd)
+    table = torch.randperm(L // page, generator=g, device="cuda").to(torch.int32)
+    v = (0.5 + torch.rand((1, KV, hd), generator=g, device="cuda")) * (1 + 0.25 * torch.rand((L, KV, hd), generator=g, device="cuda"))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache.append(rnd(L, KV, hd), v, K.Kv8Batch(table[None].contiguous(), i32(0, L), i32(L), L, L))
+    q = (rnd(n_seq * T, H, hd) * 0.2).to(dtype)
+    b = K.Kv8Batch(table[None].repeat(n_seq, 1), torch.arange(n_seq + 1, dtype=torch.int32, device="cuda") * T,
+                   torch.full((n_seq,), L, dtype=torch.int32, device="cuda"), T, L)
+    got = cache.attend(q, b, K.Score(causal=False))
+    at = torch.cat([torch.arange(12), torch.arange(n_seq * T - 12, n_seq * T)]).cuda()
+    want, mag, top = on_device(cache, table, L, q[at], H)
+    out = got[at].double()
+    bound = (2.0 ** -18 * top[..., None] + 2.0 ** -18) * mag + 1e-6 * 2.0 ** -20
+    if dtype != torch.float32:
+        # one f16 a weight, the truncated sums, the output; f16's smallest step is 2^-39 of the largest p v_scale, some 1e-7 here
+        bound = 1.01 * (bound + 2.0 ** -11 * mag + 2.0 ** -13 * mag) + want.abs() * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11)
+    assert ((out - want).abs() <= bound).all(), float(((out - want).abs() / bound).max())
+    if dtype == torch.float16:
+        mean = float(((out - want) / want).mean())
+        assert abs(mean) <= 2.0 ** -13 + 2.0 ** -14, mean

@@ -4,7 +4,7 @@
 // out = sum_t p_t v_t / sum_t p_t with p_t = 2^(score_t - reference): 4 hd flops a visible pair, so the tensor core is
 // the floor (2,048 clocks a key tile of 256 rows at hd 128). What is reached is set by the way from a tile's scores to its
 // weights: 2,600 clocks of softmax and 1,700 of MMAs and signals, half of each under the other tile's. 65,536 rows x 2,048
-// tokens x 32 heads of 128: 2,070 us, 1,046 TFLOP/s; a chunk of 2,048 on 16,384 rows 644 us, with a soft cap 1,026.
+// tokens x 32 heads of 128: 2,070 us, 1,046 TFLOP/s; a chunk of 2,048 on 16,384 rows 642 us, with a soft cap 1,046.
 //
 // 16-bit queries: one CTA per SM takes 256 query rows (token, head of the
 // group) of one KV head in two tiles A and B of 128, and walks the visible keys
@@ -36,6 +36,8 @@
 // 16, so 8 lanes write 8 rows of one chunk, 128 contiguous bytes. The same
 // bytes are K as a K-major B operand (contraction over dims) and V as an
 // MN-major one (contraction over keys).
+//
+// O's sums truncate: after RUN tiles O goes into an f32 sum of the softmax threads and starts again from zero.
 //
 // f32 queries (one query tile a CTA): Q and P are two f16 each, the high part and the remainder (P's times 2^11); S
 // sums the two products of Q, O's two products stay apart, start from zero at every key tile and are added to f32
@@ -286,6 +288,10 @@ __device__ __forceinline__ float cap_exp(float y, float capl) {
 
 constexpr float TOP = 14.0f;   // log2 of the largest p * v_scale right after a row's reference moved
 constexpr float GROW = 1.9f;   // how far it may grow before the reference moves again: 2^15.9 is an f16 (65,504 its largest)
+// 16-bit queries: key tiles whose products O adds up in the tensor core before they go into an f32 sum of rounded
+// additions. The tensor core's own sums truncate, 8 a tile and 2^-23 at most each, all towards zero: a run loses 2^-13 of
+// sum p |v| at most (1e-4 measured, at 131,072 and at 524,288 positive rows; as one sum 8.3e-4 and 3.3e-3).
+constexpr int RUN = 128;
 
 // The CTAs' work: one item a query tile and KV head, last tokens first since they see the most keys; the items from a.n_full
 // on are cut along the keys.
@@ -652,6 +658,15 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
             float wref = -INFINITY, lsum = 0.0f;
             // f32 queries: this thread's half of the row's output, and what the reference's last move multiplies it by
             float o[F32 ? HD / 2 : 1], fo = 1.0f;
+            // 16-bit queries: this thread's half of O of the runs so far and the reference it goes by, in local memory: none of
+            // it takes a register of the tile loop (the index is one that the compiler cannot know)
+            float4 runs[F32 ? 1 : HD / 8 + 1];
+            auto run_at = [&]() -> float4 * {
+                int zero = 0;
+                if constexpr (!F32) asm volatile("" : "+r"(zero));
+                return runs + zero;
+            };
+            auto run_factor = [&](const float4 *rs) { return rs[HD / 8].x == -INFINITY ? 0.0f : ex2(rs[HD / 8].x - wref); };
             auto add_o = [&] {
 #pragma unroll
                 for (int c = 0; c < (F32 ? HD / 2 : 0); c += 16) {
@@ -669,263 +684,287 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
             }
             // columns of a round of these loops: as many as the registers take (18k chunk without cap: 16 columns 702 us, 32 676)
             constexpr int CK = IMG && !F32 ? 32 : 16;
+            int j = 0, j_end = F32 ? n : min(n, RUN);
+            for (;;) {
 #pragma unroll 1
-            for (int j = 0; ok && j < n; j++) {
-                const int t0 = tile_at(j), mb = j & (META - 1);
-                const int sb = F32 ? j & 1 : w;                     // buffer of S
-                const uint32_t ts = tmem + lanes + sb * TK;
-                ok = mbar_wait_warp(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait_warp(&sm.s_full[sb], F32 ? (j >> 1) & 1 : j & 1, &sm.abort);
-                if (!ok) break;
-                tc_after();
-                const float *ks = sm.m[mb].ks, *vs = sm.m[mb].vs, *lv = sm.m[mb].lv;
-                // every key of the tile is seen by every row of the CTA
-                const bool open = lists ? *reinterpret_cast<const uint32_t *>(sm.seen[mb]) == 0x01010101u
-                                        : t0 + TK <= q.L && (!a.causal || t0 + TK - 1 <= pmin) && (!a.window || pmax - t0 < a.window);
-                // one scale for 8 keys, none of them extreme: the scales come in per group
-                const bool grp = a.c.lb >= 3 && *reinterpret_cast<const uint32_t *>(sm.tame[mb]) == 0x01010101u;
-                const bool rawS = open && grp && !(SHAPED && (a.softcap > 0.0f || a.slopes));
-                // Without tables a row sees the columns below c_pre and those in [c_lo, c_hi).
-                const int c_hi = min(a.causal ? (qp >= t0 + TK ? TK : qp + 1 - t0) : TK, q.L - t0);
-                const int c_lo = a.window ? (int)max((int64_t)qp - a.window + 1 - t0, (int64_t)0) : 0;
-                const int c_pre = min(pre - t0, q.L - t0);
-                float m0 = -INFINITY;
-                uint32_t xa[CK];
-                if (rawS) {
+                for (; ok && j < j_end; j++) {
+                    const int t0 = tile_at(j), mb = j & (META - 1);
+                    const int sb = F32 ? j & 1 : w;                     // buffer of S
+                    const uint32_t ts = tmem + lanes + sb * TK;
+                    ok = mbar_wait_warp(&sm.meta_full[mb], (j / META) & 1, &sm.abort) && mbar_wait_warp(&sm.s_full[sb], F32 ? (j >> 1) & 1 : j & 1, &sm.abort);
+                    if (!ok) break;
+                    tc_after();
+                    const float *ks = sm.m[mb].ks, *vs = sm.m[mb].vs, *lv = sm.m[mb].lv;
+                    // every key of the tile is seen by every row of the CTA
+                    const bool open = lists ? *reinterpret_cast<const uint32_t *>(sm.seen[mb]) == 0x01010101u
+                                            : t0 + TK <= q.L && (!a.causal || t0 + TK - 1 <= pmin) && (!a.window || pmax - t0 < a.window);
+                    // one scale for 8 keys, none of them extreme: the scales come in per group
+                    const bool grp = a.c.lb >= 3 && *reinterpret_cast<const uint32_t *>(sm.tame[mb]) == 0x01010101u;
+                    const bool rawS = open && grp && !(SHAPED && (a.softcap > 0.0f || a.slopes));
+                    // Without tables a row sees the columns below c_pre and those in [c_lo, c_hi).
+                    const int c_hi = min(a.causal ? (qp >= t0 + TK ? TK : qp + 1 - t0) : TK, q.L - t0);
+                    const int c_lo = a.window ? (int)max((int64_t)qp - a.window + 1 - t0, (int64_t)0) : 0;
+                    const int c_pre = min(pre - t0, q.L - t0);
+                    float m0 = -INFINITY;
+                    uint32_t xa[CK];
+                    if (rawS) {
 #pragma unroll 1
-                    for (int c = k0; c < k0 + HC; c += CK) {
-                        tmem_ldc(ts + c, xa);
+                        for (int c = k0; c < k0 + HC; c += CK) {
+                            tmem_ldc(ts + c, xa);
 #pragma unroll
-                        for (int g = 0; g < CK; g += 8) {
-                            float y = __uint_as_float(xa[g]), y1 = __uint_as_float(xa[g + 1]);
+                            for (int g = 0; g < CK; g += 8) {
+                                float y = __uint_as_float(xa[g]), y1 = __uint_as_float(xa[g + 1]);
 #pragma unroll
-                            for (int i = 2; i < 8; i += 2) {
-                                y = fmaxf(y, __uint_as_float(xa[g + i]));
-                                y1 = fmaxf(y1, __uint_as_float(xa[g + i + 1]));
-                            }
-                            m0 = fmaxf(m0, __fmaf_rn(fmaxf(y, y1), ks[c + g] * qs2, lv[c + g]));
-                        }
-                    }
-                } else if (grp) {
-                    // scores in log2 units, masked ones -inf, written back over S
-#pragma unroll 1
-                    for (int c = k0; c < k0 + HC; c += CK) {
-                        // (the flags are made to look new in every round: the compiler would copy the loop for each of them)
-                        int cap = SHAPED && a.softcap > 0.0f, ali = SHAPED && a.slopes, by_pos = SHAPED && a.c.pos, by_doc = SHAPED && docs, shut = !open;
-                        if constexpr (SHAPED) asm volatile("" : "+r"(cap), "+r"(ali), "+r"(by_pos), "+r"(by_doc), "+r"(shut));
-                        tmem_ldc(ts + c, xa);
-                        float z[CK];
-#pragma unroll
-                        for (int g = 0; g < CK; g += 8) {
-                            const float k = ks[c + g] * mul;
-#pragma unroll
-                            for (int i = 0; i < 8; i += 2) upk(mul2(pku(xa[g + i], xa[g + i + 1]), pk(k, k)), z[g + i], z[g + i + 1]);
-                        }
-                        if (cap) {
-                            float big = 0.0f;
-#pragma unroll
-                            for (int i = 0; i < CK; i++) big = fmaxf(big, fabsf(z[i]));
-                            if (__all_sync(0xFFFFFFFFu, big < TANH_X)) {   // (a NaN may pass: the polynomial keeps it)
-                                const f2 cl = pk(capl, capl);
-#pragma unroll
-                                for (int i = 0; i < CK; i += 2) {
-                                    const f2 y = pk(z[i], z[i + 1]), y2 = mul2(y, y);
-                                    f2 r = pk(TANH_C[5], TANH_C[5]);
-#pragma unroll
-                                    for (int k = 4; k >= 0; k--) r = fma2(r, y2, pk(TANH_C[k], TANH_C[k]));
-                                    upk(mul2(mul2(r, y), cl), z[i], z[i + 1]);
+                                for (int i = 2; i < 8; i += 2) {
+                                    y = fmaxf(y, __uint_as_float(xa[g + i]));
+                                    y1 = fmaxf(y1, __uint_as_float(xa[g + i + 1]));
                                 }
-                            } else {   // tanh(y) = 1 - 2 / (e^2y + 1)
-#pragma unroll
-                                for (int i = 0; i < CK; i++) z[i] = cap_exp(z[i], capl);
+                                m0 = fmaxf(m0, __fmaf_rn(fmaxf(y, y1), ks[c + g] * qs2, lv[c + g]));
                             }
                         }
-                        if (ali) {
-                            if (by_pos) {
+                    } else if (grp) {
+                        // scores in log2 units, masked ones -inf, written back over S
+#pragma unroll 1
+                        for (int c = k0; c < k0 + HC; c += CK) {
+                            // (the flags are made to look new in every round: the compiler would copy the loop for each of them)
+                            int cap = SHAPED && a.softcap > 0.0f, ali = SHAPED && a.slopes, by_pos = SHAPED && a.c.pos, by_doc = SHAPED && docs, shut = !open;
+                            if constexpr (SHAPED) asm volatile("" : "+r"(cap), "+r"(ali), "+r"(by_pos), "+r"(by_doc), "+r"(shut));
+                            tmem_ldc(ts + c, xa);
+                            float z[CK];
 #pragma unroll
-                                for (int i = 0; i < CK; i++) z[i] = __fmaf_rn(-slope, fabsf((float)(qp - sm.m[mb].pos[c + i])), z[i]);
-                            } else {
-                                const float far = (float)(qp - t0 - c);
+                            for (int g = 0; g < CK; g += 8) {
+                                const float k = ks[c + g] * mul;
 #pragma unroll
-                                for (int i = 0; i < CK; i++) z[i] = __fmaf_rn(-slope, fabsf(far - (float)i), z[i]);
+                                for (int i = 0; i < 8; i += 2) upk(mul2(pku(xa[g + i], xa[g + i + 1]), pk(k, k)), z[g + i], z[g + i + 1]);
                             }
-                        }
-                        if (shut) {
-                            const int lo = c_lo - c, hi = c_hi - c, pr = c_pre - c;
-                            if (by_pos) {
+                            if (cap) {
+                                float big = 0.0f;
 #pragma unroll
-                                for (int i = 0; i < CK; i++) {
-                                    const int kp = sm.m[mb].pos[c + i];
-                                    const bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
-                                    z[i] = see && t0 + c + i < q.L ? z[i] : -INFINITY;
-                                }
-                            } else {
+                                for (int i = 0; i < CK; i++) big = fmaxf(big, fabsf(z[i]));
+                                if (__all_sync(0xFFFFFFFFu, big < TANH_X)) {   // (a NaN may pass: the polynomial keeps it)
+                                    const f2 cl = pk(capl, capl);
 #pragma unroll
-                                for (int i = 0; i < CK; i++) z[i] = (i >= lo && i < hi) || i < pr ? z[i] : -INFINITY;
-                            }
-                            if (by_doc) {
+                                    for (int i = 0; i < CK; i += 2) {
+                                        const f2 y = pk(z[i], z[i + 1]), y2 = mul2(y, y);
+                                        f2 r = pk(TANH_C[5], TANH_C[5]);
 #pragma unroll
-                                for (int i = 0; i < CK; i += 4) {
-                                    const int4 d = *reinterpret_cast<const int4 *>(&sm.m[mb].doc[c + i]);
-                                    z[i] = d.x == qd ? z[i] : -INFINITY;
-                                    z[i + 1] = d.y == qd ? z[i + 1] : -INFINITY;
-                                    z[i + 2] = d.z == qd ? z[i + 2] : -INFINITY;
-                                    z[i + 3] = d.w == qd ? z[i + 3] : -INFINITY;
+                                        for (int k = 4; k >= 0; k--) r = fma2(r, y2, pk(TANH_C[k], TANH_C[k]));
+                                        upk(mul2(mul2(r, y), cl), z[i], z[i + 1]);
+                                    }
+                                } else {   // tanh(y) = 1 - 2 / (e^2y + 1)
+#pragma unroll
+                                    for (int i = 0; i < CK; i++) z[i] = cap_exp(z[i], capl);
                                 }
                             }
-                        }
+                            if (ali) {
+                                if (by_pos) {
 #pragma unroll
-                        for (int g = 0; g < CK; g += 8) {
-                            const float y = fmaxf(fmaxf(z[g], z[g + 1]), z[g + 2]), y1 = fmaxf(fmaxf(z[g + 3], z[g + 4]), z[g + 5]);
-                            m0 = fmaxf(m0, fmaxf(fmaxf(fmaxf(y, y1), z[g + 6]), z[g + 7]) + lv[c + g]);
-                        }
+                                    for (int i = 0; i < CK; i++) z[i] = __fmaf_rn(-slope, fabsf((float)(qp - sm.m[mb].pos[c + i])), z[i]);
+                                } else {
+                                    const float far = (float)(qp - t0 - c);
 #pragma unroll
-                        for (int i = 0; i < CK; i++) xa[i] = __float_as_uint(z[i]);
-                        tmem_stc(ts + c, xa);
-                    }
-                    tmem_wait_st();
-                } else {
-                    // scales of single keys: the same, four columns a round
+                                    for (int i = 0; i < CK; i++) z[i] = __fmaf_rn(-slope, fabsf(far - (float)i), z[i]);
+                                }
+                            }
+                            if (shut) {
+                                const int lo = c_lo - c, hi = c_hi - c, pr = c_pre - c;
+                                if (by_pos) {
+#pragma unroll
+                                    for (int i = 0; i < CK; i++) {
+                                        const int kp = sm.m[mb].pos[c + i];
+                                        const bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
+                                        z[i] = see && t0 + c + i < q.L ? z[i] : -INFINITY;
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int i = 0; i < CK; i++) z[i] = (i >= lo && i < hi) || i < pr ? z[i] : -INFINITY;
+                                }
+                                if (by_doc) {
+#pragma unroll
+                                    for (int i = 0; i < CK; i += 4) {
+                                        const int4 d = *reinterpret_cast<const int4 *>(&sm.m[mb].doc[c + i]);
+                                        z[i] = d.x == qd ? z[i] : -INFINITY;
+                                        z[i + 1] = d.y == qd ? z[i + 1] : -INFINITY;
+                                        z[i + 2] = d.z == qd ? z[i + 2] : -INFINITY;
+                                        z[i + 3] = d.w == qd ? z[i + 3] : -INFINITY;
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int g = 0; g < CK; g += 8) {
+                                const float y = fmaxf(fmaxf(z[g], z[g + 1]), z[g + 2]), y1 = fmaxf(fmaxf(z[g + 3], z[g + 4]), z[g + 5]);
+                                m0 = fmaxf(m0, fmaxf(fmaxf(fmaxf(y, y1), z[g + 6]), z[g + 7]) + lv[c + g]);
+                            }
+#pragma unroll
+                            for (int i = 0; i < CK; i++) xa[i] = __float_as_uint(z[i]);
+                            tmem_stc(ts + c, xa);
+                        }
+                        tmem_wait_st();
+                    } else {
+                        // scales of single keys: the same, four columns a round
 #pragma unroll 1
-                    for (int c = k0; c < k0 + HC; c += 4) {
-                        uint32_t x[4];
-                        tmem_ld4(ts + c, x);
+                        for (int c = k0; c < k0 + HC; c += 4) {
+                            uint32_t x[4];
+                            tmem_ld4(ts + c, x);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int col = c + i, t = t0 + col, kp = SHAPED && a.c.pos ? sm.m[mb].pos[col] : t;
-                            float z = __uint_as_float(x[i]) * (ks[col] * mul);
-                            if (SHAPED && a.softcap > 0.0f) z = cap_exp(z, capl);
-                            if (SHAPED && a.slopes) z = __fmaf_rn(-slope, fabsf((float)(qp - kp)), z);
-                            bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
-                            see = see && t < q.L && (!(SHAPED && docs) || sm.m[mb].doc[col] == qd);
-                            z = see ? z : -INFINITY;
-                            m0 = fmaxf(m0, z + lv[col]);
-                            x[i] = __float_as_uint(z);
-                        }
-                        tmem_st4(ts + c, x);
-                    }
-                    tmem_wait_st();
-                }
-                // The other half's maximum: both threads of a row go by the same reference. 16-bit queries: this tile's
-                // scores came after the last tile's weights of all threads, so the entries of that tile have been read.
-                // f32 ones: S of this tile may have come before; two buffers in turn, and x_full of the tile between
-                // says that they have.
-                const int pb = F32 ? j & 1 : w;
-                sm.part[pb][half][r] = m0;
-                mbar_arrive(&sm.x_full[w]);
-                ok = mbar_wait_warp(&sm.x_full[w], j & 1, &sm.abort);
-                if (!ok) break;
-                m0 = fmaxf(m0, sm.part[pb][half ^ 1][r]);
-                const bool grow = m0 > wref + GROW;
-                float fnew = 1.0f;
-                if (__any_sync(0xFFFFFFFFu, grow)) {
-                    const float f = grow && wref != -INFINITY ? ex2(wref - m0) : 1.0f;
-                    if (grow) wref = m0;
-                    lsum *= f;
-                    fnew = f;
-                    if (!F32 && j > 0) {
-#pragma unroll 1
-                        for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += CK) {
-                            tmem_ldc(to + c, xa);
-#pragma unroll
-                            for (int i = 0; i < CK; i++) xa[i] = __float_as_uint(__uint_as_float(xa[i]) * f);
-                            tmem_stc(to + c, xa);
+                            for (int i = 0; i < 4; i++) {
+                                const int col = c + i, t = t0 + col, kp = SHAPED && a.c.pos ? sm.m[mb].pos[col] : t;
+                                float z = __uint_as_float(x[i]) * (ks[col] * mul);
+                                if (SHAPED && a.softcap > 0.0f) z = cap_exp(z, capl);
+                                if (SHAPED && a.slopes) z = __fmaf_rn(-slope, fabsf((float)(qp - kp)), z);
+                                bool see = kp < pre || ((!a.causal || kp <= qp) && (!a.window || qp - kp < a.window));
+                                see = see && t < q.L && (!(SHAPED && docs) || sm.m[mb].doc[col] == qd);
+                                z = see ? z : -INFINITY;
+                                m0 = fmaxf(m0, z + lv[col]);
+                                x[i] = __float_as_uint(z);
+                            }
+                            tmem_st4(ts + c, x);
                         }
                         tmem_wait_st();
                     }
-                }
-                const float sub = wref == -INFINITY ? 0.0f : TOP - wref;
-                if (grp) {
-                    // p * v_scale = 2^(score + sub + log2 v_scale); the group's sum over v_scale is the sum of its p
+                    // The other half's maximum: both threads of a row go by the same reference. 16-bit queries: this tile's
+                    // scores came after the last tile's weights of all threads, so the entries of that tile have been read.
+                    // f32 ones: S of this tile may have come before; two buffers in turn, and x_full of the tile between
+                    // says that they have.
+                    const int pb = F32 ? j & 1 : w;
+                    sm.part[pb][half][r] = m0;
+                    mbar_arrive(&sm.x_full[w]);
+                    ok = mbar_wait_warp(&sm.x_full[w], j & 1, &sm.abort);
+                    if (!ok) break;
+                    m0 = fmaxf(m0, sm.part[pb][half ^ 1][r]);
+                    const bool grow = m0 > wref + GROW;
+                    float fnew = 1.0f;
+                    if (__any_sync(0xFFFFFFFFu, grow)) {
+                        const float f = grow && wref != -INFINITY ? ex2(wref - m0) : 1.0f;
+                        if (grow) wref = m0;
+                        lsum *= f;
+                        fnew = f;
+                        if (!F32 && j > 0) {
 #pragma unroll 1
-                    for (int c = k0; c < k0 + HC; c += CK) {
-                        uint32_t p[CK / 2];
-                        tmem_ldc(ts + c, xa);
+                            for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += CK) {
+                                tmem_ldc(to + c, xa);
 #pragma unroll
-                        for (int g = 0; g < CK; g += 8) {
-                            const float k = rawS ? ks[c + g] * qs2 : 1.0f, off = sub + lv[c + g];
-                            const f2 k2 = pk(k, k), o2 = pk(off, off);
-                            float y[8];
-#pragma unroll
-                            for (int i = 0; i < 8; i += 2) {
-                                upk(fma2(pku(xa[g + i], xa[g + i + 1]), k2, o2), y[i], y[i + 1]);
-                                y[i] = ex2(y[i]), y[i + 1] = ex2(y[i + 1]);
-                                p[(g + i) / 2] = pack_f16(y[i], y[i + 1]);
-                                if constexpr (F32) xa[(g + i) / 2] = rest_f16(y[i], y[i + 1], p[(g + i) / 2], 0x1p11f);
+                                for (int i = 0; i < CK; i++) xa[i] = __float_as_uint(__uint_as_float(xa[i]) * f);
+                                tmem_stc(to + c, xa);
                             }
-                            float u0, u1;
-                            upk(add2(add2(pk(y[0], y[1]), pk(y[2], y[3])), add2(pk(y[4], y[5]), pk(y[6], y[7]))), u0, u1);
-                            lsum = __fmaf_rn(u0 + u1, sm.m[mb].rv[c + g], lsum);
+                            tmem_wait_st();
                         }
-                        if constexpr (F32) {   // high parts and remainders of 16 keys over their 16 scores
+                    }
+                    const float sub = wref == -INFINITY ? 0.0f : TOP - wref;
+                    if (grp) {
+                        // p * v_scale = 2^(score + sub + log2 v_scale); the group's sum over v_scale is the sum of its p
+#pragma unroll 1
+                        for (int c = k0; c < k0 + HC; c += CK) {
+                            uint32_t p[CK / 2];
+                            tmem_ldc(ts + c, xa);
+#pragma unroll
+                            for (int g = 0; g < CK; g += 8) {
+                                const float k = rawS ? ks[c + g] * qs2 : 1.0f, off = sub + lv[c + g];
+                                const f2 k2 = pk(k, k), o2 = pk(off, off);
+                                float y[8];
+#pragma unroll
+                                for (int i = 0; i < 8; i += 2) {
+                                    upk(fma2(pku(xa[g + i], xa[g + i + 1]), k2, o2), y[i], y[i + 1]);
+                                    y[i] = ex2(y[i]), y[i + 1] = ex2(y[i + 1]);
+                                    p[(g + i) / 2] = pack_f16(y[i], y[i + 1]);
+                                    if constexpr (F32) xa[(g + i) / 2] = rest_f16(y[i], y[i + 1], p[(g + i) / 2], 0x1p11f);
+                                }
+                                float u0, u1;
+                                upk(add2(add2(pk(y[0], y[1]), pk(y[2], y[3])), add2(pk(y[4], y[5]), pk(y[6], y[7]))), u0, u1);
+                                lsum = __fmaf_rn(u0 + u1, sm.m[mb].rv[c + g], lsum);
+                            }
+                            if constexpr (F32) {   // high parts and remainders of 16 keys over their 16 scores
+                                tmem_stc(ts + c, p);
+#pragma unroll
+                                for (int i = 0; i < CK / 2; i++) p[i] = xa[i];
+                                tmem_stc(ts + c + 8, p);
+                            } else {
+                                tmem_stc(ts + (c + k0) / 2, p);   // columns whose scores are read already
+                                if (c == k0 + HC / 2 - CK) {        // the first half of these weights: their product can start
+                                    tmem_wait_st();
+                                    tc_before();
+                                    mbar_arrive(&sm.p_half[w]);
+                                }
+                            }
+                        }
+                    } else if constexpr (F32) {
+#pragma unroll 1
+                        for (int c = k0; c < k0 + HC; c += CK) {
+                            uint32_t p[CK / 2];
+                            tmem_ldc(ts + c, xa);
+#pragma unroll
+                            for (int i = 0; i < CK; i += 2) {
+                                const float y0 = __uint_as_float(xa[i]), y1 = __uint_as_float(xa[i + 1]), e0 = ex2(y0 + sub), e1 = ex2(y1 + sub);
+                                lsum += e0 + e1;
+                                const float u0 = y0 == -INFINITY ? 0.0f : e0 * vs[c + i], u1 = y1 == -INFINITY ? 0.0f : e1 * vs[c + i + 1];
+                                p[i / 2] = pack_f16(u0, u1);
+                                xa[i / 2] = rest_f16(u0, u1, p[i / 2], 0x1p11f);
+                            }
                             tmem_stc(ts + c, p);
 #pragma unroll
                             for (int i = 0; i < CK / 2; i++) p[i] = xa[i];
                             tmem_stc(ts + c + 8, p);
-                        } else {
-                            tmem_stc(ts + (c + k0) / 2, p);   // columns whose scores are read already
-                            if (c == k0 + HC / 2 - CK) {        // the first half of these weights: their product can start
-                                tmem_wait_st();
-                                tc_before();
-                                mbar_arrive(&sm.p_half[w]);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int c = k0; c < k0 + HC; c += 4) {
+                            uint32_t x[4], p[2];
+                            tmem_ld4(ts + c, x);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const float y = __uint_as_float(x[i]), e = ex2(y + sub);
+                                lsum += e;
+                                // a masked key's scale has no part in this, whatever it is
+                                x[i] = __float_as_uint(y == -INFINITY ? 0.0f : e * vs[c + i]);
                             }
+                            p[0] = pack_f16(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                            p[1] = pack_f16(__uint_as_float(x[2]), __uint_as_float(x[3]));
+                            tmem_st2(ts + (c + k0) / 2, p);
                         }
-                    }
-                } else if constexpr (F32) {
-#pragma unroll 1
-                    for (int c = k0; c < k0 + HC; c += CK) {
-                        uint32_t p[CK / 2];
-                        tmem_ldc(ts + c, xa);
-#pragma unroll
-                        for (int i = 0; i < CK; i += 2) {
-                            const float y0 = __uint_as_float(xa[i]), y1 = __uint_as_float(xa[i + 1]), e0 = ex2(y0 + sub), e1 = ex2(y1 + sub);
-                            lsum += e0 + e1;
-                            const float u0 = y0 == -INFINITY ? 0.0f : e0 * vs[c + i], u1 = y1 == -INFINITY ? 0.0f : e1 * vs[c + i + 1];
-                            p[i / 2] = pack_f16(u0, u1);
-                            xa[i / 2] = rest_f16(u0, u1, p[i / 2], 0x1p11f);
-                        }
-                        tmem_stc(ts + c, p);
-#pragma unroll
-                        for (int i = 0; i < CK / 2; i++) p[i] = xa[i];
-                        tmem_stc(ts + c + 8, p);
-                    }
-                } else {
-#pragma unroll 1
-                    for (int c = k0; c < k0 + HC; c += 4) {
-                        uint32_t x[4], p[2];
-                        tmem_ld4(ts + c, x);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float y = __uint_as_float(x[i]), e = ex2(y + sub);
-                            lsum += e;
-                            // a masked key's scale has no part in this, whatever it is
-                            x[i] = __float_as_uint(y == -INFINITY ? 0.0f : e * vs[c + i]);
-                        }
-                        p[0] = pack_f16(__uint_as_float(x[0]), __uint_as_float(x[1]));
-                        p[1] = pack_f16(__uint_as_float(x[2]), __uint_as_float(x[3]));
-                        tmem_st2(ts + (c + k0) / 2, p);
+                        tmem_wait_st();
+                        tc_before();
+                        mbar_arrive(&sm.p_half[w]);
                     }
                     tmem_wait_st();
-                    tc_before();
-                    mbar_arrive(&sm.p_half[w]);
-                }
-                tmem_wait_st();
-                if constexpr (F32) {   // the last tile's product: the next one starts over it
-                    if (j > 0) {
-                        ok = mbar_wait_warp(&sm.o_full[0], (j - 1) & 1, &sm.abort);
-                        if (!ok) break;
-                        tc_after();
-                        add_o();
+                    if constexpr (F32) {   // the last tile's product: the next one starts over it
+                        if (j > 0) {
+                            ok = mbar_wait_warp(&sm.o_full[0], (j - 1) & 1, &sm.abort);
+                            if (!ok) break;
+                            tc_after();
+                            add_o();
+                        }
+                        fo = fnew;
                     }
-                    fo = fnew;
+                    tc_before();
+                    mbar_arrive(&sm.p_full[w]);
                 }
-                tc_before();
-                mbar_arrive(&sm.p_full[w]);
+                if (F32 || !ok || j_end == n) break;
+                // a run ends, and more are to come: its products join the sum, and the next one starts O from zero
+                ok = mbar_wait_warp(&sm.o_full[w], (j / RUN - 1) & 1, &sm.abort);
+                if (!ok) break;
+                tc_after();
+                float4 *rs = run_at();
+                const float f = j > RUN ? run_factor(rs) : 0.0f;
+#pragma unroll 1
+                for (int c = 0; c < HD / 2; c += 16) {
+                    uint32_t x[16];
+                    tmem_ldc(to + half * (HD / 2) + c, x);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        float4 &v = rs[(c + i) / 4];
+                        const float4 u = j > RUN ? v : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        v = make_float4(__fmaf_rn(u.x, f, __uint_as_float(x[i])), __fmaf_rn(u.y, f, __uint_as_float(x[i + 1])),
+                                        __fmaf_rn(u.z, f, __uint_as_float(x[i + 2])), __fmaf_rn(u.w, f, __uint_as_float(x[i + 3])));
+                    }
+                }
+                rs[HD / 8].x = wref;
+                j_end = min(n, j_end + RUN);
             }
             float l = 0.0f;
             if (ok && n > 0) {
                 sm.sums[w][half][r] = lsum;
                 mbar_arrive(&sm.x_full[w]);
-                ok = mbar_wait_warp(&sm.x_full[w], n & 1, &sm.abort) && mbar_wait_warp(&sm.o_full[w], F32 ? (n - 1) & 1 : 0, &sm.abort);
+                ok = mbar_wait_warp(&sm.x_full[w], n & 1, &sm.abort) && mbar_wait_warp(&sm.o_full[w], (F32 ? n - 1 : (n - 1) / RUN) & 1, &sm.abort);
                 l = lsum + sm.sums[w][half ^ 1][r];
             }
             tc_after();
@@ -952,6 +991,18 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                 uint32_t x[32];
                 if (ok && n > 0) {
                     tmem_ld32(to + c, x);
+                    if (n > RUN) {
+                        const float4 *rs = run_at();
+                        const float f = run_factor(rs);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 u = rs[(c - half * (HD / 2) + i) / 4];
+                            x[i] = __float_as_uint(__fmaf_rn(u.x, f, __uint_as_float(x[i])));
+                            x[i + 1] = __float_as_uint(__fmaf_rn(u.y, f, __uint_as_float(x[i + 1])));
+                            x[i + 2] = __float_as_uint(__fmaf_rn(u.z, f, __uint_as_float(x[i + 2])));
+                            x[i + 3] = __float_as_uint(__fmaf_rn(u.w, f, __uint_as_float(x[i + 3])));
+                        }
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; i++) x[i] = 0;
@@ -1134,7 +1185,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
 #pragma unroll
                     for (int i = 0; i < TK / 32; i++) {
                         const int k = (i & 1) + (i & 2) * 2, kk = k + 2 * part;
-                        umma_ts(tm + 2 * TK + w * HD, tm + w * TK + 8 * kk + (k >= HC / 16 ? HC / 2 : 0), va + 2 * SBO / 16 * kk, id_pv, j > 0 || part > 0 || i > 0, lead);
+                        umma_ts(tm + 2 * TK + w * HD, tm + w * TK + 8 * kk + (k >= HC / 16 ? HC / 2 : 0), va + 2 * SBO / 16 * kk, id_pv, (j & (RUN - 1)) != 0 || part > 0 || i > 0, lead);
                     }
                 }
             };
@@ -1178,11 +1229,10 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
                     tc_after();
                     pv(w, j, 1);
                     if (w == nw - 1) umma_commit(&sm.v_empty[j & 1], lead);
+                    if (j + 1 == nt || ((j + 1) & (RUN - 1)) == 0) umma_commit(&sm.o_full[w], lead);
                     if (j + 1 < nt) {
                         qk(w, j + 1);
                         if (w == nw - 1) umma_commit(&sm.k_empty[(j + 1) & 1], lead);
-                    } else {
-                        umma_commit(&sm.o_full[w], lead);
                     }
                 }
             }
