@@ -600,7 +600,9 @@ typedef struct {
  * other bounds. A sequence
  * whose device-side lengths break 0 <= n <= max_q, n <= kv_len <= max_kv,
  * kv_len <= table_stride * page or the bounds of total_q is not followed:
- * appends skip it, attention returns NaN for its tokens. A page-table entry
+ * appends skip it, attention returns NaN for its tokens. Tokens that no
+ * sequence covers are not read, and their rows of out and lse are left
+ * unspecified; a call with total_q or max_q 0 writes nothing. A page-table entry
  * outside [0, n_pages) is not dereferenced: rows on it are not written, and a
  * query that sees one returns NaN. */
 typedef struct {

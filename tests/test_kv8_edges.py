@@ -1,13 +1,43 @@
 """Edges of the 8-bit KV cache (tierlm_b200/kvcache.py) beside tests/test_kv8.py, whose restatement and bounds it uses."""
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
-from test_kv8 import WIDE, Host, assert_cache, batch, check_attend, make, quantise, select_reference, tables, up
+from test_kv8 import WIDE, Host, assert_cache, batch, c_batch, c_cache, c_score, check_attend, make, quantise, select_reference, tables, up
 
+from tierlm_b200 import _lib
 from tierlm_b200 import kvcache as K
+
+
+# ---- bounds of zero ----------------------------------------------------------------------
+@pytest.mark.parametrize("kw", [dict(max_q=0), dict(total_q=0), dict(total_q=0, max_q=0), dict(max_kv=0), dict(max_q=0, max_kv=0)])
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("weights", [0, 1])
+def test_work_bytes_of_empty_calls(kw, hd, weights):
+    L = _lib.load()
+    got = L.tlmg_kv8_attend_work_bytes(C.byref(c_cache(hd=hd)), C.byref(c_batch(**kw)), C.byref(c_score()), 4, 0, weights)
+    assert 0 < got < 1 << 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_bounds_of_zero(dtype):
+    """Tokens where max_q allows none: NaN, and weights as they were."""
+    lens, news, H, KV, hd = [20, 30], [2, 1], 4, 2, 64
+    host, table, q_start, q, _ = make(43, lens, news, H, KV, hd, dtype=dtype)
+    cache = host.gpu()
+    for bounds in (dict(max_q=0), dict(max_q=0, max_kv=0)):
+        w = torch.full((2, KV, 33), 0.5, device="cuda")
+        out, lse = cache.attend(q.cuda(), batch(table, q_start, lens, **bounds), lse=True, weights=w)
+        assert torch.isnan(out).all() and torch.isnan(lse).all() and (w == 0.5).all()
+    out, lse = cache.attend(q[:0].cuda(), batch(table, [0, 0, 0], lens), lse=True)
+    assert out.shape == (0, H, hd) and lse.shape == (0, H)
+    out = cache.attend(q[:0].cuda(), batch(table, [0, 0, 0], [0, 0]))
+    assert out.shape == (0, H, hd)
 
 
 # ---- eviction ---------------------------------------------------------------------------

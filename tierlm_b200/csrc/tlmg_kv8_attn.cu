@@ -820,6 +820,7 @@ using namespace tlmg;
 extern "C" size_t tlmg_kv8_attend_work_bytes(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const tlmg_kv8_score *s, int H,
                                              int q_dt, int with_weights) {
     if (check_attend(c, b, s, H, q_dt)) return 0;
+    if (b->total_q == 0 || b->max_q == 0) return 16;   // nothing to do
     return split_plan(*c, *b, *s, H, q_dt, with_weights != 0).total;
 }
 

@@ -242,6 +242,10 @@ class Kv8Cache:
         lse_t = None
         if lse is not False and lse is not None:
             lse_t = torch.empty((n, H), dtype=torch.float32, device=q.device) if lse is True else lse
+        if batch.max_q == 0:    # no sequence may have a token: those that do break the bound
+            out.fill_(float("nan"))
+            if lse_t is not None:
+                lse_t.fill_(float("nan"))
         w_stride = 0
         if weights is not None:
             if weights.dim() != 3 or weights.shape[:2] != (batch.n_seq, self.KV):
