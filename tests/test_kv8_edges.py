@@ -40,6 +40,21 @@ def test_bounds_of_zero(dtype):
     assert out.shape == (0, H, hd)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weights_without_rows(dtype):
+    """max_kv 0: tokens have no row of their own, so they are NaN; sequences without tokens are in order. Weights stay."""
+    lens, news, H, KV, hd = [20, 30], [2, 1], 4, 2, 64
+    host, table, q_start, q, _ = make(43, lens, news, H, KV, hd, dtype=dtype)
+    cache = host.gpu()
+    w = torch.full((2, KV, 33), 0.5, device="cuda")
+    out, lse = cache.attend(q.cuda(), batch(table, q_start, lens, max_kv=0), lse=True, weights=w)
+    assert torch.isnan(out).all() and torch.isnan(lse).all() and (w == 0.5).all()
+    none = torch.empty((2, KV, 0), device="cuda")
+    out = cache.attend(q[:0].cuda(), batch(table, [0, 0, 0], [0, 0]), weights=none)
+    assert out.shape == (0, H, hd)
+
+
 # ---- eviction ---------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("src_fmt,dst_fmt", [(K.INT8, K.INT8), (K.E4M3, K.INT8), (K.INT8, K.E4M3)])

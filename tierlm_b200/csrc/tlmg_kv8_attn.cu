@@ -768,7 +768,7 @@ int launch_split_rows(const Kv8Attn &a, const Split &p, cudaStream_t st) {
         e = launch_dep(k_kv8_join<HD, QT>, dim3((unsigned)((int64_t)a.b.total_q * a.H)), JOIN_THREADS, a, st);
         count_launch();
     }
-    if (e == cudaSuccess && a.weights) {
+    if (e == cudaSuccess && a.weights && a.b.max_kv > 0) {
         const dim3 grid((a.b.max_kv + WG_THREADS - 1) / WG_THREADS, a.c.KV, a.b.n_seq);
         e = launch_dep(k_kv8_weights<ROWS>, grid, WG_THREADS, a, st);
         count_launch();
