@@ -130,11 +130,12 @@ def on_device(cache, table_row, L, q, H, scale=0.0, visible=None):
     for h in range(H):
         kk, vv = k[:, h * KV // H].double(), v[:, h * KV // H].double()
         z = scale * (q[:, h].double() @ kk.T)
+        size = scale * (q[:, h].double().abs() @ kk.abs().T)
         if visible is not None:
-            z = z.masked_fill(torch.arange(L, device="cuda")[None] >= visible[:, None], -torch.inf)
+            hidden = torch.arange(L, device="cuda")[None] >= visible[:, None]
+            z, size = z.masked_fill(hidden, -torch.inf), size.masked_fill(hidden, 0)
         p = torch.softmax(z, -1)
-        out[:, h], mag[:, h] = p @ vv, p @ vv.abs()
-        top[:, h] = scale * (q[:, h].double().abs() @ kk.abs().T).amax(-1)
+        out[:, h], mag[:, h], top[:, h] = p @ vv, p @ vv.abs(), size.amax(-1)
     return out, mag, top
 
 
@@ -162,11 +163,49 @@ def test_long_rows(hd, n_seq, T, dtype):
     at = torch.cat([torch.arange(12), torch.arange(n_seq * T - 12, n_seq * T)]).cuda()
     want, mag, top = on_device(cache, table, L, q[at], H)
     out = got[at].double()
-    bound = (2.0 ** -18 * top[..., None] + 2.0 ** -18) * mag + 1e-6 * 2.0 ** -20
+    bound = (2.0 ** -18 * top[..., None] + 2.0 ** -18) * mag + 1e-11
     if dtype != torch.float32:
-        # one f16 a weight, the truncated sums, the output; f16's smallest step is 2^-39 of the largest p v_scale, some 1e-7 here
+        # one f16 a weight, the truncated sums, the output (f16's smallest step comes to less than 1e-11 here)
         bound = 1.01 * (bound + 2.0 ** -11 * mag + 2.0 ** -13 * mag) + want.abs() * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11)
     assert ((out - want).abs() <= bound).all(), float(((out - want).abs() / bound).max())
     if dtype == torch.float16:
         mean = float(((out - want) / want).mean())
         assert abs(mean) <= 2.0 ** -13 + 2.0 ** -14, mean
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2])
+@pytest.mark.parametrize("hd,KV,H", [(256, 2, 32), (256, 8, 16), (128, 2, 32), (64, 4, 64), (256, 1, 16)])
+@pytest.mark.parametrize("n", [16384, 1 << 20])
+def test_long_prompts_are_served(hd, KV, H, n, dt):
+    """No number of tokens whose rows of all heads can be counted is refused."""
+    L = _lib.load()
+    b = c_batch(n_seq=1, total_q=n, max_q=n, max_kv=n, table_stride=n // 16)
+    assert L.tlmg_kv8_attend_work_bytes(C.byref(c_cache(hd=hd, KV=KV)), C.byref(b), C.byref(c_score()), H, dt, 0) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [256, 64])
+def test_long_prompt_against_64_bits(hd, dtype):
+    """A prompt of 16,500 tokens of 32 heads: first, middle and last tokens, and a sequence of too many tokens beside it
+    (head_dim 256, f32: more query tiles than a grid's second dimension takes). Bounds of test_kv8.py; f16's smallest step comes to
+    less than 2^-39 * 127 * 16,500 * the largest scale of V."""
+    L, H, KV, page = 16500, 32, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    k, v, q = (torch.randn((L + 3, h, hd), generator=g, device="cuda").to(dtype) for h in (KV, KV, H))
+    cache = K.Kv8Cache(-(-L // page) + 1, KV, page, hd)
+    table = torch.randperm(-(-L // page) + 1, generator=g, device="cuda").to(torch.int32)[None]
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    one = K.Kv8Batch(table, i32(0, L), i32(L), L, L)
+    cache.append(k[:L], v[:L], one)
+    b = K.Kv8Batch(table.repeat(2, 1), i32(0, L, L + 3), i32(L, 2), L, L)
+    got, lse = cache.attend(q, b, lse=True)
+    assert torch.isnan(got[L:]).all() and torch.isnan(lse[L:]).all() and torch.isfinite(got[:L]).all()
+    at = torch.tensor([0, 1, 2, 63, 64, 127, 128, 8190, 8191, 8192, 8193, 16374, 16375, 16376, 16384, L - 2, L - 1], device="cuda")
+    want, mag, top = on_device(cache, table[0], L, q[at], H, visible=at + 1)
+    low = 2.0 ** -39 * 127 * L * float(cache.v_scale.max())
+    bound = (2.0 ** -18 * top[..., None] + 2.0 ** -18) * mag + 2.0 ** -11 * low
+    if dtype == torch.bfloat16:
+        bound = 1.01 * (bound + 2.0 ** -11 * mag + 2.0 ** -13 * mag + low) + want.abs() * 2.0 ** -8
+    out = got[at].double()
+    assert ((out - want).abs() <= bound).all(), float(((out - want).abs() / bound).max())

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(32 * NW, split_ctas(HD, sizeof(QT) == 4, RM, F
     using P = Plan<HD>;
     extern __shared__ __align__(16) uint8_t sm[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-    const int s = blockIdx.z, kvh = blockIdx.y % a.c.KV, rt = blockIdx.y / a.c.KV, split = blockIdx.x;
+    const int s = blockIdx.z, kvh = blockIdx.y % a.c.KV, rt = a.rt0 + blockIdx.y / a.c.KV, split = blockIdx.x;
     const int G = a.G, H = a.H;
     QT *out = static_cast<QT *>(a.out);
     Kv8Seq q;
@@ -723,7 +723,7 @@ Split split_plan(const tlmg_kv8 &c, const tlmg_kv8_batch &b, const tlmg_kv8_scor
     // 16 query rows a CTA where there are more than 8 (not for f32 ones of 256 dims: no registers)
     p.rm = (int64_t)b.max_q * G > 8 && (q_dt != TLMG_DT_F32 || c.hd <= 128) ? 2 : 1;
     const int rows = 8 * p.rm;
-    p.rtiles = ((int64_t)b.max_q * G + rows - 1) / rows;
+    p.rtiles = ((int64_t)std::min(b.max_q, b.total_q) * G + rows - 1) / rows;
     // rows that a query tile can see at most (the prefix is only known to the device)
     int64_t vis = b.max_kv;
     if (s.window > 0 && s.causal && !c.pos && !s.prefix && !b.q_pos)
@@ -761,9 +761,16 @@ int launch_split_rows(const Kv8Attn &a, const Split &p, cudaStream_t st) {
     constexpr int ROWS = 8 * RM;
     constexpr size_t join = (size_t)NW * ROWS * (HD + 18) * 4, sm = std::max<size_t>(Plan<HD>::SMEM, join);
     if (!smem_opt_in((const void *)fn, sm)) return set_error(TLMG_EIO, "kv8_attend: shared memory opt-in failed");
-    fn<<<dim3(p.n, (unsigned)(p.rtiles * a.c.KV), a.b.n_seq), 32 * NW, sm, st>>>(a);
-    count_launch();
-    cudaError_t e = cudaGetLastError();
+    // query tiles and KV heads are the grid's y, which ends at 65,535: longer calls take launches of whole tiles in turn
+    Kv8Attn part = a;
+    const int64_t step = 65535 / a.c.KV;
+    cudaError_t e = cudaSuccess;
+    for (int64_t t = 0; e == cudaSuccess && t < p.rtiles; t += step) {
+        part.rt0 = (int)t;
+        fn<<<dim3(p.n, (unsigned)(std::min(step, p.rtiles - t) * a.c.KV), a.b.n_seq), 32 * NW, sm, st>>>(part);
+        count_launch();
+        e = cudaGetLastError();
+    }
     if (e == cudaSuccess && p.n > 1) {
         e = launch_dep(k_kv8_join<HD, QT>, dim3((unsigned)((int64_t)a.b.total_q * a.H)), JOIN_THREADS, a, st);
         count_launch();
@@ -806,9 +813,9 @@ int check_attend(const tlmg_kv8 *c, const tlmg_kv8_batch *b, const tlmg_kv8_scor
         s->window < 0 || (s->doc && s->doc_stride <= 0))
         return set_error(TLMG_EINVAL, "kv8_attend: scale %g, softcap %g, window %d, document stride %d", (double)s->scale,
                          (double)s->softcap, s->window, s->doc_stride);
-    const int64_t rows = (int64_t)b->max_q * (H / c->KV);   // (the kernel for few rows has query tiles in its grid's y)
-    if ((int64_t)b->total_q * H > INT32_MAX || (kv8_prefill_serves(*c, *b, H) ? rows >= 1 << 28 : (rows + 7) / 8 * c->KV > 65535))
-        return set_error(TLMG_ERANGE, "kv8_attend: %d tokens x %d heads, at most %d tokens a sequence", b->total_q, H, b->max_q);
+    if ((int64_t)b->total_q * H > INT32_MAX || c->KV > 65535 ||
+        (kv8_prefill_serves(*c, *b, H) && (int64_t)b->max_q * (H / c->KV) >= 1 << 28))
+        return set_error(TLMG_ERANGE, "kv8_attend: %d tokens x %d heads on %d, at most %d tokens a sequence", b->total_q, H, c->KV, b->max_q);
     return TLMG_OK;
 }
 

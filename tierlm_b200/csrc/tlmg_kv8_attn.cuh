@@ -21,6 +21,7 @@ struct Kv8Attn {
     const float *slopes;
     const int32_t *prefix, *doc;
     int doc_stride, causal, window;
+    int rt0;          // few query rows: the launch's first query tile
     // spans: partial outputs, maxima (log2 units) and sums [row][n_split], scores [row][s_stride]
     int n_split, tiles;
     float *po, *pm, *pl, *scores, *lse2;
