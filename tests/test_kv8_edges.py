@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -53,6 +54,61 @@ def test_weights_without_rows(dtype):
     none = torch.empty((2, KV, 0), device="cuda")
     out = cache.attend(q[:0].cuda(), batch(table, [0, 0, 0], [0, 0]), weights=none)
     assert out.shape == (0, H, hd)
+
+
+
+# ---- calls from several threads -----------------------------------------------------------
+def test_score_struct_lives_as_long_as_the_score():
+    """Calls with other batch sizes and head counts leave the struct where it is: a call of another thread may be reading it."""
+    s = K.Score(softcap=5.0, window=7)
+    at = s._at(1, 8)
+    assert all(s._at(n, H) == at for n in range(1, 50) for H in (8, 16, 32))
+    c = K._Score.from_address(at)
+    assert (c.softcap, c.window, c.causal, c.doc_stride, c.slopes) == (5.0, 7, 1, 0, None)
+
+
+def test_batch_struct_per_number_of_tokens():
+    """A call on other numbers of tokens leaves the struct of an earlier one as it was."""
+    b = K.Kv8Batch.__new__(K.Kv8Batch)
+    b.q_pos, b._calls, b._c = None, {}, c_batch(total_q=0, max_q=9, max_kv=50)
+    at = [b._at(n) for n in range(20)]
+    assert len(set(at)) == 20 and [b._at(n) for n in range(20)] == at
+    for n, p in enumerate(at):
+        c = K._Batch.from_address(p)
+        assert (c.total_q, c.max_q, c.max_kv, c.n_seq) == (n, 9, 50, 2)
+
+
+@pytest.mark.gpu
+def test_threads():
+    """Threads with streams of their own share a cache, the default score and a batch; every call has its own sizes."""
+    lens, H, KV, hd = [300, 200, 100], 4, 2, 64
+    host, table, _, _, rng = make(44, lens, [0, 0, 0], H, KV, hd)
+    cache = host.gpu()
+    shared = batch(table, [0, 1, 2, 3], lens)
+    q = up(rng.standard_normal((8, 16, hd)).astype(np.float32))
+    jobs = []
+    for i in range(4):
+        n = 1 + i % 3
+        own = batch(table[:n], list(range(n + 1)), lens[:n])
+        jobs += [(own, q[:n, :2 * (i + 1)].contiguous()), (shared, q[:3 + i, :4].contiguous())]
+    want = [cache.attend(x, b)[:b.n_seq].clone() for b, x in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(400):
+                j = (i * (2 * k + 1) + k) % len(jobs)
+                b, x = jobs[j]
+                if not torch.equal(cache.attend(x, b)[:b.n_seq], want[j]):
+                    wrong.append((k, i, j))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong, wrong[:5]
 
 
 # ---- eviction ---------------------------------------------------------------------------

@@ -109,14 +109,19 @@ class Kv8Batch:
         self.max_q, self.max_kv = max_q, max_kv
         self._c = _Batch(_i32(page_table, "page_table"), _i32(q_start, "q_start", (n_seq + 1,)),
                          _i32(kv_len, "kv_len", (n_seq,)), _i32(q_pos, "q_pos"), n_seq, stride, 0, max_q, max_kv)
-        self._p = C.addressof(self._c)
+        self._calls: dict[int, tuple[_Batch, int]] = {}     # tokens -> struct, address
 
     def _at(self, total: int) -> int:
-        """The address of the C struct for a call on `total` tokens."""
-        if self.q_pos is not None and self.q_pos.numel() < total:
-            raise TlmError(-3, f"q_pos has {self.q_pos.numel()} entries for {total} tokens")
-        self._c.total_q = total
-        return self._p
+        """The address of the C struct for a call on `total` tokens: one for each number of tokens, as long as the batch
+        lives (another thread's call may be reading it)."""
+        made = self._calls.get(total)
+        if made is None:
+            if self.q_pos is not None and self.q_pos.numel() < total:
+                raise TlmError(-3, f"q_pos has {self.q_pos.numel()} entries for {total} tokens")
+            c = _Batch.from_buffer_copy(self._c)
+            c.total_q = total
+            made = self._calls.setdefault(total, (c, C.addressof(c)))
+        return made[1]
 
 
 @dataclass(frozen=True)
@@ -134,16 +139,20 @@ class Score:
     doc: torch.Tensor | None = None
 
     def _at(self, n_seq: int, H: int) -> int:
-        """The address of the C struct for a call on n_seq sequences and H heads."""
-        key = (n_seq, H)
-        if self.__dict__.get("_made") != key:
+        """The address of the C struct, after the shapes were found to be those of n_seq sequences and H heads. It is built
+        once and lives as long as the score (another thread's call may be reading it): no field depends on the call."""
+        made = self.__dict__.get("_made")
+        if made is None:
+            c = _Score(self.scale, self.softcap, _f32(self.slopes, "slopes"), _i32(self.prefix, "prefix"), _i32(self.doc, "doc"),
+                       self.doc.shape[-1] if self.doc is not None else 0, 1 if self.causal else 0, self.window)
+            made = self.__dict__.setdefault("_made", (c, C.addressof(c), set()))
+        if (n_seq, H) not in made[2]:
+            _f32(self.slopes, "slopes", (H,))
+            _i32(self.prefix, "prefix", (n_seq,))
             if self.doc is not None and (self.doc.dim() != 2 or self.doc.shape[0] != n_seq):
                 raise TlmError(-3, f"doc has shape {tuple(self.doc.shape)}, not [{n_seq}][positions]")
-            c = _Score(self.scale, self.softcap, _f32(self.slopes, "slopes", (H,)),
-                       _i32(self.prefix, "prefix", (n_seq,)), _i32(self.doc, "doc"),
-                       self.doc.shape[1] if self.doc is not None else 0, 1 if self.causal else 0, self.window)
-            self.__dict__.update(_c=c, _p=C.addressof(c), _made=key)   # built once: the fields never change
-        return self._p
+            made[2].add((n_seq, H))
+        return made[1]
 
 
 _PLAIN = Score()
