@@ -111,6 +111,93 @@ def test_threads():
     assert not wrong, wrong[:5]
 
 
+
+@pytest.mark.gpu
+def test_threads_on_one_stream():
+    """Calls of several kernels from threads on the same stream: each joins its own partial results."""
+    lens, H, KV, hd = [3000, 1800], 8, 2, 64
+    host, table, _, _, rng = make(45, lens, [0, 0], H, KV, hd, page=64)
+    caches = [host.gpu() for _ in range(2)]
+    q = up(rng.standard_normal((4, H, hd)).astype(np.float32))
+    jobs = [(batch(table[:1], [0, 1 + i], lens[:1]), q[:1 + i]) for i in range(4)] + [(batch(table, [0, 1, 3], lens), q[:3])]
+    want = [caches[0].attend(x, b) for b, x in jobs]
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(k):
+        for i in range(300):
+            j = (i * (2 * k + 1) + k) % len(jobs)
+            got[k, i] = j, caches[k % 2].attend(jobs[j][1], jobs[j][0])
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert len(got) == 1200 and all(torch.equal(out, want[j]) for j, out in got.values())
+
+
+# ---- scratch ------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_scratch_is_shared_and_bounded():
+    """Layers used on one stream take one scratch; that of a prompt is torch's again after the call."""
+    KV, hd, page, L, n = 2, 128, 64, 20000, 2000
+    caches = [K.Kv8Cache(-(-L // page), KV, page, hd) for _ in range(3)]
+    table = torch.arange(-(-L // page), dtype=torch.int32, device="cuda")[None]
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    one, many = K.Kv8Batch(table, i32(0, 1), i32(L), 1, L), K.Kv8Batch(table, i32(0, n), i32(L), n, L)
+    q = torch.randn((n, 32, hd), device="cuda").to(torch.bfloat16)
+    out, few = torch.empty_like(q), torch.empty_like(q[:1])
+    caches[0].attend(q[:1], one, out=few)
+    at = torch.cuda.memory_allocated()
+    for c in caches:
+        c.attend(q[:1], one, out=few)
+        c.attend(q, many, out=out)
+    assert torch.cuda.memory_allocated() == at
+    peak = torch.cuda.max_memory_allocated()
+    assert peak - at < 1 << 30
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("news,H", [([1, 1], 8), ([40, 30], 16)])
+def test_graph_replay_after_larger_calls(news, H):
+    """A captured call's scratch stays its own: larger calls on the capture's stream and new tensors between the replays
+    neither change its output nor are changed by it."""
+    lens, KV, hd = [3000, 1700], 2, 64
+    host, table, q_start, q, rng = make(46, lens, news, H, KV, hd, page=64)
+    cache, b, qd = host.gpu(), batch(table, q_start, lens), q.cuda()
+    more = [0, 60, 120]
+    large, ql = batch(table, more, lens), up(rng.standard_normal((120, H, hd)).astype(np.float32))
+    w, wl = (torch.zeros((2, KV, 3000), device="cuda") for _ in range(2))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        want = cache.attend(qd, b, weights=w).clone()
+        for _ in range(2):
+            cache.attend(qd, b, weights=w)
+    torch.cuda.synchronize()
+    w.zero_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = cache.attend(qd, b, weights=w)
+    with torch.cuda.stream(s):
+        first = cache.attend(ql, large, weights=wl).clone()
+        fills = [torch.full((1 << 18,), float(i), device="cuda") for i in range(64)]
+    torch.cuda.synchronize()
+    for i in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert all((f == i).all() for i, f in enumerate(fills))
+    with torch.cuda.stream(s):
+        assert torch.equal(cache.attend(ql, large, weights=wl), first)
+    one = torch.zeros_like(w)
+    cache.attend(qd, b, weights=one)
+    torch.testing.assert_close(w, 3 * one, rtol=2.0 ** -20, atol=0)
+
+
 # ---- eviction ---------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("src_fmt,dst_fmt", [(K.INT8, K.INT8), (K.E4M3, K.INT8), (K.INT8, K.E4M3)])

@@ -6,17 +6,19 @@ One layer's K and V rows are 8-bit codes in page pools [n_pages][KV][page]
 [hd] (torch.int8, or torch.float8_e4m3fn) with one f32 scale per `block` rows
 of a head. A batch of sequences shares the pools: `Kv8Batch` holds the page
 tables, the lengths and where each sequence's new tokens sit. Calls run on
-torch's current stream; the cache keeps one scratch buffer per stream that
-it was used on.
+torch's current stream. Scratch of up to KEEP bytes is kept for each stream,
+for all caches (the layers of a model) that are used on it; what is larger, and
+all scratch of a call under graph capture, is torch's for the call.
 """
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from dataclasses import dataclass
 
 import torch
 
-from ._lib import BF16, F16, F32, TlmError, check, load
+from ._lib import BF16, F16, F32, TLMG_ERANGE, TlmError, check, load
 from .quant import CUDA_STREAM_LEGACY, _dev
 
 INT8, E4M3 = 1, 2
@@ -27,6 +29,30 @@ def _stream(index: int) -> int:
     """The current stream of a device for the C calls (see quant.stream_handle; without building a Stream object)."""
     s = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
     return s if s else CUDA_STREAM_LEGACY
+
+
+# A call's scratch up to this size is kept: torch.empty takes 1.8 us, a call from Python on 701 rows 17. Prompts take up to
+# 600 MB, in calls that are long beside it.
+KEEP = 32 << 20
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
+
+
+class _Scratch:
+    """What is kept for a stream. The lock covers a call's launches: those of two threads on one stream must not mix, since
+    the later kernels of a call read what the first one left here. It may grow, never under capture: an outgrown buffer
+    goes back to torch, which gives it to later work of the same stream."""
+    __slots__ = ("lock", "size", "at", "buffer")
+
+    def __init__(self, device):
+        self.lock = threading.Lock()
+        self.grow(1 << 20, device)
+
+    def grow(self, size: int, device) -> None:
+        self.buffer = torch.empty(size, dtype=torch.uint8, device=device)
+        self.size, self.at = size, self.buffer.data_ptr()
+
+
+_scratch: dict[tuple[int, int], _Scratch] = {}     # (device, stream)
 
 
 _FMT = {torch.int8: INT8, torch.float8_e4m3fn: E4M3}
@@ -203,7 +229,6 @@ class Kv8Cache:
         lib = load()
         self._append, self._read, self._attend = lib.tlmg_kv8_append, lib.tlmg_kv8_read, lib.tlmg_kv8_attend
         self._need, self._select, self._compact = lib.tlmg_kv8_attend_work_bytes, lib.tlmg_kv8_select, lib.tlmg_kv8_compact
-        self._work: dict[int, tuple[int, int, torch.Tensor]] = {}    # stream -> size, address, scratch
 
     def append(self, k: torch.Tensor, v: torch.Tensor, batch: Kv8Batch) -> None:
         """Stores the batch's new rows k, v [n][KV][hd] (float32, float16 or
@@ -261,13 +286,22 @@ class Kv8Cache:
                 raise TlmError(-3, f"weights have shape {tuple(weights.shape)}, not [{batch.n_seq}][{self.KV}][rows]")
             w_stride = weights.shape[2]
         st = _stream(self._dev)
-        need = self._need(self._p, b, s, H, dt, 0 if weights is None else 1)
-        have = self._work.get(st)
-        if have is None or have[0] < need:
-            work = torch.empty(max(need, 1 << 20), dtype=torch.uint8, device=q.device)
-            have = self._work[st] = (work.numel(), work.data_ptr(), work)
-        check(self._attend(self._p, b, s, H, dt, qp, sq, _dev(out, "out"), _f32(lse_t, "lse", (n, H)),
-                           _f32(weights, "weights"), w_stride, have[1], have[0], st))
+        call = (self._p, b, s, H, dt, qp, sq, _dev(out, "out"), _f32(lse_t, "lse", (n, H)), _f32(weights, "weights"), w_stride)
+        rc, dev = TLMG_ERANGE, q.device
+        if not _capturing():
+            w = _scratch.get((self._dev, st)) or _scratch.setdefault((self._dev, st), _Scratch(dev))
+            with w.lock:
+                rc = self._attend(*call, w.at, w.size, st)
+                if rc == TLMG_ERANGE:                  # what is kept is too small, most likely
+                    need = self._need(self._p, b, s, H, dt, 0 if weights is None else 1)
+                    if w.size < need <= KEEP:
+                        w.grow(need, dev)
+                        rc = self._attend(*call, w.at, w.size, st)
+        if rc == TLMG_ERANGE:
+            need = self._need(self._p, b, s, H, dt, 0 if weights is None else 1)
+            work = torch.empty(need, dtype=torch.uint8, device=dev)
+            rc = self._attend(*call, work.data_ptr(), need, st)
+        check(rc)
         return out if lse_t is None else (out, lse_t)
 
     def evict(self, weights: torch.Tensor, batch: Kv8Batch, dst_table: torch.Tensor, n_keep: int, sink: int = 0,
