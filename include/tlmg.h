@@ -680,8 +680,8 @@ int tlmg_kv8_select(int n_seq, int KV, const int32_t *kv_len, int max_kv, const 
  * row rows[s][kv][j] of page_table's, stored again by dst's blocks and format.
  * No page of dst_table may be one that page_table names. dst->pos (which must
  * exist) receives the rows' positions; weights_out [n_seq][KV][wo_stride]
- * (may be NULL) the rows' weights, 0 elsewhere. Entries of rows outside
- * [0, kv_len[s]) are skipped. */
+ * (may be NULL) the rows' weights, 0 elsewhere (rows from w_stride on have
+ * none). Entries of rows outside [0, kv_len[s]) are skipped. */
 int tlmg_kv8_compact(const tlmg_kv8 *c, const tlmg_kv8 *dst, int n_seq, const int32_t *page_table, int table_stride,
                      const int32_t *kv_len, const int32_t *dst_table, int dst_stride, const int32_t *rows, int n_keep,
                      const float *weights, int64_t w_stride, float *weights_out, int64_t wo_stride, void *stream);

@@ -240,6 +240,25 @@ def test_evict_large_blocks(hd, dblock, keep, src_fmt, dst_fmt):
     assert (w_out.cpu().numpy() == want_w).all()
 
 
+@pytest.mark.gpu
+def test_compact_rows_past_the_weights():
+    """Rows of the caller's own choice that have no weight: they move, their weight is 0."""
+    L, KV, page, n_keep, stride = 100, 2, 16, 12, 40
+    host, table, _, _, rng = make(47, [L], [0], 2, KV, 64, K.INT8, page, 16, True)
+    src, dst = host.gpu(), Host(2, KV, page, 64, K.INT8, 16, True, 3).gpu()
+    r = np.stack([np.sort(rng.permutation(L)[:n_keep]) for _ in range(KV)])[None].astype(np.int32)
+    r[0, 0, :3], r[0, 1, -3:] = [38, 39, 40], [98, 99, -1]
+    r[0, 0] = np.sort(r[0, 0])
+    w = rng.random((1, KV, stride)).astype(np.float32)
+    wd, rd, td, ld, dd = up(w), up(r), up(table), up(np.array([L], np.int32)), up(np.array([[1]], np.int32))
+    out = torch.full((1, KV, n_keep), 7.0, device="cuda")
+    _lib.check(_lib.load().tlmg_kv8_compact(src._p, dst._p, 1, td.data_ptr(), td.shape[1], ld.data_ptr(), dd.data_ptr(), 1, rd.data_ptr(),
+                                            n_keep, wd.data_ptr(), stride, out.data_ptr(), n_keep, 1))
+    want = np.where((r >= 0) & (r < stride), np.take_along_axis(w, np.clip(r, 0, stride - 1), 2), 0)
+    assert (out.cpu().numpy() == want).all()
+    assert (dst.pos[1].cpu().numpy()[:, :n_keep][r[0] >= 0] == host.positions(table[0], L)[r[0], np.arange(KV)[:, None]][r[0] >= 0]).all()
+
+
 # ---- attention ----------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])

@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_compact(const Kv8View c, 
             if (ok && dok) d.pos[dr + (uint32_t)j] = c.pos ? c.pos[r] : src[j];
             if (wout)
                 wout[((size_t)s * c.KV + kv) * wo_stride + j0 + j] =
-                    ok ? weights[((size_t)s * c.KV + kv) * w_stride + src[j]] : 0.0f;
+                    ok && src[j] < w_stride ? weights[((size_t)s * c.KV + kv) * w_stride + src[j]] : 0.0f;
         }
 }
 
