@@ -679,9 +679,12 @@ int tlmg_kv8_select(int n_seq, int KV, const int32_t *kv_len, int max_kv, const 
  * with the same KV and hd): row j of (s, kv) in dst_table's pages becomes
  * row rows[s][kv][j] of page_table's, stored again by dst's blocks and format.
  * No page of dst_table may be one that page_table names. dst->pos (which must
- * exist) receives the rows' positions; weights_out [n_seq][KV][wo_stride]
- * (may be NULL) the rows' weights, 0 elsewhere (rows from w_stride on have
- * none). Entries of rows outside [0, kv_len[s]) are skipped. */
+ * exist) receives the rows' positions; the first n_keep entries of every
+ * weights_out [n_seq][KV][wo_stride] (may be NULL) receive the rows' weights, 0
+ * where there is no row (rows from w_stride on have no weight). Entries from
+ * n_keep on stay as they are: clear them where later calls are to add the weights
+ * of new rows. weights_out must not overlap weights (refused). Entries of rows
+ * outside [0, kv_len[s]) are skipped. */
 int tlmg_kv8_compact(const tlmg_kv8 *c, const tlmg_kv8 *dst, int n_seq, const int32_t *page_table, int table_stride,
                      const int32_t *kv_len, const int32_t *dst_table, int dst_stride, const int32_t *rows, int n_keep,
                      const float *weights, int64_t w_stride, float *weights_out, int64_t wo_stride, void *stream);

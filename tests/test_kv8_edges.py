@@ -259,6 +259,28 @@ def test_compact_rows_past_the_weights():
     assert (dst.pos[1].cpu().numpy()[:, :n_keep][r[0] >= 0] == host.positions(table[0], L)[r[0], np.arange(KV)[:, None]][r[0] >= 0]).all()
 
 
+@pytest.mark.parametrize("at", [0, 4, -4, 4 * (2 * 2 * 40) - 4, -4 * (2 * 2 * 12) + 4])
+def test_weights_out_over_weights(at):
+    """Kept weights may not go where the weights are read from, in part neither."""
+    L, ok, w = _lib.load(), 1 << 20, 1 << 24
+    rc = L.tlmg_kv8_compact(C.byref(c_cache()), C.byref(c_cache()), 2, ok, 4, ok, ok, 4, ok, 8, w, 40, w + at, 12, 1)
+    assert rc == -3 and b"overlaps" in L.tlmg_errmsg()
+
+
+@pytest.mark.gpu
+def test_weights_out_beside_weights():
+    """The buffer right behind the weights is another one; entries from n_keep on stay as they were."""
+    L, KV, keep = 60, 2, 20
+    host, table, _, _, rng = make(48, [L], [0], 2, KV, 64, K.INT8, 16, 16, True)
+    both = torch.full((2 * KV * L,), 7.0, device="cuda")
+    w, out = both[:KV * L].view(1, KV, L), both[KV * L:].view(1, KV, L)
+    wn = rng.random((1, KV, L)).astype(np.float32)
+    w.copy_(up(wn))
+    rows, _ = host.gpu().evict(w, batch(table, [0, 0], [L], max_q=1), up(np.array([[0, 1]], np.int32)), keep, 2, 4,
+                               dst=Host(2, KV, 16, 64, K.INT8, 16, True, 3).gpu(), weights_out=out)
+    assert (out[..., :keep].cpu().numpy() == np.take_along_axis(wn, rows.cpu().numpy(), 2)).all() and (out[..., keep:] == 7.0).all()
+
+
 # ---- attention ----------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])

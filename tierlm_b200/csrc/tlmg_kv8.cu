@@ -566,6 +566,11 @@ extern "C" int tlmg_kv8_compact(const tlmg_kv8 *c, const tlmg_kv8 *dst, int n_se
     if (!page_table || !kv_len || !dst_table || !rows) return set_error(TLMG_EINVAL, "kv8_compact: null pointer");
     if (weights_out && (!weights || wo_stride < n_keep))
         return set_error(TLMG_EINVAL, "kv8_compact: weights_out needs weights and a stride of %d (%lld)", n_keep, (long long)wo_stride);
+    if (weights_out) {   // warps write it while others read the weights
+        const int64_t rows_all = (int64_t)n_seq * c->KV;
+        if (weights_out < weights + rows_all * std::max<int64_t>(w_stride, 0) && weights < weights_out + rows_all * wo_stride)
+            return set_error(TLMG_EINVAL, "kv8_compact: weights_out overlaps weights");
+    }
     const int64_t units = ((int64_t)(n_keep + dst->block - 1) / dst->block) * c->KV * 2;
     if (units > INT32_MAX - 64) return set_error(TLMG_ERANGE, "kv8_compact: %lld blocks", (long long)units);
     const dim3 grid((unsigned)((units + AP_WARPS - 1) / AP_WARPS), n_seq);

@@ -312,7 +312,10 @@ class Kv8Cache:
         dst_table's pages (of `dst`, or of this cache: other pages than
         the sequences hold). Returns (rows int32 [n_seq][KV][n_keep], lens
         int32 [n_seq]): the rows kept, ascending and -1 after the last, and
-        the new lengths."""
+        the new lengths. weights_out float32 [n_seq][KV][n_keep or more]
+        (another buffer than weights) takes the kept rows' weights; its entries
+        from n_keep on, which later tokens add theirs to, are left to the caller
+        to clear."""
         d = dst or self
         n, dev = batch.n_seq, self.k.device
         if weights.dim() != 3 or weights.shape[:2] != (n, self.KV):
