@@ -61,8 +61,8 @@ def test_weights_without_rows(dtype):
 def test_score_struct_lives_as_long_as_the_score():
     """Calls with other batch sizes and head counts leave the struct where it is: a call of another thread may be reading it."""
     s = K.Score(softcap=5.0, window=7)
-    at = s._at(1, 8)
-    assert all(s._at(n, H) == at for n in range(1, 50) for H in (8, 16, 32))
+    at = s._at(1, 8, 0)
+    assert all(s._at(n, H, 0) == at for n in range(1, 50) for H in (8, 16, 32))
     c = K._Score.from_address(at)
     assert (c.softcap, c.window, c.causal, c.doc_stride, c.slopes) == (5.0, 7, 1, 0, None)
 
@@ -70,9 +70,9 @@ def test_score_struct_lives_as_long_as_the_score():
 def test_batch_struct_per_number_of_tokens():
     """A call on other numbers of tokens leaves the struct of an earlier one as it was."""
     b = K.Kv8Batch.__new__(K.Kv8Batch)
-    b.q_pos, b._calls, b._c = None, {}, c_batch(total_q=0, max_q=9, max_kv=50)
-    at = [b._at(n) for n in range(20)]
-    assert len(set(at)) == 20 and [b._at(n) for n in range(20)] == at
+    b.q_pos, b._dev, b._calls, b._c = None, 0, {}, c_batch(total_q=0, max_q=9, max_kv=50)
+    at = [b._at(n, 0) for n in range(20)]
+    assert len(set(at)) == 20 and [b._at(n, 0) for n in range(20)] == at
     for n, p in enumerate(at):
         c = K._Batch.from_address(p)
         assert (c.total_q, c.max_q, c.max_kv, c.n_seq) == (n, 9, 50, 2)
@@ -136,6 +136,70 @@ def test_threads_on_one_stream():
         th.join()
     torch.cuda.synchronize()
     assert len(got) == 1200 and all(torch.equal(out, want[j]) for j, out in got.values())
+
+
+# ---- devices ------------------------------------------------------------------------------
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+def test_refuses_tensors_of_other_devices(monkeypatch):
+    """Everything a call reads has to be on the cache's device, and that the current one: no call reaches the library."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    def called(*a):
+        raise AssertionError("the library was called")
+
+    def refused(fn, what):
+        with pytest.raises(_lib.TlmError) as e:
+            fn()
+        assert e.value.code == -3 and "cuda:" in str(e.value) and what in str(e.value), str(e.value)
+
+    monkeypatch.setattr(K, "_current_device", lambda: 0, raising=False)
+    monkeypatch.setattr(K, "_raw_stream", lambda index: 0)
+    i32 = lambda d, *shape: torch.empty(shape, dtype=torch.int32, device=f"cuda:{d}")  # noqa: E731
+    f32 = lambda d, *shape: torch.empty(shape, device=f"cuda:{d}")  # noqa: E731
+    with FakeTensorMode():
+        pools = lambda *d: (f32(d[0], 4, 2, 16, 64).to(torch.int8), f32(d[1], 4, 2, 16, 64).to(torch.int8),  # noqa: E731
+                            f32(d[2], 4, 2, 1), f32(d[3], 4, 2, 1), i32(d[4], 4, 2, 16))
+        for i, what in enumerate(["v", "k_scale", "v_scale", "pos"], 1):
+            d = [0] * 5
+            d[i] = 1
+            refused(lambda: K.Kv8Cache.from_pools(*pools(*d)), what)
+        cache, other = K.Kv8Cache.from_pools(*pools(*[0] * 5)), K.Kv8Cache.from_pools(*pools(*[1] * 5))
+        for c in (cache, other):
+            c._append = c._read = c._attend = c._need = c._select = c._compact = called
+        arrays = lambda *d: (i32(d[0], 3, 2), i32(d[1], 4), i32(d[2], 3), 1, 20, i32(d[3], 3))  # noqa: E731
+        for i, what in enumerate(["q_start", "kv_len", "q_pos"], 1):
+            d = [0] * 4
+            d[i] = 1
+            refused(lambda: K.Kv8Batch(*arrays(*d)), what)
+        b, far = K.Kv8Batch(*arrays(*[0] * 4)), K.Kv8Batch(*arrays(*[1] * 4))
+        rows, q, w, table = f32(0, 3, 2, 64), f32(0, 3, 4, 64), f32(0, 3, 2, 20), i32(0, 3, 2)
+        refused(lambda: cache.append(f32(1, 3, 2, 64), rows, b), "k ")
+        refused(lambda: cache.append(rows, f32(1, 3, 2, 64), b), "v ")
+        refused(lambda: cache.append(rows, rows, far), "batch")
+        refused(lambda: cache.attend(f32(1, 3, 4, 64), b), "q ")
+        refused(lambda: cache.attend(q, far), "batch")
+        refused(lambda: cache.attend(q, b, out=f32(1, 3, 4, 64)), "out")
+        refused(lambda: cache.attend(q, b, lse=f32(1, 3, 4)), "lse")
+        refused(lambda: cache.attend(q, b, weights=f32(1, 3, 2, 20)), "weights")
+        for kw in (dict(slopes=f32(1, 4)), dict(prefix=i32(1, 3)), dict(doc=i32(1, 3, 20))):
+            refused(lambda: cache.attend(q, b, K.Score(**kw)), next(iter(kw)))
+        row0, start = i32(0, 3), i32(0, 4)
+        refused(lambda: cache.read(i32(1, 3, 2), row0, start, 5), "page_table")
+        refused(lambda: cache.read(table, i32(1, 3), start, 5), "row0")
+        refused(lambda: cache.read(table, row0, i32(1, 4), 5), "start")
+        refused(lambda: cache.read(table, row0, start, 5, k=f32(1, 5, 2, 64), v=f32(0, 5, 2, 64)), "k ")
+        refused(lambda: cache.evict(f32(1, 3, 2, 20), b, table, 8), "weights")
+        refused(lambda: cache.evict(w, far, table, 8), "batch")
+        refused(lambda: cache.evict(w, b, table, 8, dst=other), "destination")
+        refused(lambda: cache.evict(w, b, table, 8, rows=i32(1, 3, 2, 8)), "rows")
+        refused(lambda: cache.evict(w, b, table, 8, lens=i32(1, 3)), "lens")
+        refused(lambda: cache.evict(w, b, i32(1, 3, 2), 8), "dst_table")
+        refused(lambda: cache.evict(w, b, table, 8, weights_out=f32(1, 3, 2, 8)), "weights_out")
+        # all of it on another device than the current one
+        refused(lambda: other.append(f32(1, 3, 2, 64), f32(1, 3, 2, 64), far), "current device")
+        refused(lambda: other.attend(f32(1, 3, 4, 64), far), "current device")
+        refused(lambda: other.read(i32(1, 3, 2), i32(1, 3), i32(1, 4), 5), "current device")
+        refused(lambda: other.evict(f32(1, 3, 2, 20), far, i32(1, 3, 2), 8), "current device")
 
 
 # ---- scratch ------------------------------------------------------------------------------

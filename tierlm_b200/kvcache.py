@@ -23,10 +23,14 @@ from .quant import CUDA_STREAM_LEGACY, _dev
 
 INT8, E4M3 = 1, 2
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream(index: int) -> int:
-    """The current stream of a device for the C calls (see quant.stream_handle; without building a Stream object)."""
+    """The current stream of a device for the C calls (see quant.stream_handle; without building a Stream object). It has
+    to be the current device, on which the library launches: kernels elsewhere could not read the pools."""
+    if _current_device() != index:
+        raise TlmError(-3, f"the cache is on cuda:{index}, the current device is cuda:{_current_device()}")
     s = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
     return s if s else CUDA_STREAM_LEGACY
 
@@ -79,35 +83,45 @@ class _Score(C.Structure):
                 ("doc", C.c_void_p), ("doc_stride", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32)]
 
 
-def _i32(t: torch.Tensor | None, what: str, shape: tuple | None = None) -> int | None:
+def _ptr(t: torch.Tensor, what: str, dev: int) -> int:
+    """The address of a contiguous tensor on CUDA device dev (calls of a few microseconds: one check does for "CUDA" and "which")."""
+    if t.get_device() != dev:
+        raise TlmError(-3, f"{what} is on {t.device}, not on cuda:{dev} as the rest")
+    if not t.is_contiguous():
+        raise TlmError(-3, f"{what} must be contiguous")
+    return t.data_ptr()
+
+
+def _i32(t: torch.Tensor | None, what: str, shape: tuple | None = None, dev: int | None = None) -> int | None:
+    """The address of an int32 tensor of this shape on CUDA device dev (None: any)."""
     if t is None:
         return None
     if t.dtype != torch.int32:
         raise TlmError(-3, f"{what} must be int32, not {t.dtype}")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise TlmError(-3, f"{what} has shape {tuple(t.shape)}, not {shape}")
-    return _dev(t, what)
+    return _dev(t, what) if dev is None else _ptr(t, what, dev)
 
 
-def _f32(t: torch.Tensor | None, what: str, shape: tuple | None = None) -> int | None:
+def _f32(t: torch.Tensor | None, what: str, shape: tuple | None = None, dev: int | None = None) -> int | None:
     if t is None:
         return None
     if t.dtype != torch.float32:
         raise TlmError(-3, f"{what} must be float32, not {t.dtype}")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise TlmError(-3, f"{what} has shape {tuple(t.shape)}, not {shape}")
-    return _dev(t, what)
+    return _dev(t, what) if dev is None else _ptr(t, what, dev)
 
 
-def _rows(t: torch.Tensor, what: str, heads: int, hd: int) -> tuple[torch.Tensor, int, int]:
+def _rows(t: torch.Tensor, what: str, heads: int, hd: int, dev: int) -> tuple[torch.Tensor, int, int]:
     """[n][heads][hd] rows, their stride in elements and their address; a copy
     where the library cannot read them in place (heads apart, rows off 16 bytes)."""
     if t.dtype not in _X_DT:
         raise TlmError(-3, f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
     if t.dim() != 3 or t.shape[1:] != (heads, hd):
         raise TlmError(-3, f"{what} has shape {tuple(t.shape)}, not [n][{heads}][{hd}]")
-    if not t.is_cuda:
-        raise TlmError(-3, f"{what} must be a CUDA tensor")
+    if t.get_device() != dev:
+        raise TlmError(-3, f"{what} is on {t.device}, not on cuda:{dev} as the cache")
     st, sh, sd = t.stride()
     at = t.data_ptr()
     if sd != 1 or sh != hd or st < heads * hd or st * (4 if t.dtype is torch.float32 else 2) % 16 or at % 16:
@@ -133,13 +147,16 @@ class Kv8Batch:
         self._keep = (page_table, q_start, kv_len, q_pos)
         self.n_seq, self.page_table, self.kv_len, self.q_pos = n_seq, page_table, kv_len, q_pos
         self.max_q, self.max_kv = max_q, max_kv
-        self._c = _Batch(_i32(page_table, "page_table"), _i32(q_start, "q_start", (n_seq + 1,)),
-                         _i32(kv_len, "kv_len", (n_seq,)), _i32(q_pos, "q_pos"), n_seq, stride, 0, max_q, max_kv)
+        self._dev = dev = page_table.get_device()
+        self._c = _Batch(_i32(page_table, "page_table"), _i32(q_start, "q_start", (n_seq + 1,), dev),
+                         _i32(kv_len, "kv_len", (n_seq,), dev), _i32(q_pos, "q_pos", None, dev), n_seq, stride, 0, max_q, max_kv)
         self._calls: dict[int, tuple[_Batch, int]] = {}     # tokens -> struct, address
 
-    def _at(self, total: int) -> int:
-        """The address of the C struct for a call on `total` tokens: one for each number of tokens, as long as the batch
+    def _at(self, total: int, dev: int) -> int:
+        """The address of the C struct for a call on `total` tokens and device dev: one for each number of tokens, as long as the batch
         lives (another thread's call may be reading it)."""
+        if self._dev != dev:
+            raise TlmError(-3, f"the batch is on cuda:{self._dev}, the cache on cuda:{dev}")
         made = self._calls.get(total)
         if made is None:
             if self.q_pos is not None and self.q_pos.numel() < total:
@@ -164,20 +181,21 @@ class Score:
     prefix: torch.Tensor | None = None
     doc: torch.Tensor | None = None
 
-    def _at(self, n_seq: int, H: int) -> int:
-        """The address of the C struct, after the shapes were found to be those of n_seq sequences and H heads. It is built
+    def _at(self, n_seq: int, H: int, dev: int) -> int:
+        """The address of the C struct, after the tensors were found to be those of n_seq sequences and H heads on device dev. It is built
         once and lives as long as the score (another thread's call may be reading it): no field depends on the call."""
         made = self.__dict__.get("_made")
         if made is None:
             c = _Score(self.scale, self.softcap, _f32(self.slopes, "slopes"), _i32(self.prefix, "prefix"), _i32(self.doc, "doc"),
                        self.doc.shape[-1] if self.doc is not None else 0, 1 if self.causal else 0, self.window)
             made = self.__dict__.setdefault("_made", (c, C.addressof(c), set()))
-        if (n_seq, H) not in made[2]:
-            _f32(self.slopes, "slopes", (H,))
-            _i32(self.prefix, "prefix", (n_seq,))
+        if (n_seq, H, dev) not in made[2]:
+            _f32(self.slopes, "slopes", (H,), dev)
+            _i32(self.prefix, "prefix", (n_seq,), dev)
+            _i32(self.doc, "doc", None, dev)
             if self.doc is not None and (self.doc.dim() != 2 or self.doc.shape[0] != n_seq):
                 raise TlmError(-3, f"doc has shape {tuple(self.doc.shape)}, not [{n_seq}][positions]")
-            made[2].add((n_seq, H))
+            made[2].add((n_seq, H, dev))
         return made[1]
 
 
@@ -221,11 +239,11 @@ class Kv8Cache:
         blocks = k_scale.shape[2]
         self.k, self.v, self.k_scale, self.v_scale, self.pos = k, v, k_scale, v_scale, pos
         self.KV, self.page_size, self.hd, self.block, self.fmt = KV, page, hd, page // blocks, _FMT[k.dtype]
-        self._c = _Cache(_dev(k, "k"), _dev(v, "v"), _f32(k_scale, "k_scale", (n_pages, KV, blocks)),
-                         _f32(v_scale, "v_scale", (n_pages, KV, blocks)), _i32(pos, "pos", (n_pages, KV, page)),
+        self._dev = dev = k.get_device()
+        self._c = _Cache(_dev(k, "k"), _ptr(v, "v", dev), _f32(k_scale, "k_scale", (n_pages, KV, blocks), dev),
+                         _f32(v_scale, "v_scale", (n_pages, KV, blocks), dev), _i32(pos, "pos", (n_pages, KV, page), dev),
                          self.fmt, n_pages, KV, page, self.block, hd)
         self._p = C.addressof(self._c)
-        self._dev = k.device.index or 0
         lib = load()
         self._append, self._read, self._attend = lib.tlmg_kv8_append, lib.tlmg_kv8_read, lib.tlmg_kv8_attend
         self._need, self._select, self._compact = lib.tlmg_kv8_attend_work_bytes, lib.tlmg_kv8_select, lib.tlmg_kv8_compact
@@ -233,14 +251,14 @@ class Kv8Cache:
     def append(self, k: torch.Tensor, v: torch.Tensor, batch: Kv8Batch) -> None:
         """Stores the batch's new rows k, v [n][KV][hd] (float32, float16 or
         bfloat16)."""
-        k, sk, kp = _rows(k, "k", self.KV, self.hd)
-        v, sv, vp = _rows(v, "v", self.KV, self.hd)
+        k, sk, kp = _rows(k, "k", self.KV, self.hd, self._dev)
+        v, sv, vp = _rows(v, "v", self.KV, self.hd, self._dev)
         if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
             raise TlmError(-3, f"k and v differ: {k.dtype} x {k.shape[0]} rows, {v.dtype} x {v.shape[0]} rows")
         if sk != sv:
             k, v = k.contiguous(), v.contiguous()
             sk, kp, vp = self.KV * self.hd, k.data_ptr(), v.data_ptr()
-        check(self._append(self._p, batch._at(k.shape[0]), _X_DT[k.dtype], kp, vp, sk, _stream(self._dev)))
+        check(self._append(self._p, batch._at(k.shape[0], self._dev), _X_DT[k.dtype], kp, vp, sk, _stream(self._dev)))
 
     def read(self, page_table: torch.Tensor, row0: torch.Tensor, start: torch.Tensor, total: int,
              k: torch.Tensor | None = None, v: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -250,9 +268,10 @@ class Kv8Cache:
         shape = (total, self.KV, self.hd)
         k = torch.empty(shape, dtype=torch.float32, device=self.k.device) if k is None else k
         v = torch.empty_like(k) if v is None else v
-        check(self._read(self._p, n_seq, _i32(page_table, "page_table"), stride, _i32(row0, "row0", (n_seq,)),
-                         _i32(start, "start", (n_seq + 1,)), total, _f32(k, "k", shape), _f32(v, "v", shape),
-                         _stream(self._dev)))
+        dev = self._dev
+        check(self._read(self._p, n_seq, _i32(page_table, "page_table", None, dev), stride, _i32(row0, "row0", (n_seq,), dev),
+                         _i32(start, "start", (n_seq + 1,), dev), total, _f32(k, "k", shape, dev), _f32(v, "v", shape, dev),
+                         _stream(dev)))
         return k, v
 
     def attend(self, q: torch.Tensor, batch: Kv8Batch, score: Score | None = None, out: torch.Tensor | None = None,
@@ -265,9 +284,9 @@ class Kv8Cache:
         if len(shape) != 3:
             raise TlmError(-3, f"q has shape {tuple(shape)}, not [n][H][{self.hd}]")
         n, H = shape[0], shape[1]
-        q, sq, qp = _rows(q, "q", H, self.hd)
-        b = batch._at(n)
-        s = (score or _PLAIN)._at(batch.n_seq, H)
+        q, sq, qp = _rows(q, "q", H, self.hd, self._dev)
+        b = batch._at(n, self._dev)
+        s = (score or _PLAIN)._at(batch.n_seq, H, self._dev)
         dt = _X_DT[q.dtype]
         if out is None:
             out = torch.empty(shape, dtype=q.dtype, device=q.device)
@@ -286,7 +305,8 @@ class Kv8Cache:
                 raise TlmError(-3, f"weights have shape {tuple(weights.shape)}, not [{batch.n_seq}][{self.KV}][rows]")
             w_stride = weights.shape[2]
         st = _stream(self._dev)
-        call = (self._p, b, s, H, dt, qp, sq, _dev(out, "out"), _f32(lse_t, "lse", (n, H)), _f32(weights, "weights"), w_stride)
+        call = (self._p, b, s, H, dt, qp, sq, _ptr(out, "out", self._dev), _f32(lse_t, "lse", (n, H), self._dev),
+                _f32(weights, "weights", None, self._dev), w_stride)
         rc, dev = TLMG_ERANGE, q.device
         if not _capturing():
             w = _scratch.get((self._dev, st)) or _scratch.setdefault((self._dev, st), _Scratch(dev))
@@ -317,7 +337,9 @@ class Kv8Cache:
         from n_keep on, which later tokens add theirs to, are left to the caller
         to clear."""
         d = dst or self
-        n, dev = batch.n_seq, self.k.device
+        n, dev, on = batch.n_seq, self.k.device, self._dev
+        if batch._dev != on or d._dev != on:
+            raise TlmError(-3, f"the cache is on cuda:{on}, the batch on cuda:{batch._dev}, the destination on cuda:{d._dev}")
         if weights.dim() != 3 or weights.shape[:2] != (n, self.KV):
             raise TlmError(-3, f"weights have shape {tuple(weights.shape)}, not [{n}][{self.KV}][rows]")
         if dst_table.dim() != 2 or dst_table.shape[0] != n:
@@ -326,15 +348,14 @@ class Kv8Cache:
             raise TlmError(-3, f"weights_out has shape {tuple(weights_out.shape)}, not [{n}][{self.KV}][rows]")
         rows = torch.empty((n, self.KV, max(n_keep, 0)), dtype=torch.int32, device=dev) if rows is None else rows
         lens = torch.empty((n,), dtype=torch.int32, device=dev) if lens is None else lens
-        st = _stream(self._dev)
-        w = _f32(weights, "weights")
-        r = _i32(rows, "rows", (n, self.KV, n_keep))
-        check(self._select(n, self.KV, batch._c.kv_len, batch.max_kv, w, weights.shape[2], n_keep, sink,
-                                        recent, r, _i32(lens, "lens", (n,)), st))
-        check(self._compact(self._p, d._p, n, batch._c.page_table, batch._c.table_stride,
-                                         batch._c.kv_len, _i32(dst_table, "dst_table"), dst_table.shape[1], r, n_keep, w,
-                                         weights.shape[2], _f32(weights_out, "weights_out"),
-                                         0 if weights_out is None else weights_out.shape[2], st))
+        st = _stream(on)
+        w, r = _f32(weights, "weights", None, on), _i32(rows, "rows", (n, self.KV, n_keep), on)
+        to, wo = _i32(dst_table, "dst_table", None, on), _f32(weights_out, "weights_out", None, on)
+        b = batch._c
+        check(self._select(n, self.KV, b.kv_len, batch.max_kv, w, weights.shape[2], n_keep, sink, recent, r,
+                           _i32(lens, "lens", (n,), on), st))
+        check(self._compact(self._p, d._p, n, b.page_table, b.table_stride, b.kv_len, to, dst_table.shape[1], r, n_keep, w,
+                            weights.shape[2], wo, 0 if weights_out is None else weights_out.shape[2], st))
         return rows, lens
 
 
