@@ -33,8 +33,6 @@
 // precision, and the tensor core's truncating sums stay short.
 #include <algorithm>
 #include <cmath>
-#include <utility>
-#include <vector>
 
 #include "tlmg_dev.cuh"
 #include "tlmg_internal.h"
@@ -686,21 +684,6 @@ __global__ void __launch_bounds__(WG_THREADS) k_kv8_weights(const __grid_constan
         }
     }
     a.weights[((int64_t)s * a.c.KV + kvh) * a.w_stride + t] += sum;
-}
-
-
-bool smem_opt_in(const void *fn, size_t bytes) {
-    static thread_local std::vector<std::pair<const void *, int>> done;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    for (auto &d : done)
-        if (d.first == fn && d.second == dev) return true;
-    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
-        cudaGetLastError();
-        return false;
-    }
-    done.push_back({ fn, dev });
-    return true;
 }
 
 struct Split {

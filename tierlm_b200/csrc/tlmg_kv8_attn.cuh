@@ -1,6 +1,9 @@
 // tlmg_kv8_attn.cuh - arguments of the 8-bit cache's attention kernels.
 #pragma once
 #include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
 
 #include "tlmg_kv8.cuh"
 
@@ -97,6 +100,25 @@ inline int sm_count() {
         dev = d;
     }
     return n;
+}
+
+// Lets a kernel take `bytes` of dynamic shared memory; asked for once a thread and device. Nothing leaves a C call as an
+// exception: without memory for the note it is asked for again.
+inline bool smem_opt_in(const void *fn, size_t bytes) {
+    static thread_local std::vector<std::pair<const void *, int>> done;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    for (auto &d : done)
+        if (d.first == fn && d.second == dev) return true;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    try {
+        done.push_back({ fn, dev });
+    } catch (const std::bad_alloc &) {
+    }
+    return true;
 }
 
 // The form for many query rows (tlmg_kv8_prefill.cu): whether it serves a call, its workspace, and the call.

@@ -47,8 +47,6 @@
 // Every wait is bounded: a role whose wait runs out sets a flag, all roles
 // leave, and the CTA's outputs are NaN.
 #include <cstdint>
-#include <utility>
-#include <vector>
 
 #include "tlmg_dev.cuh"
 #include "tlmg_internal.h"
@@ -1289,20 +1287,6 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
     __syncthreads();
     tc_after();
     if (warp == MW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-}
-
-bool smem_opt_in(const void *fn, size_t bytes) {
-    static thread_local std::vector<std::pair<const void *, int>> done;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    for (auto &d : done)
-        if (d.first == fn && d.second == dev) return true;
-    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
-        cudaGetLastError();
-        return false;
-    }
-    done.push_back({ fn, dev });
-    return true;
 }
 
 // Key tiles of a sequence, and (sequence, KV head) pairs whose images one launch holds; 0 pairs: converting warps. Images
