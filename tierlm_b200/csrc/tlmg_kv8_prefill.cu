@@ -279,7 +279,8 @@ __device__ __forceinline__ uint32_t rest_f16(float x, float y, uint32_t h, float
     return pack_f16((x - f.x) * mul, (y - f.y) * mul);
 }
 
-// softcap * log2(e) * tanh(y) by the exponential
+// softcap * log2(e) * tanh(y) by the exponential. The approximate division and exponential, of 2 units
+// in the last place each, keep it within 2^-20 of the cap: 1 / (1 + e^2y) is at most 1 and no steeper than 1 / 4 in 2y.
 __device__ __forceinline__ float cap_exp(float y, float capl) {
     return __fmaf_rn(-2.0f * capl, __fdividef(1.0f, ex2(y * (2.0f * LOG2E)) + 1.0f), capl);
 }
@@ -967,7 +968,7 @@ __global__ void __launch_bounds__(Role<sizeof(QT) == 4, IMG>::THREADS, 1) k_kv8_
             }
             tc_after();
             const bool part = it.pieces > 1;     // the sums go to the workspace, for the join
-            const float inv = !ok ? __uint_as_float(0x7FC00000u) : part ? unit : l == 0.0f ? 0.0f : __fdividef(unit, l);
+            const float inv = !ok ? __uint_as_float(0x7FC00000u) : part ? unit : l == 0.0f ? 0.0f : __fdiv_rn(unit, l);
             const size_t prow = part ? ((size_t)(blockIdx.x - a.n_full) * RPC + w * TQ + r) : 0;
             // The warp's 32 half rows go through its share of the queries' buffer (their products are done), 16-byte chunks
             // crossed so that neither side meets a bank twice, and out in whole lines: one row a lane, as they lie in TMEM,
