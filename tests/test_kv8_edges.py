@@ -215,6 +215,7 @@ def test_scratch_is_shared_and_bounded():
     out, few = torch.empty_like(q), torch.empty_like(q[:1])
     caches[0].attend(q[:1], one, out=few)
     at = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()      # (earlier tests' peak is not these calls')
     for c in caches:
         c.attend(q[:1], one, out=few)
         c.attend(q, many, out=out)
