@@ -618,7 +618,8 @@ typedef struct {
  * KV * hd; 16-byte aligned rows). Where the first new row continues a block
  * begun earlier, the block's scale becomes max(old, the new rows' d) and
  * its old rows are rounded again from code * old scale. With a position pool
- * the tokens' positions are stored too. */
+ * the tokens' positions are stored too. A page that receives new rows belongs to
+ * one sequence of the batch (others may share the pages before it). */
 int tlmg_kv8_append(const tlmg_kv8 *c, const tlmg_kv8_batch *b, int x_dt, const void *k, const void *v,
                     int64_t x_stride, void *stream);
 
@@ -633,7 +634,11 @@ int tlmg_kv8_read(const tlmg_kv8 *c, int n_seq, const int32_t *page_table, int t
  * |q_pos - k_pos|. A query sees a key iff their documents are the same (doc
  * given: doc[s * doc_stride + position], -1 outside the table) and either
  * k_pos < prefix[s] (prefix given) or all of: causal off or k_pos <= q_pos;
- * window 0 or q_pos - k_pos < window. A query that sees no key returns 0
+ * window 0 or q_pos - k_pos < window. The prefix is that of a prefix-LM mask: every
+ * query sees it whole, also the part that comes after the query. As the first
+ * rows that a window always keeps it serves queries at prefix[s] - 1 and later
+ * (decoding, later chunks); earlier ones of a prompt would see ahead, up to
+ * prefix[s], and go into a call without it. A query that sees no key returns 0
  * with lse -inf. What a masked key's row or scale holds has no effect. */
 typedef struct {
     float scale;                    /* 0: 1 / sqrt(hd) */
@@ -649,8 +654,10 @@ typedef struct {
  * H * hd, 16-byte aligned rows) -> out [total_q][H][hd] of q_dt and, where
  * not NULL, lse f32 [total_q][H] = log sum exp of the visible scores. H is a
  * multiple of KV, at most 16 query heads per KV head. Sums and softmax
- * statistics are f32; f32 queries and probabilities enter the tensor cores
- * as two f16 terms (22 bits), 16-bit ones as one.
+ * statistics are f32 (a tensor core's sums, which truncate, run over at most
+ * 16,384 rows for many 16-bit query rows, 128 for many f32 ones and 32 for few,
+ * and are joined by rounded additions); f32 queries and probabilities enter the
+ * tensor cores as two f16 terms (22 bits), 16-bit ones as one.
  *
  * weights (may be NULL; max_q <= 64): weights[s][kv][row] += the sum of the
  * softmax weights that the call's tokens and the KV head's query heads gave

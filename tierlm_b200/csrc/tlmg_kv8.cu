@@ -5,10 +5,11 @@
 // divisions are IEEE f32 and the rounding is to nearest even, so that codes are
 // a function of the inputs alone. One warp owns one block of K or of V: it takes the maximum
 // over the block's rows, then rounds them in a second pass that finds the
-// rows in L1. All of these kernels move a few bytes per element and are bound
-// by HBM or, for one token per sequence, by the launch: 12,000 bf16 rows of 4
-// heads of 128 in 16.5 us (4.2 TB/s), read back as f32 in 13.5; 64 one-token
-// sequences 8 us, 19 with the call from Python.
+// rows in L1. All of these kernels move a few bytes per element. What bounds them
+// is the chain of dependent loads or, for one token per sequence, the launch: 8,511
+// bf16 rows of 4 heads of 128 in 14 us (26 MB, 1.9 TB/s: the rows of a block come
+// twice, the maximum between), read back as f32 in 11 (44 MB, 4.0 TB/s); 64
+// one-token sequences 2.7 us, 9 with the call from Python.
 #include <algorithm>
 
 #include "tlmg_dev.cuh"
@@ -219,8 +220,8 @@ __device__ __forceinline__ uint32_t ld_cluster(const uint32_t *p, uint32_t rank)
 // digit in every CTA's part, summed over the cluster), then one ordered pass
 // writes the rows above it and as many rows equal to it, lowest first, as m
 // leaves. Latency-bound: the weights are 4 bytes a row; 32,768 rows took 61 us
-// with one CTA a head, 27 with a cluster of 8 (three passes, each with two
-// cluster barriers).
+// with one CTA a head, 27 with a cluster of 8 (three passes with a cluster barrier
+// each, and two more barriers after them).
 template <int CS>
 __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_t *__restrict__ kv_len, int max_kv,
                                                             const float *__restrict__ weights, int64_t w_stride,
@@ -349,7 +350,10 @@ __global__ void __launch_bounds__(SEL_THREADS) k_kv8_select(int KV, const int32_
 }
 
 // One warp per (destination block, KV head, K or V). Kept rows lie apart, so
-// that every row is two lines of its own: 4 heads x 4,096 rows in 11 us.
+// that every row is two lines of its own: 4 heads x 4,096 rows of 128 in 11 us.
+// Blocks of more than 32 rows, or than the registers hold, go over their rows
+// twice (32,768 rows of 64 to 4,096, with the selection and the read-back: 44 us in
+// blocks of 32, 50 in blocks of 64).
 template <int FS, int FD>
 __global__ void __launch_bounds__(32 * AP_WARPS) k_kv8_compact(const Kv8View c, const Kv8View d, const int32_t *__restrict__ table,
                                                                int stride, const int32_t *__restrict__ kv_len,

@@ -9,7 +9,7 @@
 // MMA, maximum, exponential, MMA of a tile (about 950 instructions for 32 rows)
 // at the 8 to 12 warps that the registers allow: issue 41 %, HBM 41 %. One f32 query over 131,071 int8 rows
 // of 4 heads of 128 takes 49 us (2.7 TB/s), 64 bf16 ones over 1 .. 8,192 e4m3
-// rows 101 us (2.7 TB/s).
+// rows 102 us (2.7 TB/s).
 //
 // Products run on mma.sync.m16n8k16 (f16 in, f32 out): the query rows of a
 // group (1 .. 16) are below the 64-row minimum of tcgen05.mma, and at the HBM

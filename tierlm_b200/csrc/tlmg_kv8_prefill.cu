@@ -4,7 +4,7 @@
 // out = sum_t p_t v_t / sum_t p_t with p_t = 2^(score_t - reference): 4 hd flops a visible pair, so the tensor core is
 // the floor (2,048 clocks a key tile of 256 rows at hd 128). What is reached is set by the way from a tile's scores to its
 // weights: 2,600 clocks of softmax and 1,700 of MMAs and signals, half of each under the other tile's. 65,536 rows x 2,048
-// tokens x 32 heads of 128: 2,070 us, 1,046 TFLOP/s; a chunk of 2,048 on 16,384 rows 642 us, with a soft cap 1,046.
+// tokens x 32 heads of 128: 2,055 us, 1,053 TFLOP/s; a chunk of 2,048 on 16,384 rows 642 us, with a soft cap 1,046.
 //
 // 16-bit queries: one CTA per SM takes 256 query rows (token, head of the
 // group) of one KV head in two tiles A and B of 128, and walks the visible keys
@@ -1428,7 +1428,10 @@ template <int HD> int launch_fmt(const Kv8Attn &a, int q_dt, void *work, cudaStr
 bool kv8_prefill_serves(const tlmg_kv8 &c, const tlmg_kv8_batch &b, int H) {
     // 32 heads on 4 of 128, a call as Python makes it: 16 tokens over 701 / 2,048 / 8,192 / 131,072 rows take 36 / 43 / 49 /
     // 135 us here and 20 / 25 / 40 / 318 us in the kernel for few rows; 32 tokens over 2,048 / 8,192 rows 51 / 57 and 32 / 64,
-    // 64 tokens over 2,048 rows 51 and 45. The two meet where rows x keys x dims of all heads come to WIDE_WORK.
+    // 64 tokens over 2,048 rows 51 and 45. The two meet where rows x keys x dims of all heads come to WIDE_WORK. Other
+    // layouts (8 on 2, 64 on 4; dims 64 and 128; f32 and bf16; 701 .. 131,072 rows) meet between half of it and it for one
+    // sequence: at 2/3 of it 34 .. 51 us here and 29 .. 43 there, at 4/3 39 .. 60 and 49 .. 76. Batches of short sequences
+    // meet at a fourth of it (8 x 32 tokens over 701 rows, 32 on 4 of 128, 0.9 of it: 35 here, 70 there).
     constexpr int64_t WIDE_WORK = (int64_t)3 << 28;
     const int64_t rows = (int64_t)b.max_q * (H / c.KV);
     return c.hd <= 128 && rows >= TQ && (double)rows * c.KV * b.n_seq * b.max_kv * c.hd >= (double)WIDE_WORK;

@@ -171,8 +171,10 @@ class Kv8Batch:
 class Score:
     """How scores are formed and masked (tlmg_kv8_score): softcap c > 0:
     c * tanh(z / c); slopes f32 [H]: minus slopes[h] * distance; causal,
-    window, prefix int32 [n_seq] (rows below it stay visible) and doc int32
-    [n_seq][positions] (other documents are masked). scale 0: 1 / sqrt(hd)."""
+    window, prefix int32 [n_seq] (positions below it are visible to every
+    token, those ahead of it included: a prefix-LM mask; the first rows that a
+    window keeps only for tokens behind them) and doc int32 [n_seq][positions]
+    (other documents are masked). scale 0: 1 / sqrt(hd)."""
     scale: float = 0.0
     softcap: float = 0.0
     slopes: torch.Tensor | None = None
